@@ -484,6 +484,89 @@ int qqt_mlp_train_backward(const void *pack, int32_t n_rows, int32_t k_in, const
                            void *work, qqt_stream_t stream);
 uint64_t qqt_mlp_train_work_bytes(int32_t n_rows);
 
+/* ---- Training operators: layer norm, gated recurrence, policy loss ----
+ * Element types of their large operands; parameters, states, statistics and
+ * per-row values are float32.  Rows and sequences have a unit innermost
+ * stride; the other strides are in elements.  Null pointers mark what an
+ * entry point says is optional.  Sizes of zero are no error. */
+enum { QQT_F32 = 0, QQT_F16 = 1, QQT_BF16 = 2 };
+
+/* Layer norm of rows of d values (the norms of train/model.py:77-101 and
+ * 140-153 on their own): y [rows][d] = (x - mean) rstd w + b (b optional);
+ * mean, rstd [rows] (optional) are what the backward call reads. */
+int qqt_layernorm_forward(const void *x, int32_t dtype, int64_t rows, int64_t d, int64_t x_stride,
+                          const float *w, const float *b, float eps, void *y, float *mean,
+                          float *rstd, qqt_stream_t stream);
+/* dx [rows][d], dw [d] and db [d] (each optional) for dy rows of dy_stride;
+ * work = qqt_layernorm_work_bytes(rows, d) bytes, needed for dw or db. */
+int qqt_layernorm_backward(const void *dy, int64_t dy_stride, const void *x, int64_t x_stride,
+                           int32_t dtype, int64_t rows, int64_t d, const float *mean,
+                           const float *rstd, const float *w, void *dx, float *dw, float *db,
+                           void *work, qqt_stream_t stream);
+uint64_t qqt_layernorm_work_bytes(int64_t rows, int64_t d);
+
+/* One (T, N, D) sequence operand: address and element strides of t and n. */
+typedef struct QqtSeq {
+  const void *p;
+  int64_t t_stride, n_stride;
+} QqtSeq;
+
+/* Gated linear recurrence over T ticks of N sequences:
+ *   f = sigmoid(gate_t), h_t = f k_t h_{t-1} + (1 - f) x_t, k_t = !reset_t
+ * x, gate -> h of type dtype; reset (optional) uint8 (T, N); h0 (optional,
+ * zero) and h_last (optional) [N][D]; carry (optional) [qqt_recurrence_chunks(T)]
+ * [N][D], the states that the backward call reads; work =
+ * qqt_recurrence_work_bytes(T, N, D) bytes. */
+int qqt_recurrence_forward(const QqtSeq *x, const QqtSeq *gate, const QqtSeq *reset,
+                           const float *h0, int32_t dtype, int64_t T, int64_t N, int64_t D,
+                           const QqtSeq *h, float *h_last, float *carry, void *work,
+                           qqt_stream_t stream);
+/* dx, dgate (type dtype) and dh0 (optional) [N][D] for dh (optional) and
+ * dh_last (optional) [N][D]. */
+int qqt_recurrence_backward(const QqtSeq *dh, const float *dh_last, const QqtSeq *x,
+                            const QqtSeq *gate, const QqtSeq *reset, const float *carry,
+                            int32_t dtype, int64_t T, int64_t N, int64_t D, const QqtSeq *dx,
+                            const QqtSeq *dgate, float *dh0, void *work, qqt_stream_t stream);
+int64_t qqt_recurrence_chunks(int64_t T);
+uint64_t qqt_recurrence_work_bytes(int64_t T, int64_t N, int64_t D);
+
+/* Clipped policy loss with a KL term and an entropy bonus over masked
+ * categorical heads (train/ppo.py:397-424, train/model.py:216-256):
+ *   r = exp(logp - old_logp), q = ref_logp - logp
+ *   loss = mean over rows with mask of
+ *          -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+ *          + kl_coef (exp(q) - 1 - q) - entropy_coef H
+ * logits [rows] of row_stride, split into n_heads segments of width[h];
+ * legal (optional) uint8 rows of legal_stride; actions int64 [n_heads] per
+ * row; mask (optional) uint8 [rows]; ref_logp optional.  A row none of whose
+ * categories in some head is legal, or whose action is not, has logp -inf
+ * and adds nothing to the sums or the gradient; an action outside its head
+ * raises QQT_DEV_BAD_ACTION.  Outputs, each optional: logp, entropy [rows];
+ * stats [5] = loss and the means of policy term, KL, entropy and clipped
+ * share; dlogits rows of dlogits_stride = grad_scale upstream[0] dloss/dlogits
+ * (upstream optional, 1).  Without stats and dlogits, old_logp .. mask and
+ * work are not read.  work = qqt_policy_loss_work_bytes(rows) bytes. */
+#define QQT_MAX_HEADS 8
+typedef struct QqtPolicyLoss {
+  const void *logits;
+  int64_t row_stride, rows;
+  const uint8_t *legal;
+  int64_t legal_stride;
+  const int64_t *actions;
+  int64_t action_stride;
+  const float *old_logp, *adv, *ref_logp;
+  const uint8_t *mask;
+  const float *upstream;
+  float *logp, *entropy, *stats;
+  void *dlogits;
+  int64_t dlogits_stride;
+  void *work;
+  float clip_low, clip_high, kl_coef, entropy_coef, grad_scale;
+  int32_t dtype, n_heads, width[QQT_MAX_HEADS];
+} QqtPolicyLoss;
+int qqt_policy_loss(const QqtPolicyLoss *args, qqt_stream_t stream);
+uint64_t qqt_policy_loss_work_bytes(int64_t rows);
+
 /* Device error word: returns the accumulated QQT_DEV_* bits and clears
  * them (synchronises the device). */
 int qqt_get_error(uint32_t *code_out);

@@ -7,4 +7,7 @@
 #include "policy_cnn.cu"
 #include "train_gae.cu"
 #include "train_mlp.cu"
+#include "layer_norm.cu"
+#include "recurrence.cu"
+#include "policy_loss.cu"
 #include "phase_stamps.cu"

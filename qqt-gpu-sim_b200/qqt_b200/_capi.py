@@ -83,6 +83,24 @@ class QqtStepOut(ctypes.Structure):
                 ("hit", c_p)]
 
 
+class QqtSeq(ctypes.Structure):
+    _fields_ = [("p", c_p), ("t_stride", c_i64), ("n_stride", c_i64)]
+
+
+MAX_HEADS = 8
+
+
+class QqtPolicyLoss(ctypes.Structure):
+    _fields_ = [("logits", c_p), ("row_stride", c_i64), ("rows", c_i64), ("legal", c_p),
+                ("legal_stride", c_i64), ("actions", c_p), ("action_stride", c_i64),
+                ("old_logp", c_p), ("adv", c_p), ("ref_logp", c_p), ("mask", c_p),
+                ("upstream", c_p), ("logp", c_p), ("entropy", c_p), ("stats", c_p),
+                ("dlogits", c_p), ("dlogits_stride", c_i64), ("work", c_p),
+                ("clip_low", c_f32), ("clip_high", c_f32), ("kl_coef", c_f32),
+                ("entropy_coef", c_f32), ("grad_scale", c_f32), ("dtype", c_i32),
+                ("n_heads", c_i32), ("width", c_i32 * MAX_HEADS)]
+
+
 _lib = None
 
 
@@ -137,6 +155,20 @@ def lib():
             "qqt_mlp_train_backward": (c_i32, [c_p, c_i32, c_i32, c_p, c_p, c_p, c_i32, c_p,
                                                c_i32, c_p, c_i32, c_p, c_p, c_p, c_p, c_p]),
             "qqt_mlp_train_work_bytes": (c_u64, [c_i32]),
+            "qqt_layernorm_forward": (c_i32, [c_p, c_i32, c_i64, c_i64, c_i64, c_p, c_p, c_f32, c_p,
+                                              c_p, c_p, c_p]),
+            "qqt_layernorm_backward": (c_i32, [c_p, c_i64, c_p, c_i64, c_i32, c_i64, c_i64, c_p,
+                                               c_p, c_p, c_p, c_p, c_p, c_p, c_p]),
+            "qqt_layernorm_work_bytes": (c_u64, [c_i64, c_i64]),
+            "qqt_recurrence_forward": (c_i32, [P(QqtSeq), P(QqtSeq), P(QqtSeq), c_p, c_i32, c_i64,
+                                               c_i64, c_i64, P(QqtSeq), c_p, c_p, c_p, c_p]),
+            "qqt_recurrence_backward": (c_i32, [P(QqtSeq), c_p, P(QqtSeq), P(QqtSeq), P(QqtSeq),
+                                                c_p, c_i32, c_i64, c_i64, c_i64, P(QqtSeq),
+                                                P(QqtSeq), c_p, c_p, c_p]),
+            "qqt_recurrence_chunks": (c_i64, [c_i64]),
+            "qqt_recurrence_work_bytes": (c_u64, [c_i64, c_i64, c_i64]),
+            "qqt_policy_loss": (c_i32, [P(QqtPolicyLoss), c_p]),
+            "qqt_policy_loss_work_bytes": (c_u64, [c_i64]),
             "qqt_get_error": (c_i32, [P(ctypes.c_uint32)]),
             "qqt_phase_read": (c_i32, [c_p, ctypes.c_uint32, P(ctypes.c_uint32)]),
             "qqt_phase_reset": (c_i32, []),
@@ -183,6 +215,29 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def stream_ptr(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def need(ok: bool, what: str, exc=ValueError) -> None:
+    """Argument check of the training operators."""
+    if not ok:
+        raise exc(what)
+
+
+def need_cuda(*tensors) -> None:
+    """All given tensors (None allowed) on one CUDA device, the current one
+    (kernels launch on its current stream)."""
+    dev = tensors[0].device
+    if dev.type != "cuda":
+        raise ValueError(f"tensors must be on a CUDA device, got {dev}")
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+    if dev.index != torch.cuda.current_device():
+        raise ValueError(f"tensors on {dev}, but the current device is "
+                         f"cuda:{torch.cuda.current_device()}")
 
 
 def device_error() -> int:
