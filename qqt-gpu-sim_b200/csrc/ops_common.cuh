@@ -41,6 +41,33 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
+// VEC consecutive elements, moved by one access of their whole size.
+template <class T, int VEC>
+struct alignas(sizeof(T) * VEC) Vec {
+  T v[VEC];
+};
+template <class T, int VEC>
+__device__ __forceinline__ Vec<T, VEC> ld_vec(const T* p) {
+  return *reinterpret_cast<const Vec<T, VEC>*>(p);
+}
+template <class T, int VEC>
+__device__ __forceinline__ void st_vec(T* p, const Vec<T, VEC>& x) {
+  *reinterpret_cast<Vec<T, VEC>*>(p) = x;
+}
+static inline bool aligned_to(const void* p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+
+// 2^x and 1/x by the special-function unit (relative errors of about 2^-22).
+__device__ __forceinline__ float ex2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // Maximum that keeps a NaN (fmaxf drops it).
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
