@@ -41,18 +41,97 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
-// VEC consecutive elements, moved by one access of their whole size.
+// VEC consecutive elements, moved by one access of their whole size; 16-bit
+// elements stay packed in 32-bit words (a word a pair) until they are read.
 template <class T, int VEC>
-struct alignas(sizeof(T) * VEC) Vec {
-  T v[VEC];
+struct alignas(sizeof(T) * VEC) Vec;
+template <int VEC>
+struct alignas(4 * VEC) Vec<float, VEC> {
+  float v[VEC];
+  __device__ __forceinline__ float get(int j) const { return v[j]; }
+  __device__ __forceinline__ void put(const float* f) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = f[j];
+  }
+};
+template <>
+struct alignas(2) Vec<__half, 1> {
+  __half v;
+  __device__ __forceinline__ float get(int) const { return __half2float(v); }
+  __device__ __forceinline__ void put(const float* f) { v = __float2half_rn(f[0]); }
+};
+template <>
+struct alignas(2) Vec<__nv_bfloat16, 1> {
+  __nv_bfloat16 v;
+  __device__ __forceinline__ float get(int) const { return __bfloat162float(v); }
+  __device__ __forceinline__ void put(const float* f) { v = __float2bfloat16_rn(f[0]); }
+};
+template <int VEC>
+struct alignas(2 * VEC) Vec<__half, VEC> {
+  uint32_t w[VEC / 2];
+  __device__ __forceinline__ float get(int j) const {
+    const __half2 h = *reinterpret_cast<const __half2*>(&w[j / 2]);
+    return j & 1 ? __high2float(h) : __low2float(h);
+  }
+  __device__ __forceinline__ void put(const float* f) {
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) {
+      const __half2 h = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+      w[j] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+};
+template <int VEC>
+struct alignas(2 * VEC) Vec<__nv_bfloat16, VEC> {
+  uint32_t w[VEC / 2];
+  __device__ __forceinline__ float get(int j) const {   // a bfloat16 is a float's upper half
+    return __uint_as_float(j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+  }
+  __device__ __forceinline__ void put(const float* f) {
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
+      w[j] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+};
+// The access of that size: a vector type, so that a pair of 16-bit elements
+// is not taken apart into two registers by the load.
+template <int BYTES>
+struct Word;
+template <>
+struct Word<2> {
+  using type = unsigned short;
+};
+template <>
+struct Word<4> {
+  using type = unsigned;
+};
+template <>
+struct Word<8> {
+  using type = uint2;
+};
+template <>
+struct Word<16> {
+  using type = uint4;
 };
 template <class T, int VEC>
 __device__ __forceinline__ Vec<T, VEC> ld_vec(const T* p) {
-  return *reinterpret_cast<const Vec<T, VEC>*>(p);
+  using W = typename Word<sizeof(T) * VEC>::type;
+  const W w = *reinterpret_cast<const W*>(p);
+  return *reinterpret_cast<const Vec<T, VEC>*>(&w);
 }
 template <class T, int VEC>
 __device__ __forceinline__ void st_vec(T* p, const Vec<T, VEC>& x) {
-  *reinterpret_cast<Vec<T, VEC>*>(p) = x;
+  using W = typename Word<sizeof(T) * VEC>::type;
+  *reinterpret_cast<W*>(p) = *reinterpret_cast<const W*>(&x);
+}
+template <class T, int VEC>
+__device__ __forceinline__ Vec<T, VEC> vec_zero() {
+  Vec<T, VEC> x;
+  const float z[VEC] = {};
+  x.put(z);
+  return x;
 }
 static inline bool aligned_to(const void* p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 

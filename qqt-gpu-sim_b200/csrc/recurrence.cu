@@ -6,45 +6,64 @@
 //   e_t = dh_t + f_{t+1} k_{t+1} e_{t+1}      (+ dh_last at the last tick)
 //   dx_t = (1 - f) e_t,   dgate_t = f (1 - f) e_t (k h_{t-1} - x_t)
 //   dh0 = f_1 k_1 e_1
-// States are float32 whatever the type of the sequence.  The backward pass
-// recomputes them from the state entering every kRecChunk ticks, which the
-// forward pass saves in float32: rounded outputs are not read back.
+// States are float32 whatever the type of the sequence.  The forward pass
+// saves the state entering every kRecU ticks in float32 (half a byte per
+// element and tick); the backward pass starts from it, so rounded outputs are
+// not read back and gates are computed once.
 //
-// A stretch of ticks acts on the state as h -> A h + B, and on the gradient
-// that leaves it downwards as g -> A g + B', with the same A.  A block takes
-// a tile of kRecChunk ticks of 32 x VEC channels ((n, d) pairs); each of its
-// warps holds U ticks in registers and reduces them to (A, B), one thread per
-// channel composes the warps' pairs with the state that enters the tile, and
-// the warps then finish from the state that enters theirs.  A stretch that
-// holds a reset has A = -0 (products of gates are +0 or more): the state
-// entering it is dropped by a select, whatever it is.
-//
-// Two ways to get a tile's incoming state:
-//  * enough channels to fill the GPU: a block walks its channels' tiles along
-//    T, the next tile's loads issued before the present one is finished;
-//  * few channels, many ticks: one block per tile, in the order of a ticket.
-//    Tile k publishes its (A, B) at once; its incoming state is the one that
-//    entered its group of kRecGroup tiles, published by the last tile of the
-//    group before, composed with the pairs of the group's tiles before k --
-//    always in that order, so results do not depend on timing.  A tile waits
-//    only on tiles with smaller tickets, and only for kRecPolls polls.
+// A thread walks its VEC channels ((n, d) pairs) along time, the loads of the
+// tick kRecU later issued as soon as a tick is consumed.  Where the channels
+// do not fill the GPU, time is cut into segments, and a thread walks one of
+// them: a stretch of ticks acts on the state as h -> A h + B, and on the
+// gradient that passes down through it as g -> A g + G, with the same A.  A
+// first kernel finds each segment's pair (k_rec_sum), a second what enters
+// each segment, one after the other (k_rec_join), and then every segment is
+// walked from there: inputs are read twice, no block waits for another, and
+// the order of all sums is fixed by the sizes.  A stretch that holds a reset
+// has A = -0 (products of gates are +0 or more): what enters it is dropped by
+// a select, whatever it is.
 
 #include "ops_common.cuh"
 
 namespace qqt {
 
-constexpr int kRecChunk = 64;
-constexpr int kRecGroup = 32;
-constexpr uint32_t kRecPolls = 1u << 22;
+constexpr int kRecU = 8;                     // ticks a thread holds, and between saved states
+constexpr int kSeqThreads = 128;
+// Blocks of an SM that the registers are cut for.  16-bit forward walks take 4
+// channels a thread, backward ones 2: 8 ticks of 4 channels' states and
+// operands do not fit 128 registers (213 against 340 us measured at 128 ticks
+// x 5632 x 128).
+constexpr int kFwdBlocks = 6, kBwdBlocks = 4;
+// Channel walks wanted per SM before time is cut: 3072 against 1024 measured
+// 140 against 368 us at 65536 ticks x 1024 channels, and within 2 % of 4096.
+constexpr int64_t kRecWalks = 3072;
 
-// f = sigmoid(g) and i = 1 - f = sigmoid(-g), each to float32 accuracy: with
-// e = exp(-|g|) the larger of the two is 1/(1+e) and the smaller e/(1+e).
-__device__ __forceinline__ void gates(float g, float& f, float& i) {
-  const float e = expf(-fabsf(g));
-  const float big = rcp_approx(1.f + e);
-  const float small = e * big;
-  f = g < 0.f ? small : big;
-  i = g < 0.f ? big : small;
+// f = sigmoid(g) and i = 1 - f = sigmoid(-g), each to a few units of its own
+// last place: e = exp(-g), f = 1 / (1 + e), i = e f.  e = 2^(-g log2 e) carries
+// the rounding of that product, |g| 2^-25 of itself; 32-bit sequences add the
+// product's lost part back.  The exponent stops at 125, where f is 2^-125 and
+// i is 1; a NaN passes.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+template <class T>
+__device__ __forceinline__ void gates(float gate, float& f, float& i) {
+  constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+  float e;
+  if constexpr (sizeof(T) == 4) {
+    const float g = max_nan(min_nan(gate, 120.f), -86.f);
+    const float p = g * kLog2e;
+    // g log2 e - p: the product's rounding and log2 e's own tail
+    const float lost = fmaf(g, 1.9259629911e-8f, fmaf(g, kLog2e, -p));
+    e = ex2_approx(-p);
+    e = fmaf(e, -kLn2 * lost, e);
+  } else {
+    e = ex2_approx(min_nan(gate * -kLog2e, 125.f));
+  }
+  f = rcp_approx(1.f + e);
+  i = e * f;
 }
 
 __device__ __forceinline__ bool drops(float a) { return __float_as_int(a) < 0; }
@@ -62,19 +81,20 @@ struct RecArgs {
   RecSeq dx, dg;
   const float* s0;                 // h0 or dh_last
   float* s_end;                    // h_last or dh0
-  float* carry;                    // state entering every kRecChunk ticks
-  int64_t nT, nN, nD;
-  unsigned long long* agg;         // [tiles][channels] (A, B), all ones before they are known
-  unsigned* group_in;              // [groups][channels] state entering a group, ditto
-  unsigned* ticket;                // -1 at first
+  float* carry;                    // [ticks / kRecU rounded up][channels] states
+  int64_t nT;
+  uint32_t nC, nD;                 // channels (N D) and D
+  int64_t seg;                     // ticks of a segment, a multiple of kRecU
+  float2* pair;                    // [segments][channels] (A, B or G)
+  float* enters;                   // [segments][channels] what enters each; null with one segment
 };
 
 // One tick for every channel: what acting does.
 template <class T, int VEC>
 __global__ void k_rec_step(RecArgs a) {
-  const int64_t c = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * VEC;
-  if (c >= a.nN * a.nD) return;
-  const int64_t n = c / a.nD, d = c % a.nD;
+  const uint32_t c = (blockIdx.x * blockDim.x + threadIdx.x) * VEC;
+  if (c >= a.nC) return;
+  const int64_t n = c / a.nD, d = c - (uint32_t)n * a.nD;
   const auto x = ld_vec<T, VEC>((const T*)a.x.p + n * a.x.ns + d);
   const auto g = ld_vec<T, VEC>((const T*)a.g.p + n * a.g.ns + d);
   Vec<float, VEC> s;
@@ -88,349 +108,403 @@ __global__ void k_rec_step(RecArgs a) {
 #pragma unroll
   for (int v = 0; v < VEC; ++v) {
     float f, i;
-    gates(to_f(g.v[v]), f, i);
-    s.v[v] = fmaf(f, s.v[v], i * to_f(x.v[v]));
-    o.v[v] = from_f<T>(s.v[v]);
+    gates<T>(g.get(v), f, i);
+    s.v[v] = fmaf(f, s.v[v], i * x.get(v));
   }
+  o.put(s.v);
   st_vec((T*)a.h.p + n * a.h.ns + d, o);
   if (a.s_end) st_vec(a.s_end + c, s);
 }
 
-// The gates' resets of this thread's U ticks as a bit mask.
-template <int U>
-__device__ __forceinline__ unsigned load_resets(const RecSeq& r, int64_t n, bool one_n, int64_t t0,
-                                                int64_t nT) {
-  if (!r.p) return 0;
-  const uint8_t* p = (const uint8_t*)r.p + n * r.ns;
-  unsigned m = 0;
-  if (one_n) {                      // the whole warp follows one sequence
+// Where a thread's VEC channels are: of sequence n from d on.  A thread past
+// the last channel reads the last ones and stores nothing.
+struct RecPlace {
+  uint32_t c;
+  int64_t n, d;
+  bool on, one_n;                  // one_n: the whole warp follows one sequence
+};
+template <int VEC>
+__device__ __forceinline__ RecPlace rec_place(const RecArgs& a, uint32_t c) {
+  RecPlace p;
+  p.on = c < a.nC;
+  p.c = p.on ? c : a.nC - VEC;
+  const uint32_t n = p.c / a.nD;
+  p.n = n;
+  p.d = p.c - n * a.nD;
+  p.one_n = __shfl_sync(QQT_FULL, n, 0) == __shfl_sync(QQT_FULL, n, 31);
+  return p;
+}
+template <class T>
+__device__ __forceinline__ T* at(const RecSeq& s, const RecPlace& p, int64_t t) {
+  return (T*)s.p + p.n * s.ns + p.d + t * s.ts;
+}
+
+// The resets of kRecU ticks from t0 as a bit mask per lane.
+__device__ __forceinline__ unsigned load_resets(const RecArgs& a, const RecPlace& p, int64_t t0) {
+  if (!a.reset.p) return 0;
+  const uint8_t* r = (const uint8_t*)a.reset.p + p.n * a.reset.ns;
+  if (p.one_n) {
     const int64_t t = t0 + lane_id();
-    m = __ballot_sync(QQT_FULL, lane_id() < U && t < nT && p[t * r.ts]);
-  } else {
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (t0 + u < nT && p[(t0 + u) * r.ts]) m |= 1u << u;
+    return __ballot_sync(QQT_FULL, lane_id() < kRecU && t < a.nT && r[t * a.reset.ts]);
   }
+  unsigned m = 0;
+#pragma unroll
+  for (int u = 0; u < kRecU; ++u)
+    if (t0 + u < a.nT && r[(t0 + u) * a.reset.ts]) m |= 1u << u;
   return m;
 }
 
-template <class T, int VEC, int U>
-__device__ __forceinline__ void load_ticks(const RecSeq& s, int64_t off, int64_t t0, int64_t nT,
-                                           bool on, Vec<T, VEC>* out) {
-  const T* p = (const T*)s.p + off + t0 * s.ts;
+template <class T, int VEC>
+__device__ __forceinline__ void load_ticks(const T* p, int64_t ts, int n, Vec<T, VEC>* out) {
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    if (on && t0 + u < nT) {
-      out[u] = ld_vec<T, VEC>(p);
-    } else {
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) out[u].v[v] = from_f<T>(0.f);
-    }
-    p += s.ts;
+  for (int u = 0; u < kRecU; ++u, p += ts)
+    if (u < n) out[u] = ld_vec<T, VEC>(p);
+}
+
+// ------------------------------------------------------ walking along time
+
+template <class T, int VEC>
+__global__ void __launch_bounds__(kSeqThreads, kFwdBlocks) k_rec_seq_fwd(RecArgs a) {
+  const RecPlace p = rec_place<VEC>(a, (blockIdx.x * kSeqThreads + threadIdx.x) * VEC);
+  const int64_t first = blockIdx.y * a.seg;
+  const int64_t ticks = a.nT - first < a.seg ? a.nT - first : a.seg;
+  const T *xp = at<T>(a.x, p, first), *gp = at<T>(a.g, p, first);
+  T* hp = at<T>(a.h, p, first);
+  const float* from = a.enters ? a.enters + (int64_t)blockIdx.y * a.nC : a.s0;
+  Vec<float, VEC> s = from ? ld_vec<float, VEC>(from + p.c) : vec_zero<float, VEC>();
+  float* cp = a.carry ? a.carry + first / kRecU * a.nC + p.c : nullptr;
+  const int64_t full = ticks / kRecU;
+  const int rem = (int)(ticks % kRecU);
+  Vec<T, VEC> x[kRecU], g[kRecU];
+  if (full > 0) {
+    load_ticks<T, VEC>(xp, a.x.ts, kRecU, x);
+    load_ticks<T, VEC>(gp, a.g.ts, kRecU, g);
   }
-}
-
-__device__ __forceinline__ unsigned long long ld_poll64(const unsigned long long* p) {
-  unsigned long long v;
-  asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
-  return v;
-}
-__device__ __forceinline__ unsigned ld_poll32(const unsigned* p) {
-  unsigned v;
-  asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-  return v;
-}
-__device__ __forceinline__ void st_pub64(unsigned long long* p, unsigned long long v) {
-  asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
-}
-__device__ __forceinline__ void st_pub32(unsigned* p, unsigned v) {
-  asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
-}
-
-// The state entering tile k of channel c (tiles counted along the scan's own
-// direction), composed in a fixed order from what earlier tiles published.
-// Every value carries its own validity: no arithmetic result is all ones (a
-// NaN comes out of the units as 0x7fffffff).
-__device__ __forceinline__ float state_entering(const RecArgs& a, int64_t k, int64_t c, int64_t nC,
-                                                float s0) {
-  const int64_t grp = k / kRecGroup;
-  const int64_t first = grp * kRecGroup;
-  float s = s0;
-  bool late = false;
-  constexpr int B = 16;
-  for (int64_t q = first; q < k; q += B) {
-    unsigned long long v[B];
-#pragma unroll
-    for (int j = 0; j < B; ++j) v[j] = q + j < k ? ld_poll64(a.agg + (q + j) * nC + c) : 0;
-    if (q == first && grp > 0) {
-      unsigned w = ld_poll32(a.group_in + grp * nC + c);
-      for (uint32_t i = 0; w == 0xffffffffu && i < kRecPolls; ++i)
-        w = ld_poll32(a.group_in + grp * nC + c);
-      late |= w == 0xffffffffu;
-      s = __uint_as_float(w);
+  unsigned rst = load_resets(a, p, first);
+  for (int64_t b = 0; b < full; ++b) {
+    const bool more = b + 1 < full;
+    const unsigned rst_next = load_resets(a, p, first + (b + 1) * kRecU);
+    if (cp) {
+      if (p.on) st_vec(cp, s);
+      cp += a.nC;
     }
+    xp += kRecU * a.x.ts;
+    gp += kRecU * a.g.ts;
+    const T *xn = xp, *gn = gp;
 #pragma unroll
-    for (int j = 0; j < B; ++j) {
-      if (q + j < k) {
-        for (uint32_t i = 0; v[j] == ~0ull && i < kRecPolls; ++i)
-          v[j] = ld_poll64(a.agg + (q + j) * nC + c);
-        late |= v[j] == ~0ull;
-        s = through(__uint_as_float((unsigned)(v[j] >> 32)), __uint_as_float((unsigned)v[j]), s);
+    for (int u = 0; u < kRecU; ++u) {
+      if ((rst >> u) & 1) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) s.v[v] = 0.f;
       }
-    }
-  }
-  if (k == first && grp > 0) {
-    unsigned w = ld_poll32(a.group_in + grp * nC + c);
-    for (uint32_t i = 0; w == 0xffffffffu && i < kRecPolls; ++i)
-      w = ld_poll32(a.group_in + grp * nC + c);
-    late |= w == 0xffffffffu;
-    s = __uint_as_float(w);
-  }
-  if (late) flag_error(QQT_DEV_TIMEOUT);
-  return s;
-}
-
-// Tile (k, channel group) of this block: its ticket in split mode.
-__device__ __forceinline__ int64_t take_ticket(unsigned* ticket) {
-  __shared__ unsigned mine;
-  if (threadIdx.x == 0) mine = atomicAdd(ticket, 1u) + 1u;
-  __syncthreads();
-  return mine;
-}
-
-template <class T, int VEC, int U, bool SPLIT>
-__global__ void __launch_bounds__(kRecChunk / U * 32, U == 8 ? 2 : 1) k_rec_fwd(RecArgs a) {
-  constexpr int W = kRecChunk / U, CH = 32 * VEC;
-  __shared__ float sA[W][CH], sB[W][CH];
-  const int warps = blockDim.x >> 5, w = warp_id(), lane = lane_id();
-  const int64_t nC = a.nN * a.nD, nG = (nC + CH - 1) / CH;
-  const int64_t nK = (a.nT + kRecChunk - 1) / kRecChunk;
-  int64_t k = 0, grp = blockIdx.x;
-  if (SPLIT) {
-    const int64_t tk = take_ticket(a.ticket);
-    k = tk / nG;
-    grp = tk % nG;
-  }
-  const int64_t c = grp * CH + lane * VEC;
-  const bool on = c < nC;
-  const int64_t n = on ? c / a.nD : 0, d = on ? c % a.nD : 0;
-  const bool one_n = __shfl_sync(QQT_FULL, (int)n, 0) == __shfl_sync(QQT_FULL, (int)n, 31) &&
-                     __all_sync(QQT_FULL, on);
-  // thread-per-channel part
-  const int64_t cc = grp * CH + threadIdx.x;
-  const bool mine = threadIdx.x < CH && cc < nC;
-  float s = 0.f;
-  // (a block of fewer than CH threads -- few ticks -- strides over its channels)
-  Vec<T, VEC> x[U], g[U];
-  int64_t t0 = k * kRecChunk + w * U;
-  load_ticks<T, VEC, U>(a.x, n * a.x.ns + d, t0, a.nT, on, x);
-  load_ticks<T, VEC, U>(a.g, n * a.g.ns + d, t0, a.nT, on, g);
-  unsigned rst = load_resets<U>(a.reset, n, one_n, t0, a.nT);
-  (void)mine;
-  const int64_t k_end = SPLIT ? k + 1 : nK;
-  for (; k < k_end; ++k) {
-    float cA[U][VEC], lh[U][VEC];
+      Vec<T, VEC> o;
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      float A = 1.f, B = 0.f;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
+      for (int v = 0; v < VEC; ++v) {
         float f, i;
-        gates(to_f(g[u].v[v]), f, i);
-        const bool r = (rst >> u) & 1;
-        const float na = r ? -0.f : (drops(A) ? A : A * f);
-        const float nb = fmaf(f, r ? 0.f : B, i * to_f(x[u].v[v]));
-        const bool in = t0 + u < a.nT;
-        A = in ? na : A;
-        B = in ? nb : B;
-        cA[u][v] = A;
-        lh[u][v] = B;
+        gates<T>(g[u].get(v), f, i);
+        s.v[v] = fmaf(f, s.v[v], i * x[u].get(v));
       }
-      sA[w][lane * VEC + v] = A;
-      sB[w][lane * VEC + v] = B;
+      o.put(s.v);
+      if (more) {
+        x[u] = ld_vec<T, VEC>(xn);
+        g[u] = ld_vec<T, VEC>(gn);
+      }
+      xn += a.x.ts;
+      gn += a.g.ts;
+      if (p.on) st_vec(hp, o);
+      hp += a.h.ts;
     }
-    const int64_t t_now = t0;
-    if (!SPLIT && k + 1 < k_end) {
-      t0 += kRecChunk;
-      load_ticks<T, VEC, U>(a.x, n * a.x.ns + d, t0, a.nT, on, x);
-      load_ticks<T, VEC, U>(a.g, n * a.g.ns + d, t0, a.nT, on, g);
-      rst = load_resets<U>(a.reset, n, one_n, t0, a.nT);
+    rst = rst_next;
+  }
+  if (rem) {
+    if (cp && p.on) st_vec(cp, s);
+    load_ticks<T, VEC>(xp, a.x.ts, rem, x);
+    load_ticks<T, VEC>(gp, a.g.ts, rem, g);
+#pragma unroll
+    for (int u = 0; u < kRecU; ++u) {
+      if (u >= rem) break;
+      Vec<T, VEC> o;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        float f, i;
+        gates<T>(g[u].get(v), f, i);
+        s.v[v] = fmaf(f, (rst >> u) & 1 ? 0.f : s.v[v], i * x[u].get(v));
+      }
+      o.put(s.v);
+      if (p.on) st_vec(hp, o);
+      hp += a.h.ts;
     }
-    __syncthreads();
-    for (int j = threadIdx.x; j < CH; j += blockDim.x) {
-      const int64_t ch = grp * CH + j;
-      if (ch >= nC) break;
-      if (SPLIT) {
-        float A = 1.f, B = 0.f;
-        for (int q = 0; q < warps; ++q) {
-          B = through(sA[q][j], sB[q][j], B);
-          A = drops(sA[q][j]) ? sA[q][j] : A * sA[q][j];
+  }
+  if (a.s_end && p.on && first + ticks == a.nT) st_vec(a.s_end + p.c, s);
+}
+
+// Gradients of n ticks from the state entering them; acc: what enters from
+// the later ticks, then what leaves below.  A first walk up finds the state
+// before every tick, a second one down the gradients; the gates are computed
+// again there, which costs less than the registers to hold them.  emit(u, dx,
+// dgate) takes tick u's and may load what comes next into its operands.
+// CLEAN: no lane has a reset.
+template <class T, int VEC, bool CLEAN, class F>
+__device__ __forceinline__ void backward_ticks(const Vec<T, VEC>* x, const Vec<T, VEC>* g,
+                                               const Vec<T, VEC>* dh, unsigned rst, int n,
+                                               Vec<float, VEC> s, Vec<float, VEC>& acc, F emit) {
+  float prev[kRecU][VEC];
+#pragma unroll
+  for (int u = 0; u < kRecU; ++u) {
+    if (u < n) {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        prev[u][v] = !CLEAN && ((rst >> u) & 1) ? 0.f : s.v[v];
+        if (u + 1 < kRecU) {
+          float f, i;
+          gates<T>(g[u].get(v), f, i);
+          s.v[v] = fmaf(f, prev[u][v], i * x[u].get(v));
         }
-        if (k + 1 < nK)
-          st_pub64(a.agg + k * nC + ch,
-                   ((unsigned long long)__float_as_uint(A) << 32) | __float_as_uint(B));
-        s = state_entering(a, k, ch, nC, a.s0 ? a.s0[ch] : 0.f);
-        const float out = through(A, B, s);
-        if (k + 1 < nK && (k + 1) % kRecGroup == 0)
-          st_pub32(a.group_in + (k + 1) / kRecGroup * nC + ch, __float_as_uint(out));
-      } else if (k == 0) {
-        s = a.s0 ? a.s0[ch] : 0.f;
-      }
-      if (a.carry) a.carry[k * nC + ch] = s;
-      for (int q = 0; q < warps; ++q) {
-        const float A = sA[q][j], B = sB[q][j];
-        sB[q][j] = s;
-        s = through(A, B, s);
-      }
-      if (k + 1 == nK && a.s_end) a.s_end[ch] = s;
-    }
-    __syncthreads();
-    if (on) {
-      T* hp = (T*)a.h.p + n * a.h.ns + d + t_now * a.h.ts;
-      float in[VEC];
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) in[v] = sB[w][lane * VEC + v];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (t_now + u < a.nT) {
-          Vec<T, VEC> o;
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) o.v[v] = from_f<T>(through(cA[u][v], lh[u][v], in[v]));
-          st_vec(hp, o);
-        }
-        hp += a.h.ts;
       }
     }
-    if (!SPLIT) __syncthreads();
+  }
+#pragma unroll
+  for (int u = kRecU - 1; u >= 0; --u) {
+    if (u < n) {
+      Vec<T, VEC> dx, dg;
+      float fx[VEC], fg[VEC];
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        float f, i;
+        gates<T>(g[u].get(v), f, i);
+        const float e = dh[u].get(v) + acc.v[v];
+        const float fe = f * e;
+        fx[v] = i * e;
+        fg[v] = i * fe * (prev[u][v] - x[u].get(v));
+        acc.v[v] = !CLEAN && ((rst >> u) & 1) ? 0.f : fe;
+      }
+      dx.put(fx);
+      dg.put(fg);
+      emit(u, dx, dg);
+    }
   }
 }
 
-template <class T, int VEC, int U, bool SPLIT>
-__global__ void __launch_bounds__(kRecChunk / U * 32, U == 8 ? 2 : 1) k_rec_bwd(RecArgs a) {
-  constexpr int W = kRecChunk / U, CH = 32 * VEC;
-  __shared__ float sA[W][CH], sB[W][CH], sG[W][CH];
-  const int warps = blockDim.x >> 5, w = warp_id(), lane = lane_id();
-  const int64_t nC = a.nN * a.nD, nG = (nC + CH - 1) / CH;
-  const int64_t nK = (a.nT + kRecChunk - 1) / kRecChunk;
-  int64_t m = 0, grp = blockIdx.x;        // m counts tiles from the last one back
-  if (SPLIT) {
-    const int64_t tk = take_ticket(a.ticket);
-    m = tk / nG;
-    grp = tk % nG;
+template <class T, int VEC>
+__global__ void __launch_bounds__(kSeqThreads, kBwdBlocks) k_rec_seq_bwd(RecArgs a) {
+  const RecPlace p = rec_place<VEC>(a, (blockIdx.x * kSeqThreads + threadIdx.x) * VEC);
+  const int64_t first = blockIdx.y * a.seg;
+  const int64_t end = first + a.seg < a.nT ? first + a.seg : a.nT;
+  const int64_t full = end / kRecU;    // (batches are counted from tick 0)
+  const int rem = (int)(end % kRecU);
+  const bool has_dh = a.h.p != nullptr;
+  const float* from = a.enters ? a.enters + (int64_t)blockIdx.y * a.nC : a.s0;
+  Vec<float, VEC> acc = from ? ld_vec<float, VEC>(from + p.c) : vec_zero<float, VEC>();
+  Vec<T, VEC> x[kRecU], g[kRecU], dh[kRecU];
+#pragma unroll
+  for (int u = 0; u < kRecU; ++u) dh[u] = vec_zero<T, VEC>();
+  if (rem) {                         // the last, short stretch first
+    const int64_t t0 = full * kRecU;
+    load_ticks<T, VEC>(at<T>(a.x, p, t0), a.x.ts, rem, x);
+    load_ticks<T, VEC>(at<T>(a.g, p, t0), a.g.ts, rem, g);
+    if (has_dh) load_ticks<T, VEC>(at<T>(a.h, p, t0), a.h.ts, rem, dh);
+    T *xo = at<T>(a.dx, p, t0), *go = at<T>(a.dg, p, t0);
+    const Vec<float, VEC> s = ld_vec<float, VEC>(a.carry + full * a.nC + p.c);
+    backward_ticks<T, VEC, false>(
+        x, g, dh, load_resets(a, p, t0), rem, s, acc,
+        [&](int u, const Vec<T, VEC>& dx, const Vec<T, VEC>& dg) {
+          if (p.on) {
+            st_vec(xo + u * a.dx.ts, dx);
+            st_vec(go + u * a.dg.ts, dg);
+          }
+        });
   }
-  const int64_t c = grp * CH + lane * VEC;
-  const bool on = c < nC;
-  const int64_t n = on ? c / a.nD : 0, d = on ? c % a.nD : 0;
-  const bool one_n = __shfl_sync(QQT_FULL, (int)n, 0) == __shfl_sync(QQT_FULL, (int)n, 31) &&
-                     __all_sync(QQT_FULL, on);
-  float e_in = 0.f;
-  const int64_t m_end = SPLIT ? m + 1 : nK;
-  for (; m < m_end; ++m) {
-    const int64_t k = nK - 1 - m;
-    const int64_t t0 = k * kRecChunk + w * U;
-    Vec<T, VEC> x[U], g[U], dh[U];
-    load_ticks<T, VEC, U>(a.x, n * a.x.ns + d, t0, a.nT, on, x);
-    load_ticks<T, VEC, U>(a.g, n * a.g.ns + d, t0, a.nT, on, g);
-    load_ticks<T, VEC, U>(a.h, n * a.h.ns + d, t0, a.nT, on && a.h.p, dh);
-    const unsigned rst = load_resets<U>(a.reset, n, one_n, t0, a.nT);
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      float A = 1.f, B = 0.f, G = 0.f, f[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float i;
-        gates(to_f(g[u].v[v]), f[u], i);
-        const bool r = (rst >> u) & 1;
-        const float na = r ? -0.f : (drops(A) ? A : A * f[u]);
-        const float nb = fmaf(f[u], r ? 0.f : B, i * to_f(x[u].v[v]));
-        const bool in = t0 + u < a.nT;
-        A = in ? na : A;
-        B = in ? nb : B;
+  const int64_t b0 = first / kRecU;
+  if (full > b0) {
+    int64_t b = full - 1;
+    const T *xp = at<T>(a.x, p, b * kRecU), *gp = at<T>(a.g, p, b * kRecU);
+    const T* hp = has_dh ? at<T>(a.h, p, b * kRecU) : nullptr;
+    T *xo = at<T>(a.dx, p, full * kRecU), *go = at<T>(a.dg, p, full * kRecU);
+    load_ticks<T, VEC>(gp, a.g.ts, kRecU, g);
+    load_ticks<T, VEC>(xp, a.x.ts, kRecU, x);
+    if (has_dh) load_ticks<T, VEC>(hp, a.h.ts, kRecU, dh);
+    Vec<float, VEC> s = ld_vec<float, VEC>(a.carry + b * a.nC + p.c);
+    unsigned rst = load_resets(a, p, b * kRecU);
+    for (; b >= b0; --b) {
+      const bool more = b > b0;
+      Vec<float, VEC> s_next = s;
+      unsigned rst_next = 0;
+      // (the tick before the first is the last of the batch to come)
+      const T *xn = xp - a.x.ts, *gn = gp - a.g.ts, *hn = hp - a.h.ts;
+      if (more) {
+        s_next = ld_vec<float, VEC>(a.carry + (b - 1) * a.nC + p.c);
+        rst_next = load_resets(a, p, (b - 1) * kRecU);
       }
-#pragma unroll
-      for (int u = U - 1; u >= 0; --u) {
-        const float ng = (rst >> u) & 1 ? 0.f : f[u] * (to_f(dh[u].v[v]) + G);
-        G = t0 + u < a.nT ? ng : G;
-      }
-      sA[w][lane * VEC + v] = A;
-      sB[w][lane * VEC + v] = B;
-      sG[w][lane * VEC + v] = G;
-    }
-    __syncthreads();
-    for (int j = threadIdx.x; j < CH; j += blockDim.x) {
-      const int64_t ch = grp * CH + j;
-      if (ch >= nC) break;
-      if (SPLIT) {
-        float A = 1.f, G = 0.f;
-        for (int q = warps - 1; q >= 0; --q) {
-          G = through(sA[q][j], sG[q][j], G);
-          A = drops(sA[q][j]) ? sA[q][j] : A * sA[q][j];
+      auto emit = [&](int u, const Vec<T, VEC>& dx, const Vec<T, VEC>& dg) {
+        if (more) {
+          x[u] = ld_vec<T, VEC>(xn);
+          g[u] = ld_vec<T, VEC>(gn);
+          if (has_dh) dh[u] = ld_vec<T, VEC>(hn);
         }
-        if (m + 1 < nK)
-          st_pub64(a.agg + m * nC + ch,
-                   ((unsigned long long)__float_as_uint(A) << 32) | __float_as_uint(G));
-        e_in = state_entering(a, m, ch, nC, a.s0 ? a.s0[ch] : 0.f);
-        const float out = through(A, G, e_in);
-        if (m + 1 < nK && (m + 1) % kRecGroup == 0)
-          st_pub32(a.group_in + (m + 1) / kRecGroup * nC + ch, __float_as_uint(out));
-      } else if (m == 0) {
-        e_in = a.s0 ? a.s0[ch] : 0.f;
-      }
-      float s = a.carry[k * nC + ch];
-      for (int q = 0; q < warps; ++q) {
-        const float B = sB[q][j];
-        sB[q][j] = s;
-        s = through(sA[q][j], B, s);
-      }
-      for (int q = warps - 1; q >= 0; --q) {
-        const float G = sG[q][j];
-        sG[q][j] = e_in;
-        e_in = through(sA[q][j], G, e_in);
-      }
-      if (k == 0 && a.s_end) a.s_end[ch] = e_in;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      float f[U], i[U], prev[U];
-      float s = sB[w][lane * VEC + v], acc = sG[w][lane * VEC + v];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        gates(to_f(g[u].v[v]), f[u], i[u]);
-        prev[u] = (rst >> u) & 1 ? 0.f : s;
-        s = fmaf(f[u], prev[u], i[u] * to_f(x[u].v[v]));
-      }
-#pragma unroll
-      for (int u = U - 1; u >= 0; --u) {
-        const bool in = t0 + u < a.nT;
-        const float e = to_f(dh[u].v[v]) + acc;
-        const float ie = i[u] * e;
-        const float dg = f[u] * ie * (prev[u] - to_f(x[u].v[v]));
-        x[u].v[v] = from_f<T>(ie);
-        g[u].v[v] = from_f<T>(dg);
-        acc = in ? ((rst >> u) & 1 ? 0.f : f[u] * e) : acc;
-      }
-    }
-    if (on) {
-      T* xp = (T*)a.dx.p + n * a.dx.ns + d + t0 * a.dx.ts;
-      T* gp = (T*)a.dg.p + n * a.dg.ns + d + t0 * a.dg.ts;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (t0 + u < a.nT) {
-          st_vec(xp, x[u]);
-          st_vec(gp, g[u]);
+        xn -= a.x.ts;
+        gn -= a.g.ts;
+        hn -= a.h.ts;
+        xo -= a.dx.ts;
+        go -= a.dg.ts;
+        if (p.on) {
+          st_vec(xo, dx);
+          st_vec(go, dg);
         }
-        xp += a.dx.ts;
-        gp += a.dg.ts;
-      }
+      };
+      if (__all_sync(QQT_FULL, rst == 0))
+        backward_ticks<T, VEC, true>(x, g, dh, rst, kRecU, s, acc, emit);
+      else
+        backward_ticks<T, VEC, false>(x, g, dh, rst, kRecU, s, acc, emit);
+      gp -= kRecU * a.g.ts;
+      xp -= kRecU * a.x.ts;
+      hp -= kRecU * a.h.ts;
+      s = s_next;
+      rst = rst_next;
     }
-    if (!SPLIT) __syncthreads();
+  }
+  if (a.s_end && p.on && first == 0) st_vec(a.s_end + p.c, acc);
+}
+
+// ------------------------------------------------------------- segments
+
+// The pair of a segment of VEC channels: (A, B) of the state, or, with BWD,
+// (A, G) of the gradient, scanned from the segment's last tick down.
+template <class T, int VEC, bool BWD>
+__device__ __forceinline__ void pair_tick(const Vec<T, VEC>& x, const Vec<T, VEC>& g, bool r,
+                                          float* A, float* B) {
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) {
+    float f, i;
+    gates<T>(g.get(v), f, i);
+    B[v] = BWD ? f * (x.get(v) + B[v]) : fmaf(f, r ? 0.f : B[v], i * x.get(v));
+    if (BWD && r) B[v] = 0.f;
+    A[v] = r || drops(A[v]) ? -0.f : A[v] * f;
   }
 }
 
-// Tiles of few ticks take fewer warps, so a block may have fewer threads than
-// channels; the per-channel part strides over them, and only a whole block
-// (blockDim >= CH) may walk several tiles with the state in a register.
+template <class T, int VEC, bool BWD>
+__global__ void __launch_bounds__(kSeqThreads, kFwdBlocks) k_rec_sum(RecArgs a) {
+  const RecPlace p = rec_place<VEC>(a, (blockIdx.x * kSeqThreads + threadIdx.x) * VEC);
+  // the segments that some other one follows in the scan's direction
+  const int64_t first = (blockIdx.y + (BWD ? 1 : 0)) * a.seg;
+  const int64_t end = first + a.seg < a.nT ? first + a.seg : a.nT;
+  const RecSeq& in = BWD ? a.h : a.x;
+  const bool has_in = in.p != nullptr;
+  float A[VEC], B[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) {
+    A[v] = 1.f;
+    B[v] = 0.f;
+  }
+  Vec<T, VEC> x[kRecU], g[kRecU];
+#pragma unroll
+  for (int u = 0; u < kRecU; ++u) x[u] = vec_zero<T, VEC>();
+  const int64_t full = end / kRecU, b0 = first / kRecU;   // batches counted from tick 0
+  const int rem = (int)(end % kRecU);
+  if (BWD && rem) {                  // (only the last segment ends inside a batch)
+    load_ticks<T, VEC>(at<T>(a.g, p, full * kRecU), a.g.ts, rem, g);
+    if (has_in) load_ticks<T, VEC>(at<T>(in, p, full * kRecU), in.ts, rem, x);
+    const unsigned rst = load_resets(a, p, full * kRecU);
+#pragma unroll
+    for (int u = kRecU - 1; u >= 0; --u)
+      if (u < rem) pair_tick<T, VEC, BWD>(x[u], g[u], (rst >> u) & 1, A, B);
+  }
+  if (full > b0) {
+    const int64_t dir = BWD ? -1 : 1;
+    int64_t b = BWD ? full - 1 : b0;
+    const T* gp = at<T>(a.g, p, b * kRecU);
+    const T* xp = has_in ? at<T>(in, p, b * kRecU) : nullptr;
+    load_ticks<T, VEC>(gp, a.g.ts, kRecU, g);
+    if (has_in) load_ticks<T, VEC>(xp, in.ts, kRecU, x);
+    unsigned rst = load_resets(a, p, b * kRecU);
+    // from here on the pointers are at the scan's first tick of the next batch
+    const int64_t gs = dir * a.g.ts, xs = dir * in.ts;
+    const T* gn = BWD ? gp - a.g.ts : gp + kRecU * a.g.ts;
+    const T* xn = BWD ? xp - in.ts : xp + kRecU * in.ts;
+    for (int64_t left = full - b0; left > 0; --left) {
+      const bool more = left > 1;
+      b += dir;
+      const unsigned rst_next = more ? load_resets(a, p, b * kRecU) : 0;
+#pragma unroll
+      for (int j = 0; j < kRecU; ++j) {
+        const int u = BWD ? kRecU - 1 - j : j;
+        pair_tick<T, VEC, BWD>(x[u], g[u], (rst >> u) & 1, A, B);
+        if (more) {
+          g[u] = ld_vec<T, VEC>(gn);
+          if (has_in) x[u] = ld_vec<T, VEC>(xn);
+        }
+        gn += gs;
+        xn += xs;
+      }
+      rst = rst_next;
+    }
+  }
+  if (!p.on) return;
+#pragma unroll
+  for (int v = 0; v < VEC; ++v)
+    a.pair[(int64_t)blockIdx.y * a.nC + p.c + v] = make_float2(A[v], B[v]);
+}
+
+// What enters each segment.  Pair j is the j-th row that k_rec_sum wrote; with
+// BWD the scan begins at the last.  A block takes 32 channels; each of its 32
+// warps composes its share of the segments, one warp joins the shares, and
+// then each walks its own: two short walks in place of one of all segments.
+template <bool BWD>
+__global__ void __launch_bounds__(1024) k_rec_join(RecArgs a, int segs) {
+  __shared__ float sA[32][33], sB[32][33];
+  const int l = lane_id(), w = warp_id();
+  const uint32_t c0 = blockIdx.x * 32 + l;
+  const bool on = c0 < a.nC;
+  const uint32_t c = on ? c0 : a.nC - 1;
+  const int per = (segs + 31) / 32;
+  const int k0 = w * per, k1 = k0 + per < segs ? k0 + per : segs;
+  constexpr int Q = 8;
+  auto pair_of = [&](int k) {        // that of the k-th segment along the scan
+    return a.pair[(int64_t)(BWD ? segs - 2 - k : k) * a.nC + c];
+  };
+  float A = 1.f, B = 0.f;
+  for (int k = k0; k < k1; k += Q) {
+    float2 v[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+      if (k + q < k1 && k + q + 1 < segs) v[q] = pair_of(k + q);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      if (k + q < k1 && k + q + 1 < segs) {
+        B = through(v[q].x, v[q].y, B);
+        A = drops(A) || drops(v[q].x) ? -0.f : A * v[q].x;
+      }
+    }
+  }
+  sA[w][l] = A;
+  sB[w][l] = B;
+  __syncthreads();
+  if (w == 0) {
+    float s = a.s0 ? a.s0[c] : 0.f;
+#pragma unroll 8
+    for (int q = 0; q < 32; ++q) {
+      const float nA = sA[q][l], nB = sB[q][l];
+      sB[q][l] = s;
+      s = through(nA, nB, s);
+    }
+  }
+  __syncthreads();
+  float s = sB[w][l];
+  for (int k = k0; k < k1; k += Q) {
+    float2 v[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+      if (k + q < k1 && k + q + 1 < segs) v[q] = pair_of(k + q);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      if (k + q < k1) {
+        if (on) a.enters[(int64_t)(BWD ? segs - 1 - (k + q) : k + q) * a.nC + c] = s;
+        if (k + q + 1 < segs) s = through(v[q].x, v[q].y, s);
+      }
+    }
+  }
+}
+
 static int rec_sms() {
   static std::atomic<int> n{0};
   int v = n.load();
@@ -444,26 +518,25 @@ static int rec_sms() {
   return v;
 }
 
-struct RecWork {
-  int64_t agg, group, total;       // byte offsets; the ticket is at 0
+// How time is cut: segments of at least 4 kRecU ticks, one where fewer than
+// three would come of it (the inputs are read twice then).
+struct RecCut {
+  int64_t seg;
+  int segs;
 };
-static RecWork rec_work(int64_t T, int64_t C) {
-  const int64_t k = (T + kRecChunk - 1) / kRecChunk;
-  RecWork w;
-  w.agg = 16;
-  w.group = w.agg + k * C * 8;
-  w.total = w.group + ((k + kRecGroup - 1) / kRecGroup) * C * 4;
-  return w;
-}
-// Split along time when one block per channel group would leave SMs without
-// two blocks each and there is more than one tile to hand out.
-static bool rec_split(int64_t T, int64_t C, int vec) {
-  return T > kRecChunk && (C + 32 * vec - 1) / (32 * vec) < 2 * rec_sms();
+static RecCut rec_cut(int64_t T, int64_t C) {
+  const int64_t want = (int64_t)rec_sms() * kRecWalks / C;
+  int64_t seg = want > 1 ? (T + want - 1) / want : T;
+  if (seg < 4 * kRecU) seg = 4 * kRecU;
+  seg = (seg + kRecU - 1) / kRecU * kRecU;
+  const int64_t segs = (T + seg - 1) / seg;
+  if (segs < 3) return {(T + kRecU - 1) / kRecU * kRecU, 1};
+  return {seg, (int)segs};
 }
 
 static bool rec_sizes_ok(int64_t T, int64_t N, int64_t D) {
-  return T >= 0 && N >= 0 && D > 0 && N <= 0x7fffffffll && D <= 0x7fffffffll &&
-         (N == 0 || D <= 0x7fffffffll * 32 / N) && T <= 0x7fffffffll;
+  return T >= 0 && N >= 0 && D > 0 && T <= 0x7fffffffll && N <= 0x7fffffffll && D <= 0x7fffffffll &&
+         N * D <= 0x7fffff00ll;
 }
 static bool seq_vec(const RecSeq& s, int64_t bytes, int64_t es) {
   return !s.p || (aligned_to(s.p, bytes) && (s.ts * es) % bytes == 0 && (s.ns * es) % bytes == 0);
@@ -473,31 +546,48 @@ static RecSeq rec_seq(const QqtSeq* s) {
 }
 
 template <class T, int VEC, bool BWD>
-static int rec_launch(RecArgs a, void* work, cudaStream_t st) {
-  constexpr int U = sizeof(T) * VEC == 16 ? 4 : 8, W = kRecChunk / U;
-  const int64_t C = a.nN * a.nD, nG = (C + 32 * VEC - 1) / (32 * VEC);
-  const int64_t nK = (a.nT + kRecChunk - 1) / kRecChunk;
-  const int warps = a.nT >= kRecChunk ? W : (int)((a.nT + U - 1) / U);
-  if (rec_split(a.nT, C, VEC)) {
-    const RecWork w = rec_work(a.nT, C);
-    char* base = (char*)work;
-    if (!base) return QQT_E_ARG;
-    if (nK * nG > 0x7fffffffll) return QQT_E_LIMIT;
-    if (cudaMemsetAsync(base, 0xff, (size_t)w.total, st) != cudaSuccess) return QQT_E_LAUNCH;
-    a.ticket = (unsigned*)base;
-    a.agg = (unsigned long long*)(base + w.agg);
-    a.group_in = (unsigned*)(base + w.group);
-    if (BWD)
-      k_rec_bwd<T, VEC, U, true><<<(unsigned)(nK * nG), 32 * W, 0, st>>>(a);
-    else
-      k_rec_fwd<T, VEC, U, true><<<(unsigned)(nK * nG), 32 * W, 0, st>>>(a);
-  } else {
-    if (BWD)
-      k_rec_bwd<T, VEC, U, false><<<(unsigned)nG, 32 * warps, 0, st>>>(a);
-    else
-      k_rec_fwd<T, VEC, U, false><<<(unsigned)nG, 32 * warps, 0, st>>>(a);
+static int rec_walk(RecArgs a, void* work, cudaStream_t st) {
+  const unsigned blocks = (a.nC / VEC + kSeqThreads - 1) / kSeqThreads;
+  const RecCut cut = rec_cut(a.nT, a.nC);
+  a.seg = cut.seg;
+  if (cut.segs > 1) {
+    if (!work) return QQT_E_ARG;
+    a.pair = (float2*)work;
+    a.enters = (float*)(a.pair + (int64_t)(cut.segs - 1) * a.nC);
+    k_rec_sum<T, VEC, BWD><<<dim3(blocks, cut.segs - 1), kSeqThreads, 0, st>>>(a);
+    k_rec_join<BWD><<<(a.nC + 31) / 32, 1024, 0, st>>>(a, cut.segs);
   }
+  if (BWD)
+    k_rec_seq_bwd<T, VEC><<<dim3(blocks, cut.segs), kSeqThreads, 0, st>>>(a);
+  else
+    k_rec_seq_fwd<T, VEC><<<dim3(blocks, cut.segs), kSeqThreads, 0, st>>>(a);
   return launch_status();
+}
+
+// Channels that one access may cover: 4, 2 or 1.
+static int rec_vec(const RecArgs& a, int64_t es) {
+  for (int v = 4; v > 1; v /= 2)
+    if (a.nD % v == 0 && seq_vec(a.x, v * es, es) && seq_vec(a.g, v * es, es) &&
+        seq_vec(a.h, v * es, es) && seq_vec(a.dx, v * es, es) && seq_vec(a.dg, v * es, es) &&
+        aligned_to(a.s0, 4 * v) && aligned_to(a.s_end, 4 * v) && aligned_to(a.carry, 4 * v))
+      return v;
+  return 1;
+}
+
+template <class T, bool BWD>
+static int rec_run(const RecArgs& a, void* work, cudaStream_t st) {
+  const int vec = rec_vec(a, sizeof(T));
+  if (!BWD && a.nT == 1 && !a.carry) {
+    if (vec == 4)
+      k_rec_step<T, 4><<<(a.nC / 4 + 127) / 128, 128, 0, st>>>(a);
+    else
+      k_rec_step<T, 1><<<(a.nC + 127) / 128, 128, 0, st>>>(a);
+    return launch_status();
+  }
+  if constexpr (sizeof(T) == 2 && !BWD) {
+    if (vec == 4) return rec_walk<T, 4, BWD>(a, work, st);
+  }
+  return vec >= 2 ? rec_walk<T, 2, BWD>(a, work, st) : rec_walk<T, 1, BWD>(a, work, st);
 }
 
 }  // namespace qqt
@@ -505,12 +595,13 @@ static int rec_launch(RecArgs a, void* work, cudaStream_t st) {
 using namespace qqt;
 
 extern "C" int64_t qqt_recurrence_chunks(int64_t T) {
-  return T <= 0 ? 0 : (T + kRecChunk - 1) / kRecChunk;
+  return T <= 0 ? 0 : (T + kRecU - 1) / kRecU;
 }
 
 extern "C" uint64_t qqt_recurrence_work_bytes(int64_t T, int64_t N, int64_t D) {
   if (!rec_sizes_ok(T, N, D) || T == 0 || N == 0) return 0;
-  return rec_split(T, N * D, 1) || rec_split(T, N * D, 4) ? (uint64_t)rec_work(T, N * D).total : 0;
+  const RecCut c = rec_cut(T, N * D);
+  return c.segs > 1 ? (uint64_t)(c.segs - 1) * N * D * 8 + (uint64_t)c.segs * N * D * 4 : 0;
 }
 
 extern "C" int qqt_recurrence_forward(const QqtSeq* x, const QqtSeq* gate, const QqtSeq* reset,
@@ -538,22 +629,9 @@ extern "C" int qqt_recurrence_forward(const QqtSeq* x, const QqtSeq* gate, const
   a.s_end = h_last;
   a.carry = carry;
   a.nT = T;
-  a.nN = N;
-  a.nD = D;
-  return with_dtype(dtype, [&](auto t) {
-    using E = decltype(t);
-    const int64_t es = sizeof(E), vb = 4 * es;
-    const bool v4 = D % 4 == 0 && seq_vec(a.x, vb, es) && seq_vec(a.g, vb, es) &&
-                    seq_vec(a.h, vb, es);
-    if (T == 1 && !carry && aligned_to(h0, 16) && aligned_to(h_last, 16)) {
-      if (v4)
-        k_rec_step<E, 4><<<(unsigned)((C / 4 + 127) / 128), 128, 0, st>>>(a);
-      else
-        k_rec_step<E, 1><<<(unsigned)((C + 127) / 128), 128, 0, st>>>(a);
-      return launch_status();
-    }
-    return v4 ? rec_launch<E, 4, false>(a, work, st) : rec_launch<E, 1, false>(a, work, st);
-  });
+  a.nC = (uint32_t)C;
+  a.nD = (uint32_t)D;
+  return with_dtype(dtype, [&](auto t) { return rec_run<decltype(t), false>(a, work, st); });
 }
 
 extern "C" int qqt_recurrence_backward(const QqtSeq* dh, const float* dh_last, const QqtSeq* x,
@@ -584,13 +662,7 @@ extern "C" int qqt_recurrence_backward(const QqtSeq* dh, const float* dh_last, c
   a.s_end = dh0;
   a.carry = const_cast<float*>(carry);
   a.nT = T;
-  a.nN = N;
-  a.nD = D;
-  return with_dtype(dtype, [&](auto t) {
-    using E = decltype(t);
-    const int64_t es = sizeof(E), vb = 4 * es;
-    const bool v4 = D % 4 == 0 && seq_vec(a.x, vb, es) && seq_vec(a.g, vb, es) &&
-                    seq_vec(a.h, vb, es) && seq_vec(a.dx, vb, es) && seq_vec(a.dg, vb, es);
-    return v4 ? rec_launch<E, 4, true>(a, work, st) : rec_launch<E, 1, true>(a, work, st);
-  });
+  a.nC = (uint32_t)C;
+  a.nD = (uint32_t)D;
+  return with_dtype(dtype, [&](auto t) { return rec_run<decltype(t), true>(a, work, st); });
 }
