@@ -4,14 +4,328 @@
 //   y  = (x - mean) rstd w + b,   rstd = 1 / sqrt(var + eps)
 //   dx = rstd (q - mean(q) - xh mean(q xh)),  q = dy w,  xh = (x - mean) rstd
 //   dw = sum over rows of dy xh,  db = sum over rows of dy
-// All statistics and sums are float32; outputs are rounded once.
+// All statistics and sums are float32; the mean comes first and the variance
+// is taken around it (no cancellation for rows far from zero); outputs are
+// rounded once.
+//
+// Memory bound: 2 values moved per element forward, 3 backward (one read of x
+// and dy serves dx and the weight's gradient).  A row stays in the registers
+// of its team -- 8 lanes, a warp, or a block, by the row's number of 16-byte
+// vectors -- between the passes over it.  The backward teams walk over rows
+// and keep their columns' sums of dy xh and dy in registers; each block writes
+// one partial row and a second kernel adds the partials in a fixed order, so
+// there are no atomics and results repeat.  Rows that are not made of whole
+// vectors go element by element; rows too long for a block's registers are
+// read again for every pass.
 
 #include "ops_common.cuh"
 
 namespace qqt {
 
+constexpr int kLnWarpThreads = 256;   // block of the teams inside a warp
+#ifndef LN_FWD_G
+#define LN_FWD_G 8
+#endif
+#ifndef LN_BWD_G
+#define LN_BWD_G 4
+#endif
+#ifndef LN_FWD_B
+#define LN_FWD_B 2048
+#endif
+#ifndef LN_BWD_B
+#define LN_BWD_B 1024
+#endif
+
+// Largest block that walks rows with e elements a thread: the backward pass
+// keeps 2 e sums besides its operands.
+__host__ __device__ constexpr int ln_max_threads(int e) { return e == 16 ? 768 : 512; }
+
+// Sums of N values over a team of G lanes (G <= 32), or over the block (G =
+// 0; buf holds 2 x N x 32 floats, used in turn so that one barrier is enough).
+template <int G, int N>
+__device__ __forceinline__ void team_sum(float* v, float (*buf)[N][32], int& turn) {
+#pragma unroll
+  for (int o = (G ? G : 32) / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(QQT_FULL, v[k], o);
+  if (G == 0) {
+    const int nw = blockDim.x >> 5;
+    float(*b)[32] = buf[turn];
+    turn ^= 1;
+    if (lane_id() == 0)
+#pragma unroll
+      for (int k = 0; k < N; ++k) b[k][warp_id()] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = warp_sum_f(lane_id() < nw ? b[k][lane_id()] : 0.f);
+  }
+}
+
+// What a thread holds: vectors j, j + step, ... of its team's row, of nv.
+struct LnTeam {
+  int64_t row, rows_step;
+  int j, step;
+};
+template <int G>
+__device__ __forceinline__ LnTeam ln_team() {
+  LnTeam t;
+  if (G) {
+    constexpr int per = kLnWarpThreads / (G ? G : 1);
+    t.row = (int64_t)blockIdx.x * per + threadIdx.x / (G ? G : 1);
+    t.rows_step = (int64_t)gridDim.x * per;
+    t.j = threadIdx.x % (G ? G : 1);
+    t.step = G;
+  } else {
+    t.row = blockIdx.x;
+    t.rows_step = gridDim.x;
+    t.j = threadIdx.x;
+    t.step = blockDim.x;
+  }
+  return t;
+}
+
+template <class T, int VEC, int K>
+__device__ __forceinline__ void ln_load(const T* p, const LnTeam& t, int nv, bool on,
+                                        Vec<T, VEC>* out) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int j = t.j + k * t.step;
+    out[k] = on && j < nv ? ld_vec<T, VEC>(p + (int64_t)j * VEC) : vec_zero<T, VEC>();
+  }
+}
+template <int VEC>
+__device__ __forceinline__ Vec<float, VEC> ln_param(const float* p, int j) {
+  Vec<float, VEC> r;
+  if constexpr (VEC == 8) {
+    const float4 lo = *reinterpret_cast<const float4*>(p + j * 8);
+    const float4 hi = *reinterpret_cast<const float4*>(p + j * 8 + 4);
+    const float f[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    r.put(f);
+  } else {
+    r = ld_vec<float, VEC>(p + j * VEC);
+  }
+  return r;
+}
+
+template <class T, int VEC, int K, int G>
+__global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K))
+    k_ln_fwd(const T* __restrict__ x, int64_t xs, int64_t rows, int d, const float* __restrict__ w,
+             const float* __restrict__ b, float eps, T* __restrict__ y, float* __restrict__ mean,
+             float* __restrict__ rstd) {
+  __shared__ float buf[2][1][32];
+  int turn = 0;
+  const int nv = d / VEC;
+  const float inv_d = 1.f / (float)d;
+  LnTeam t = ln_team<G>();
+  // (a team's lanes shuffle together with the rest of their warp, so a warp
+  // goes on until its last team is done)
+  const int64_t lead = G && G < 32 ? t.row - (threadIdx.x % 32) / (G ? G : 1) : t.row;
+  Vec<T, VEC> c[K];
+  ln_load<T, VEC, K>(x + t.row * xs, t, nv, t.row < rows, c);
+  for (int64_t lr = lead; lr < rows; lr += t.rows_step) {
+    const bool on = t.row < rows;
+    float f[K][VEC];
+    float s[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        f[k][v] = c[k].get(v);
+        s[0] += f[k][v];
+      }
+    // the next row's values are on their way meanwhile
+    const int64_t next = t.row + t.rows_step;
+    ln_load<T, VEC, K>(x + next * xs, t, nv, next < rows, c);
+    team_sum<G, 1>(s, buf, turn);
+    const float mu = s[0] * inv_d;
+    s[0] = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (t.j + k * t.step < nv)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          f[k][v] -= mu;
+          s[0] = fmaf(f[k][v], f[k][v], s[0]);
+        }
+    team_sum<G, 1>(s, buf, turn);
+    const float rs = 1.f / sqrtf(s[0] * inv_d + eps);
+    if (on) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int j = t.j + k * t.step;
+        if (j < nv) {
+          const Vec<float, VEC> wv = ln_param<VEC>(w, j);
+          float o[VEC];
+          if (b) {
+            const Vec<float, VEC> bv = ln_param<VEC>(b, j);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) o[v] = fmaf(f[k][v] * rs, wv.get(v), bv.get(v));
+          } else {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) o[v] = f[k][v] * rs * wv.get(v);
+          }
+          Vec<T, VEC> out;
+          out.put(o);
+          st_vec(y + t.row * d + (int64_t)j * VEC, out);
+        }
+      }
+      if (t.j == 0 && mean) {
+        mean[t.row] = mu;
+        rstd[t.row] = rs;
+      }
+    }
+    t.row = next;
+  }
+}
+
+// dx of the team's rows, and the block's partial sums of dy xh and dy.
+template <class T, int VEC, int K, int G>
+__global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K))
+    k_ln_bwd(const T* __restrict__ dy, int64_t dys, const T* __restrict__ x, int64_t xs,
+             int64_t rows, int d, const float* __restrict__ mean, const float* __restrict__ rstd,
+             const float* __restrict__ w, T* __restrict__ dx, float* __restrict__ part) {
+  __shared__ float buf[2][2][32];
+  extern __shared__ float sums[];          // teams inside a warp: [teams][2 d]
+  int turn = 0;
+  const int nv = d / VEC;
+  const float inv_d = 1.f / (float)d;
+  LnTeam t = ln_team<G>();
+  const int64_t lead = G && G < 32 ? t.row - (threadIdx.x % 32) / (G ? G : 1) : t.row;
+  float aw[K][VEC], ab[K][VEC];
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) aw[k][v] = ab[k][v] = 0.f;
+  // Few elements: the scaled values stay for the second half and the next row
+  // is loaded meanwhile.  Many: they are made again from the packed operands.
+  constexpr bool KEEP = VEC * K <= 8;
+  Vec<T, VEC> cx[K], cy[K];
+  ln_load<T, VEC, K>(x + t.row * xs, t, nv, t.row < rows, cx);
+  ln_load<T, VEC, K>(dy + t.row * dys, t, nv, t.row < rows, cy);
+  float mu = t.row < rows ? mean[t.row] : 0.f, rs = t.row < rows ? rstd[t.row] : 0.f;
+  for (int64_t lr = lead; lr < rows; lr += t.rows_step) {
+    const bool on = t.row < rows;
+    const float m0 = mu, r0 = rs;
+    float xk[KEEP ? K : 1][VEC], qk[KEEP ? K : 1][VEC];
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int j = t.j + k * t.step;
+      if (j < nv) {
+        const Vec<float, VEC> wv = ln_param<VEC>(w, j);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          const float g = cy[k].get(v), xh = (cx[k].get(v) - m0) * r0, q = g * wv.get(v);
+          ab[k][v] += g;
+          aw[k][v] = fmaf(g, xh, aw[k][v]);
+          s[0] += q;
+          s[1] = fmaf(q, xh, s[1]);
+          if (KEEP) {
+            xk[KEEP ? k : 0][v] = xh;
+            qk[KEEP ? k : 0][v] = q;
+          }
+        }
+      }
+    }
+    const int64_t next = t.row + t.rows_step;
+    auto load_next = [&] {
+      ln_load<T, VEC, K>(x + next * xs, t, nv, next < rows, cx);
+      ln_load<T, VEC, K>(dy + next * dys, t, nv, next < rows, cy);
+      if (next < rows) {
+        mu = mean[next];
+        rs = rstd[next];
+      }
+    };
+    if (KEEP || !dx) load_next();
+    if (dx) {
+      team_sum<G, 2>(s, buf, turn);
+      const float m1 = s[0] * inv_d, m2 = s[1] * inv_d;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int j = t.j + k * t.step;
+        if (on && j < nv) {
+          float o[VEC];
+          if (KEEP) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v)
+              o[v] = r0 * (fmaf(-xk[KEEP ? k : 0][v], m2, qk[KEEP ? k : 0][v]) - m1);
+          } else {
+            const Vec<float, VEC> wv = ln_param<VEC>(w, j);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v)
+              o[v] = r0 * (fmaf(-(cx[k].get(v) - m0) * r0, m2, cy[k].get(v) * wv.get(v)) - m1);
+          }
+          Vec<T, VEC> out;
+          out.put(o);
+          st_vec(dx + t.row * d + (int64_t)j * VEC, out);
+        }
+      }
+      if (!KEEP) load_next();
+    }
+    t.row = next;
+  }
+  if (!part) return;
+  float* pw = part + (int64_t)blockIdx.x * 2 * d;
+  if (G == 0) {                            // a block's threads own their columns
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int j = t.j + k * t.step;
+      if (j < nv)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          pw[j * VEC + v] = aw[k][v];
+          pw[d + j * VEC + v] = ab[k][v];
+        }
+    }
+    return;
+  }
+  constexpr int teams = kLnWarpThreads / (G ? G : 1);
+  float* mine = sums + (int64_t)(threadIdx.x / (G ? G : 1)) * 2 * d;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int j = t.j + k * t.step;
+    if (j < nv)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        mine[j * VEC + v] = aw[k][v];
+        mine[d + j * VEC + v] = ab[k][v];
+      }
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < 2 * d; c += kLnWarpThreads) {
+    float a = 0.f;
+#pragma unroll 8
+    for (int q = 0; q < teams; ++q) a += sums[q * 2 * d + c];
+    pw[c] = a;
+  }
+}
+
+// Adds the partial rows: a block takes 32 columns, each of its warps every
+// (number of warps)-th row.
+__global__ void __launch_bounds__(512) k_ln_add(const float* __restrict__ part, int n_part, int64_t d,
+                                                float* __restrict__ dw, float* __restrict__ db) {
+  __shared__ float buf[16][33];
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane_id();
+  float s = 0.f;
+  if (c < 2 * d) {
+#pragma unroll 8
+    for (int p = warp_id(); p < n_part; p += 16) s += part[(int64_t)p * 2 * d + c];
+  }
+  buf[warp_id()][lane_id()] = s;
+  __syncthreads();
+  if (warp_id() == 0 && c < 2 * d) {
+    s = 0.f;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) s += buf[q][lane_id()];
+    float* out = c < d ? dw : db;
+    if (out) out[c < d ? c : c - d] = s;
+  }
+}
+
+// ------------------------------------- rows longer than a block's registers
+
 template <class T>
-__global__ void k_ln_fwd(const T* __restrict__ x, int64_t xs, int64_t d, const float* __restrict__ w,
+__global__ void k_ln_long_fwd(const T* __restrict__ x, int64_t xs, int64_t d, const float* __restrict__ w,
                          const float* __restrict__ b, float eps, T* __restrict__ y,
                          float* __restrict__ mean, float* __restrict__ rstd) {
   __shared__ float buf[32];
@@ -36,7 +350,7 @@ __global__ void k_ln_fwd(const T* __restrict__ x, int64_t xs, int64_t d, const f
 }
 
 template <class T>
-__global__ void k_ln_dx(const T* __restrict__ dy, int64_t dys, const T* __restrict__ x, int64_t xs,
+__global__ void k_ln_long_dx(const T* __restrict__ dy, int64_t dys, const T* __restrict__ x, int64_t xs,
                         int64_t d, const float* __restrict__ mean, const float* __restrict__ rstd,
                         const float* __restrict__ w, T* __restrict__ dx) {
   __shared__ float buf[32];
@@ -59,10 +373,8 @@ __global__ void k_ln_dx(const T* __restrict__ dy, int64_t dys, const T* __restri
   }
 }
 
-constexpr int kLnParts = 512;   // row groups of the weight gradient's first stage
-
 template <class T>
-__global__ void k_ln_dw_part(const T* __restrict__ dy, int64_t dys, const T* __restrict__ x,
+__global__ void k_ln_long_part(const T* __restrict__ dy, int64_t dys, const T* __restrict__ x,
                              int64_t xs, int64_t rows, int64_t d, const float* __restrict__ mean,
                              const float* __restrict__ rstd, float* __restrict__ part) {
   const int64_t j = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -77,17 +389,85 @@ __global__ void k_ln_dw_part(const T* __restrict__ dy, int64_t dys, const T* __r
   part[(int64_t)blockIdx.y * 2 * d + d + j] = sb;
 }
 
-__global__ void k_ln_dw_sum(const float* __restrict__ part, int n_part, int64_t d,
-                            float* __restrict__ dw, float* __restrict__ db) {
-  const int64_t j = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (j >= 2 * d) return;
-  float s = 0.f;
-  for (int p = 0; p < n_part; ++p) s += part[(int64_t)p * 2 * d + j];
-  float* out = j < d ? dw : db;
-  if (out) out[j < d ? j : j - d] = s;
+// How rows are handed out: vectors of vec elements, k of them a thread, teams
+// of g lanes (0: a block of `threads`), `blocks` blocks that walk over rows.
+struct LnPlan {
+  int vec, k, g, threads;
+  int64_t blocks;
+};
+static int ln_sms() {
+  static std::atomic<int> n{0};
+  int v = n.load();
+  if (v == 0) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0)
+      v = 148;
+    n.store(v);
+  }
+  return v;
+}
+static LnPlan ln_plan(int64_t rows, int64_t d, int vec, bool bwd) {
+  LnPlan p{vec, 0, 0, kLnWarpThreads, 0};
+  const int64_t nv = d / vec;
+  int64_t per_block;
+  if (nv <= (vec == 8 ? 64 : 128)) {       // a team inside a warp
+    const bool one = vec == 8 || nv <= 8;
+    p.k = one ? 1 : 2;
+    p.g = nv <= 8 * p.k ? 8 : nv <= 16 * p.k ? 16 : 32;
+    if (nv > 32 * p.k) p.k *= 2;
+    per_block = kLnWarpThreads / p.g;
+  } else {                                 // a block: as few vectors a thread as its size allows
+    p.k = 1;
+    while (p.k * vec < 32 && nv > (int64_t)p.k * ln_max_threads(p.k * vec)) p.k *= 2;
+    const int64_t th = (nv + p.k - 1) / p.k;
+    if (p.k * vec > (vec == 1 ? 16 : 32) || th > ln_max_threads(p.k * vec)) return p;   // too long
+    p.threads = (int)((th + 31) / 32 * 32);
+    per_block = 1;
+  }
+  const int64_t need = (rows + per_block - 1) / per_block;
+  const int64_t room = (int64_t)ln_sms() * (p.g ? (bwd ? LN_BWD_G : LN_FWD_G) : (bwd ? LN_BWD_B : LN_FWD_B) / p.threads + 1);
+  p.blocks = need < room ? need : room;
+  return p;
+}
+static int64_t ln_parts(int64_t rows, int64_t d, int vec) {
+  const LnPlan p = ln_plan(rows, d, vec, true);
+  if (p.blocks > 0) return p.blocks;
+  return rows < 512 ? (rows > 0 ? rows : 1) : 512;
+}
+// Vector width that rows of these strides and addresses allow.
+static int ln_vec(int64_t es, int64_t d, int64_t s1, int64_t s2, const void* p1, const void* p2,
+                  const void* p3, const void* w, const void* b) {
+  const int64_t v = 16 / es;
+  return d % v == 0 && s1 % v == 0 && s2 % v == 0 && aligned_to(p1, 16) && aligned_to(p2, 16) &&
+                 aligned_to(p3, 16) && aligned_to(w, 16) && aligned_to(b, 16)
+             ? (int)v
+             : 1;
 }
 
-static int ln_parts(int64_t rows) { return (int)(rows < kLnParts ? (rows > 0 ? rows : 1) : kLnParts); }
+// Calls f.template operator()<K, G>() for the plan's team shape.
+template <int VEC, class F>
+static void ln_shapes(const LnPlan& p, F f) {
+  using std::integral_constant;
+#define QQT_LN(KK, GG) \
+  if (p.k == KK && p.g == GG) return f(integral_constant<int, KK>{}, integral_constant<int, GG>{})
+  QQT_LN(1, 8);
+  if constexpr (VEC == 8) {
+    QQT_LN(1, 16);
+    QQT_LN(1, 32);
+  } else {
+    QQT_LN(2, 8);
+    QQT_LN(2, 16);
+    QQT_LN(4, 32);
+    QQT_LN(8, 0);
+  }
+  if constexpr (VEC == 1) QQT_LN(16, 0);
+  QQT_LN(2, 32);
+  QQT_LN(1, 0);
+  QQT_LN(2, 0);
+  QQT_LN(4, 0);
+#undef QQT_LN
+}
 
 }  // namespace qqt
 
@@ -95,20 +475,43 @@ using namespace qqt;
 
 extern "C" uint64_t qqt_layernorm_work_bytes(int64_t rows, int64_t d) {
   if (rows < 0 || d <= 0) return 0;
-  return (uint64_t)ln_parts(rows) * 2 * (uint64_t)d * sizeof(float);
+  int64_t parts = 1;
+  for (int vec : {1, 4, 8}) {
+    const int64_t n = d % vec == 0 ? ln_parts(rows, d, vec) : 0;
+    parts = n > parts ? n : parts;
+  }
+  return (uint64_t)parts * 2 * (uint64_t)d * sizeof(float);
 }
 
 extern "C" int qqt_layernorm_forward(const void* x, int32_t dtype, int64_t rows, int64_t d,
                                      int64_t x_stride, const float* w, const float* b, float eps,
                                      void* y, float* mean, float* rstd, qqt_stream_t stream) {
   if (!dtype_ok(dtype) || rows < 0 || d <= 0 || x_stride < 0 || !(eps >= 0.f)) return QQT_E_ARG;
-  if (rows > 0x7fffffffll || d > 0x7fffffffll) return QQT_E_LIMIT;
+  if (rows > 0x7fffffffll || d > 0x3fffffffll) return QQT_E_LIMIT;
   if (rows == 0) return QQT_OK;
-  if (!x || !w || !y) return QQT_E_ARG;
-  return with_dtype(dtype, [&](auto t) {
-    using T = decltype(t);
-    k_ln_fwd<T><<<(unsigned)rows, 256, 0, (cudaStream_t)stream>>>((const T*)x, x_stride, d, w, b,
-                                                                  eps, (T*)y, mean, rstd);
+  if (!x || !w || !y || !mean != !rstd) return QQT_E_ARG;
+  return with_dtype(dtype, [&](auto e) {
+    using T = decltype(e);
+    constexpr int V = 16 / sizeof(T);
+    cudaStream_t st = (cudaStream_t)stream;
+    const int vec = ln_vec(sizeof(T), d, x_stride, 0, x, y, nullptr, w, b);
+    const LnPlan p = ln_plan(rows, d, vec, false);
+    if (p.blocks == 0) {
+      k_ln_long_fwd<T><<<(unsigned)rows, 1024, 0, st>>>((const T*)x, x_stride, d, w, b, eps, (T*)y,
+                                                        mean, rstd);
+      return launch_status();
+    }
+    auto run = [&](auto vv) {
+      ln_shapes<decltype(vv)::value>(p, [&](auto k, auto g) {
+        k_ln_fwd<T, decltype(vv)::value, decltype(k)::value, decltype(g)::value>
+            <<<(unsigned)p.blocks, p.threads, 0, st>>>((const T*)x, x_stride, rows, (int)d, w, b, eps,
+                                                       (T*)y, mean, rstd);
+      });
+    };
+    if (vec == 1)
+      run(std::integral_constant<int, 1>{});
+    else
+      run(std::integral_constant<int, V>{});
     return launch_status();
   });
 }
@@ -119,22 +522,48 @@ extern "C" int qqt_layernorm_backward(const void* dy, int64_t dy_stride, const v
                                       void* dx, float* dw, float* db, void* work,
                                       qqt_stream_t stream) {
   if (!dtype_ok(dtype) || rows < 0 || d <= 0 || x_stride < 0 || dy_stride < 0) return QQT_E_ARG;
-  if (rows > 0x7fffffffll || d > 0x7fffffffll) return QQT_E_LIMIT;
+  if (rows > 0x7fffffffll || d > 0x3fffffffll) return QQT_E_LIMIT;
   if (rows > 0 && (!dy || !x || !mean || !rstd || !w)) return QQT_E_ARG;
-  if ((dw || db) && !work) return QQT_E_ARG;
-  return with_dtype(dtype, [&](auto t) {
-    using T = decltype(t);
+  const bool sums = dw || db;
+  if (sums && !work) return QQT_E_ARG;
+  return with_dtype(dtype, [&](auto e) {
+    using T = decltype(e);
+    constexpr int V = 16 / sizeof(T);
     cudaStream_t st = (cudaStream_t)stream;
-    if (dx && rows > 0)
-      k_ln_dx<T><<<(unsigned)rows, 256, 0, st>>>((const T*)dy, dy_stride, (const T*)x, x_stride, d,
-                                                 mean, rstd, w, (T*)dx);
-    if (dw || db) {
-      const int parts = ln_parts(rows);
-      k_ln_dw_part<T><<<dim3((unsigned)((d + 127) / 128), parts), 128, 0, st>>>(
-          (const T*)dy, dy_stride, (const T*)x, x_stride, rows, d, mean, rstd, (float*)work);
-      k_ln_dw_sum<<<(unsigned)((2 * d + 127) / 128), 128, 0, st>>>((const float*)work, parts, d, dw,
-                                                                    db);
+    float* part = sums ? (float*)work : nullptr;
+    const int vec = ln_vec(sizeof(T), d, x_stride, dy_stride, x, dy, dx, w, nullptr);
+    const LnPlan p = ln_plan(rows, d, vec, true);
+    int64_t parts = 0;
+    if (rows > 0 && (dx || sums)) {
+      if (p.blocks == 0) {
+        if (dx)
+          k_ln_long_dx<T><<<(unsigned)rows, 1024, 0, st>>>((const T*)dy, dy_stride, (const T*)x,
+                                                           x_stride, d, mean, rstd, w, (T*)dx);
+        if (sums) {
+          parts = ln_parts(rows, d, vec);
+          k_ln_long_part<T><<<dim3((unsigned)((d + 127) / 128), (unsigned)parts), 128, 0, st>>>(
+              (const T*)dy, dy_stride, (const T*)x, x_stride, rows, d, mean, rstd, part);
+        }
+      } else {
+        parts = p.blocks;
+        auto run = [&](auto vv) {
+          ln_shapes<decltype(vv)::value>(p, [&](auto k, auto g) {
+            constexpr int G = decltype(g)::value;
+            const size_t smem = G ? (size_t)(kLnWarpThreads / (G ? G : 1)) * 2 * d * 4 : 0;
+            k_ln_bwd<T, decltype(vv)::value, decltype(k)::value, G>
+                <<<(unsigned)p.blocks, p.threads, smem, st>>>((const T*)dy, dy_stride, (const T*)x,
+                                                              x_stride, rows, (int)d, mean, rstd, w,
+                                                              (T*)dx, part);
+          });
+        };
+        if (vec == 1)
+          run(std::integral_constant<int, 1>{});
+        else
+          run(std::integral_constant<int, V>{});
+      }
     }
+    if (sums)
+      k_ln_add<<<(unsigned)((2 * d + 31) / 32), 512, 0, st>>>(part, (int)parts, d, dw, db);
     return launch_status();
   });
 }
