@@ -23,18 +23,13 @@
 namespace qqt {
 
 constexpr int kLnWarpThreads = 256;   // block of the teams inside a warp
-#ifndef LN_FWD_G
-#define LN_FWD_G 8
-#endif
-#ifndef LN_BWD_G
-#define LN_BWD_G 4
-#endif
-#ifndef LN_FWD_B
-#define LN_FWD_B 2048
-#endif
-#ifndef LN_BWD_B
-#define LN_BWD_B 1024
-#endif
+// Blocks of an SM that walk over rows.  Forward more than are resident (rows
+// are short, the last blocks even out: 180 against 187 us with 8 at 1048576 x
+// 128 f32); backward as many as are resident with 80 registers, since every
+// block ends in a partial row (250 us with 3, 294 with 4 that do not all fit).
+constexpr int kLnFwdBlocks = 16, kLnBwdBlocks = 3;
+// Threads of an SM in blocks that take a row each, 16 or 32 elements a thread.
+constexpr int kLnRowThreads16 = 768, kLnRowThreads32 = 512;
 
 // Largest block that walks rows with e elements a thread: the backward pass
 // keeps 2 e sums besides its operands.
@@ -84,44 +79,79 @@ __device__ __forceinline__ LnTeam ln_team() {
   return t;
 }
 
-template <class T, int VEC, int K>
-__device__ __forceinline__ void ln_load(const T* p, const LnTeam& t, int nv, bool on,
-                                        Vec<T, VEC>* out) {
+// Vector j of a row of d values.  Without WHOLE the row may begin anywhere and
+// end inside a vector: it goes element by element, zeros past its end.
+template <class T, int VEC, bool WHOLE>
+__device__ __forceinline__ Vec<T, VEC> ln_get(const T* p, int j, int d) {
+  if constexpr (WHOLE) {
+    return ld_vec<T, VEC>(p + (int64_t)j * VEC);
+  } else {
+    float f[VEC];
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int j = t.j + k * t.step;
-    out[k] = on && j < nv ? ld_vec<T, VEC>(p + (int64_t)j * VEC) : vec_zero<T, VEC>();
+    for (int v = 0; v < VEC; ++v) f[v] = j * VEC + v < d ? to_f(p[(int64_t)j * VEC + v]) : 0.f;
+    Vec<T, VEC> r;
+    r.put(f);
+    return r;
   }
 }
-template <int VEC>
-__device__ __forceinline__ Vec<float, VEC> ln_param(const float* p, int j) {
-  Vec<float, VEC> r;
-  if constexpr (VEC == 8) {
+template <class T, int VEC, bool WHOLE>
+__device__ __forceinline__ void ln_put(T* p, int j, int d, const float* f) {
+  if constexpr (WHOLE) {
+    Vec<T, VEC> r;
+    r.put(f);
+    st_vec(p + (int64_t)j * VEC, r);
+  } else {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v)
+      if (j * VEC + v < d) p[(int64_t)j * VEC + v] = from_f<T>(f[v]);
+  }
+}
+template <int VEC, bool WHOLE>
+__device__ __forceinline__ Vec<float, VEC> ln_param(const float* p, int j, int d) {
+  if constexpr (WHOLE && VEC == 8) {
+    Vec<float, VEC> r;
     const float4 lo = *reinterpret_cast<const float4*>(p + j * 8);
     const float4 hi = *reinterpret_cast<const float4*>(p + j * 8 + 4);
     const float f[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
     r.put(f);
+    return r;
   } else {
-    r = ld_vec<float, VEC>(p + j * VEC);
+    return ln_get<float, VEC, WHOLE>(p, j, d);
   }
-  return r;
+}
+template <class T, int VEC, int K, bool WHOLE>
+__device__ __forceinline__ void ln_load(const T* p, const LnTeam& t, int nv, int d, bool on,
+                                        Vec<T, VEC>* out) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int j = t.j + k * t.step;
+    out[k] = on && j < nv ? ln_get<T, VEC, WHOLE>(p, j, d) : vec_zero<T, VEC>();
+  }
+}
+// The scaled and shifted row.
+template <int VEC>
+__device__ __forceinline__ void ln_scale(const float* c, float rs, const Vec<float, VEC>& w,
+                                         bool has_b, const Vec<float, VEC>& b, float* o) {
+#pragma unroll
+  for (int v = 0; v < VEC; ++v)
+    o[v] = has_b ? fmaf(c[v] * rs, w.get(v), b.get(v)) : c[v] * rs * w.get(v);
 }
 
-template <class T, int VEC, int K, int G>
+template <class T, int VEC, int K, int G, bool WHOLE>
 __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K))
     k_ln_fwd(const T* __restrict__ x, int64_t xs, int64_t rows, int d, const float* __restrict__ w,
              const float* __restrict__ b, float eps, T* __restrict__ y, float* __restrict__ mean,
              float* __restrict__ rstd) {
   __shared__ float buf[2][1][32];
   int turn = 0;
-  const int nv = d / VEC;
+  const int nv = (d + VEC - 1) / VEC;
   const float inv_d = 1.f / (float)d;
   LnTeam t = ln_team<G>();
   // (a team's lanes shuffle together with the rest of their warp, so a warp
   // goes on until its last team is done)
   const int64_t lead = G && G < 32 ? t.row - (threadIdx.x % 32) / (G ? G : 1) : t.row;
   Vec<T, VEC> c[K];
-  ln_load<T, VEC, K>(x + t.row * xs, t, nv, t.row < rows, c);
+  ln_load<T, VEC, K, WHOLE>(x + t.row * xs, t, nv, d, t.row < rows, c);
   for (int64_t lr = lead; lr < rows; lr += t.rows_step) {
     const bool on = t.row < rows;
     float f[K][VEC];
@@ -135,7 +165,7 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K))
       }
     // the next row's values are on their way meanwhile
     const int64_t next = t.row + t.rows_step;
-    ln_load<T, VEC, K>(x + next * xs, t, nv, next < rows, c);
+    ln_load<T, VEC, K, WHOLE>(x + next * xs, t, nv, d, next < rows, c);
     team_sum<G, 1>(s, buf, turn);
     const float mu = s[0] * inv_d;
     s[0] = 0.f;
@@ -144,7 +174,7 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K))
       if (t.j + k * t.step < nv)
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-          f[k][v] -= mu;
+          f[k][v] = WHOLE || (t.j + k * t.step) * VEC + v < d ? f[k][v] - mu : 0.f;
           s[0] = fmaf(f[k][v], f[k][v], s[0]);
         }
     team_sum<G, 1>(s, buf, turn);
@@ -154,19 +184,11 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K))
       for (int k = 0; k < K; ++k) {
         const int j = t.j + k * t.step;
         if (j < nv) {
-          const Vec<float, VEC> wv = ln_param<VEC>(w, j);
+          const Vec<float, VEC> wv = ln_param<VEC, WHOLE>(w, j, d);
+          const Vec<float, VEC> bv = b ? ln_param<VEC, WHOLE>(b, j, d) : wv;
           float o[VEC];
-          if (b) {
-            const Vec<float, VEC> bv = ln_param<VEC>(b, j);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) o[v] = fmaf(f[k][v] * rs, wv.get(v), bv.get(v));
-          } else {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) o[v] = f[k][v] * rs * wv.get(v);
-          }
-          Vec<T, VEC> out;
-          out.put(o);
-          st_vec(y + t.row * d + (int64_t)j * VEC, out);
+          ln_scale<VEC>(f[k], rs, wv, b != nullptr, bv, o);
+          ln_put<T, VEC, WHOLE>(y + t.row * d, j, d, o);
         }
       }
       if (t.j == 0 && mean) {
@@ -179,15 +201,15 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K))
 }
 
 // dx of the team's rows, and the block's partial sums of dy xh and dy.
-template <class T, int VEC, int K, int G>
-__global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K))
+template <class T, int VEC, int K, int G, bool WHOLE>
+__global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K), G ? kLnBwdBlocks : 1)
     k_ln_bwd(const T* __restrict__ dy, int64_t dys, const T* __restrict__ x, int64_t xs,
              int64_t rows, int d, const float* __restrict__ mean, const float* __restrict__ rstd,
              const float* __restrict__ w, T* __restrict__ dx, float* __restrict__ part) {
   __shared__ float buf[2][2][32];
   extern __shared__ float sums[];          // teams inside a warp: [teams][2 d]
   int turn = 0;
-  const int nv = d / VEC;
+  const int nv = (d + VEC - 1) / VEC;
   const float inv_d = 1.f / (float)d;
   LnTeam t = ln_team<G>();
   const int64_t lead = G && G < 32 ? t.row - (threadIdx.x % 32) / (G ? G : 1) : t.row;
@@ -200,8 +222,8 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K))
   // is loaded meanwhile.  Many: they are made again from the packed operands.
   constexpr bool KEEP = VEC * K <= 8;
   Vec<T, VEC> cx[K], cy[K];
-  ln_load<T, VEC, K>(x + t.row * xs, t, nv, t.row < rows, cx);
-  ln_load<T, VEC, K>(dy + t.row * dys, t, nv, t.row < rows, cy);
+  ln_load<T, VEC, K, WHOLE>(x + t.row * xs, t, nv, d, t.row < rows, cx);
+  ln_load<T, VEC, K, WHOLE>(dy + t.row * dys, t, nv, d, t.row < rows, cy);
   float mu = t.row < rows ? mean[t.row] : 0.f, rs = t.row < rows ? rstd[t.row] : 0.f;
   for (int64_t lr = lead; lr < rows; lr += t.rows_step) {
     const bool on = t.row < rows;
@@ -212,7 +234,7 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K))
     for (int k = 0; k < K; ++k) {
       const int j = t.j + k * t.step;
       if (j < nv) {
-        const Vec<float, VEC> wv = ln_param<VEC>(w, j);
+        const Vec<float, VEC> wv = ln_param<VEC, WHOLE>(w, j, d);
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
           const float g = cy[k].get(v), xh = (cx[k].get(v) - m0) * r0, q = g * wv.get(v);
@@ -229,8 +251,8 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K))
     }
     const int64_t next = t.row + t.rows_step;
     auto load_next = [&] {
-      ln_load<T, VEC, K>(x + next * xs, t, nv, next < rows, cx);
-      ln_load<T, VEC, K>(dy + next * dys, t, nv, next < rows, cy);
+      ln_load<T, VEC, K, WHOLE>(x + next * xs, t, nv, d, next < rows, cx);
+      ln_load<T, VEC, K, WHOLE>(dy + next * dys, t, nv, d, next < rows, cy);
       if (next < rows) {
         mu = mean[next];
         rs = rstd[next];
@@ -250,14 +272,12 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K))
             for (int v = 0; v < VEC; ++v)
               o[v] = r0 * (fmaf(-xk[KEEP ? k : 0][v], m2, qk[KEEP ? k : 0][v]) - m1);
           } else {
-            const Vec<float, VEC> wv = ln_param<VEC>(w, j);
+            const Vec<float, VEC> wv = ln_param<VEC, WHOLE>(w, j, d);
 #pragma unroll
             for (int v = 0; v < VEC; ++v)
               o[v] = r0 * (fmaf(-(cx[k].get(v) - m0) * r0, m2, cy[k].get(v) * wv.get(v)) - m1);
           }
-          Vec<T, VEC> out;
-          out.put(o);
-          st_vec(dx + t.row * d + (int64_t)j * VEC, out);
+          ln_put<T, VEC, WHOLE>(dx + t.row * d, j, d, o);
         }
       }
       if (!KEEP) load_next();
@@ -272,10 +292,11 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K))
       const int j = t.j + k * t.step;
       if (j < nv)
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          pw[j * VEC + v] = aw[k][v];
-          pw[d + j * VEC + v] = ab[k][v];
-        }
+        for (int v = 0; v < VEC; ++v)
+          if (WHOLE || j * VEC + v < d) {
+            pw[j * VEC + v] = aw[k][v];
+            pw[d + j * VEC + v] = ab[k][v];
+          }
     }
     return;
   }
@@ -286,10 +307,11 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K))
     const int j = t.j + k * t.step;
     if (j < nv)
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        mine[j * VEC + v] = aw[k][v];
-        mine[d + j * VEC + v] = ab[k][v];
-      }
+      for (int v = 0; v < VEC; ++v)
+        if (WHOLE || j * VEC + v < d) {
+          mine[j * VEC + v] = aw[k][v];
+          mine[d + j * VEC + v] = ab[k][v];
+        }
   }
   __syncthreads();
   for (int c = threadIdx.x; c < 2 * d; c += kLnWarpThreads) {
@@ -300,25 +322,249 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K))
   }
 }
 
-// Adds the partial rows: a block takes 32 columns, each of its warps every
-// (number of warps)-th row.
-__global__ void __launch_bounds__(512) k_ln_add(const float* __restrict__ part, int n_part, int64_t d,
-                                                float* __restrict__ dw, float* __restrict__ db) {
-  __shared__ float buf[16][33];
+// ------------------------------------------- a block per row, rows staged
+//
+// Rows of whole 16-byte vectors beyond a warp's reach: a block walks over rows,
+// bulk copies bring the next ones into a ring of stages in shared memory
+// meanwhile, and the block's threads hold K vectors each.  A register holds
+// one row's values at most, the ring the 2 to 8 rows that keep the memory
+// system busy across the block's barriers.
+
+constexpr int kLnStages = 8;
+struct LnRing {
+  int stages;
+  uint32_t stage_bytes, row_bytes;
+};
+
+template <class T, int VEC, int K>
+__global__ void __launch_bounds__(ln_max_threads(VEC* K))
+    k_ln_row_fwd(const T* __restrict__ x, int64_t xs, int64_t rows, int d,
+                 const float* __restrict__ w, const float* __restrict__ b, float eps,
+                 T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd, LnRing ring) {
+  extern __shared__ __align__(128) unsigned char stage[];
+  __shared__ uint64_t bar[kLnStages];
+  __shared__ float buf[2][1][32];
+  int turn = 0;
+  const int nv = (d + VEC - 1) / VEC;
+  const float inv_d = 1.f / (float)d;
+  auto fetch = [&](int64_t row, int s) {
+    if (row < rows) {
+      stage_arm(&bar[s], ring.row_bytes);
+      stage_copy(stage + (size_t)s * ring.stage_bytes, x + row * xs, ring.row_bytes, &bar[s]);
+    }
+  };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ring.stages; ++s) stage_init(&bar[s]);
+    stage_init_done();
+  }
+  __syncthreads();
+  if (threadIdx.x == 0)
+    for (int s = 0; s < ring.stages; ++s) fetch(blockIdx.x + (int64_t)s * gridDim.x, s);
+  // a block's columns do not change: weight and bias stay in registers
+  Vec<float, VEC> wr[K], br[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int j = threadIdx.x + k * blockDim.x;
+    wr[k] = j < nv ? ln_param<VEC, true>(w, j, d) : vec_zero<float, VEC>();
+    br[k] = j < nv && b ? ln_param<VEC, true>(b, j, d) : vec_zero<float, VEC>();
+  }
+  int s = 0;
+  uint32_t parity = 0;
+  bool alive = true;
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    if (alive) alive = stage_wait(&bar[s], parity);
+    const T* in = (const T*)(stage + (size_t)s * ring.stage_bytes);
+    float f[K][VEC];
+    float sum[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int j = threadIdx.x + k * blockDim.x;
+      if (j < nv) {
+        const Vec<T, VEC> c = ld_vec<T, VEC>(in + j * VEC);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          f[k][v] = c.get(v);
+          sum[0] += f[k][v];
+        }
+      }
+    }
+    team_sum<0, 1>(sum, buf, turn);        // (its barrier: everyone has read the stage)
+    if (threadIdx.x == 0) fetch(row + (int64_t)ring.stages * gridDim.x, s);
+    const float mu = sum[0] * inv_d;
+    sum[0] = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (threadIdx.x + k * blockDim.x < nv)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          f[k][v] -= mu;
+          sum[0] = fmaf(f[k][v], f[k][v], sum[0]);
+        }
+    team_sum<0, 1>(sum, buf, turn);
+    const float rs = 1.f / sqrtf(sum[0] * inv_d + eps);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int j = threadIdx.x + k * blockDim.x;
+      if (j < nv) {
+        float o[VEC];
+        ln_scale<VEC>(f[k], rs, wr[k], b != nullptr, br[k], o);
+        ln_put<T, VEC, true>(y + row * d, j, d, o);
+      }
+    }
+    if (threadIdx.x == 0 && mean) {
+      mean[row] = mu;
+      rstd[row] = rs;
+    }
+    if (++s == ring.stages) {
+      s = 0;
+      parity ^= 1;
+    }
+  }
+}
+
+template <class T, int VEC, int K>
+__global__ void __launch_bounds__(ln_max_threads(VEC* K))
+    k_ln_row_bwd(const T* __restrict__ dy, int64_t dys, const T* __restrict__ x, int64_t xs,
+                 int64_t rows, int d, const float* __restrict__ mean,
+                 const float* __restrict__ rstd, const float* __restrict__ w, T* __restrict__ dx,
+                 float* __restrict__ part, LnRing ring) {
+  extern __shared__ __align__(128) unsigned char stage[];
+  __shared__ uint64_t bar[kLnStages];
+  __shared__ float buf[2][2][32];
+  int turn = 0;
+  const int nv = (d + VEC - 1) / VEC;
+  const float inv_d = 1.f / (float)d;
+  constexpr bool WREG = VEC * K <= 16;     // the weights fit beside the sums
+  auto fetch = [&](int64_t row, int s) {
+    if (row < rows) {
+      unsigned char* to = stage + (size_t)s * ring.stage_bytes;
+      stage_arm(&bar[s], 2 * ring.row_bytes);
+      stage_copy(to, x + row * xs, ring.row_bytes, &bar[s]);
+      stage_copy(to + ring.stage_bytes / 2, dy + row * dys, ring.row_bytes, &bar[s]);
+    }
+  };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ring.stages; ++s) stage_init(&bar[s]);
+    stage_init_done();
+  }
+  __syncthreads();
+  if (threadIdx.x == 0)
+    for (int s = 0; s < ring.stages; ++s) fetch(blockIdx.x + (int64_t)s * gridDim.x, s);
+  float aw[K][VEC], ab[K][VEC], wr[WREG ? K : 1][VEC];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int j = threadIdx.x + k * blockDim.x;
+    Vec<float, VEC> wv = vec_zero<float, VEC>();
+    if (WREG && j < nv) wv = ln_param<VEC, true>(w, j, d);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      aw[k][v] = ab[k][v] = 0.f;
+      if (WREG) wr[WREG ? k : 0][v] = wv.get(v);
+    }
+  }
+  int s = 0, before = -1;                  // before: the stage of the row before
+  uint32_t parity = 0;
+  bool alive = true;
+  float mu = 0.f, rs = 0.f;
+  if (blockIdx.x < rows) {
+    mu = mean[blockIdx.x];
+    rs = rstd[blockIdx.x];
+  }
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const float m0 = mu, r0 = rs;
+    const int64_t next = row + gridDim.x;
+    if (next < rows) {
+      mu = mean[next];
+      rs = rstd[next];
+    }
+    if (alive) alive = stage_wait(&bar[s], parity);
+    const T* ix = (const T*)(stage + (size_t)s * ring.stage_bytes);
+    const T* iy = (const T*)((const unsigned char*)ix + ring.stage_bytes / 2);
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int j = threadIdx.x + k * blockDim.x;
+      if (j < nv) {
+        const Vec<T, VEC> cx = ld_vec<T, VEC>(ix + j * VEC), cy = ld_vec<T, VEC>(iy + j * VEC);
+        Vec<float, VEC> wv;
+        if (!WREG) wv = ln_param<VEC, true>(w, j, d);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          const float g = cy.get(v), xh = (cx.get(v) - m0) * r0;
+          const float q = g * (WREG ? wr[WREG ? k : 0][v] : wv.get(v));
+          ab[k][v] += g;
+          aw[k][v] = fmaf(g, xh, aw[k][v]);
+          sum[0] += q;
+          sum[1] = fmaf(q, xh, sum[1]);
+        }
+      }
+    }
+    if (dx)
+      team_sum<0, 2>(sum, buf, turn);      // (its barrier: the row before is done with)
+    else
+      __syncthreads();
+    if (threadIdx.x == 0 && before >= 0)
+      fetch(row + (int64_t)(ring.stages - 1) * gridDim.x, before);
+    if (dx) {
+      const float m1 = sum[0] * inv_d, m2 = sum[1] * inv_d;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int j = threadIdx.x + k * blockDim.x;
+        if (j < nv) {
+          const Vec<T, VEC> cx = ld_vec<T, VEC>(ix + j * VEC), cy = ld_vec<T, VEC>(iy + j * VEC);
+          Vec<float, VEC> wv;
+          if (!WREG) wv = ln_param<VEC, true>(w, j, d);
+          float o[VEC];
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) {
+            const float q = cy.get(v) * (WREG ? wr[WREG ? k : 0][v] : wv.get(v));
+            o[v] = r0 * (fmaf(-(cx.get(v) - m0) * r0, m2, q) - m1);
+          }
+          ln_put<T, VEC, true>(dx + row * d, j, d, o);
+        }
+      }
+    }
+    before = s;
+    if (++s == ring.stages) {
+      s = 0;
+      parity ^= 1;
+    }
+  }
+  if (!part) return;
+  float* pw = part + (int64_t)blockIdx.x * 2 * d;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int j = threadIdx.x + k * blockDim.x;
+    if (j < nv)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        pw[j * VEC + v] = aw[k][v];
+        pw[d + j * VEC + v] = ab[k][v];
+      }
+  }
+}
+
+// Adds the partial rows: a block takes 32 columns, each of its 32 warps every
+// 32nd row.
+__global__ void __launch_bounds__(1024) k_ln_add(const float* __restrict__ part, int n_part,
+                                                 int64_t d, float* __restrict__ dw,
+                                                 float* __restrict__ db) {
+  __shared__ float buf[32][33];
   const int64_t c = (int64_t)blockIdx.x * 32 + lane_id();
+  const float* p = part + (int64_t)warp_id() * 2 * d + c;
   float s = 0.f;
   if (c < 2 * d) {
-#pragma unroll 8
-    for (int p = warp_id(); p < n_part; p += 16) s += part[(int64_t)p * 2 * d + c];
+#pragma unroll 16
+    for (int r = warp_id(); r < n_part; r += 32, p += 64 * d) s += *p;
   }
   buf[warp_id()][lane_id()] = s;
   __syncthreads();
-  if (warp_id() == 0 && c < 2 * d) {
-    s = 0.f;
-#pragma unroll
-    for (int q = 0; q < 16; ++q) s += buf[q][lane_id()];
-    float* out = c < d ? dw : db;
-    if (out) out[c < d ? c : c - d] = s;
+  // column w of the 32 is warp w's to add
+  s = warp_sum_f(buf[lane_id()][warp_id()]);
+  const int64_t col = (int64_t)blockIdx.x * 32 + warp_id();
+  if (lane_id() == 0 && col < 2 * d) {
+    float* out = col < d ? dw : db;
+    if (out) out[col < d ? col : col - d] = s;
   }
 }
 
@@ -389,11 +635,13 @@ __global__ void k_ln_long_part(const T* __restrict__ dy, int64_t dys, const T* _
   part[(int64_t)blockIdx.y * 2 * d + d + j] = sb;
 }
 
-// How rows are handed out: vectors of vec elements, k of them a thread, teams
-// of g lanes (0: a block of `threads`), `blocks` blocks that walk over rows.
+// How rows are handed out: k vectors a thread, teams of g lanes (0: a block of
+// `threads`), `blocks` blocks that walk over rows (0: rows too long for them).
+// It does not depend on alignment, so neither do results.
 struct LnPlan {
-  int vec, k, g, threads;
+  int k, g, threads;
   int64_t blocks;
+  LnRing ring;
 };
 static int ln_sms() {
   static std::atomic<int> n{0};
@@ -408,26 +656,36 @@ static int ln_sms() {
   return v;
 }
 static LnPlan ln_plan(int64_t rows, int64_t d, int vec, bool bwd) {
-  LnPlan p{vec, 0, 0, kLnWarpThreads, 0};
-  const int64_t nv = d / vec;
-  int64_t per_block;
+  LnPlan p{0, 0, kLnWarpThreads, 0, {0, 0, 0}};
+  const int64_t nv = (d + vec - 1) / vec;
+  const int sms = ln_sms();
   if (nv <= (vec == 8 ? 64 : 128)) {       // a team inside a warp
     const bool one = vec == 8 || nv <= 8;
     p.k = one ? 1 : 2;
     p.g = nv <= 8 * p.k ? 8 : nv <= 16 * p.k ? 16 : 32;
     if (nv > 32 * p.k) p.k *= 2;
-    per_block = kLnWarpThreads / p.g;
-  } else {                                 // a block: as few vectors a thread as its size allows
-    p.k = 1;
-    while (p.k * vec < 32 && nv > (int64_t)p.k * ln_max_threads(p.k * vec)) p.k *= 2;
-    const int64_t th = (nv + p.k - 1) / p.k;
-    if (p.k * vec > (vec == 1 ? 16 : 32) || th > ln_max_threads(p.k * vec)) return p;   // too long
-    p.threads = (int)((th + 31) / 32 * 32);
-    per_block = 1;
+    const int64_t per_block = kLnWarpThreads / p.g, need = (rows + per_block - 1) / per_block;
+    const int64_t room = (int64_t)sms * (bwd ? kLnBwdBlocks : kLnFwdBlocks);
+    p.blocks = need < room ? need : room;
+    return p;
   }
-  const int64_t need = (rows + per_block - 1) / per_block;
-  const int64_t room = (int64_t)ln_sms() * (p.g ? (bwd ? LN_BWD_G : LN_FWD_G) : (bwd ? LN_BWD_B : LN_FWD_B) / p.threads + 1);
-  p.blocks = need < room ? need : room;
+  // a block: 16 elements a thread, 32 where that takes too many threads
+  p.k = 16 / vec;
+  if (nv > (int64_t)p.k * ln_max_threads(16)) p.k *= 2;
+  const int64_t th = (nv + p.k - 1) / p.k;
+  if (th > ln_max_threads(p.k * vec)) return p;         // too long
+  p.threads = (int)((th + 31) / 32 * 32);
+  // blocks of an SM by the threads that the registers allow, and stages by the
+  // shared memory that leaves each
+  const int room = p.k * vec == 16 ? kLnRowThreads16 : kLnRowThreads32;
+  int per_sm = room / p.threads;
+  per_sm = per_sm < 1 ? 1 : per_sm > 16 ? 16 : per_sm;
+  const int64_t row = d * (16 / vec), stage = (row + 127) / 128 * 128 * (bwd ? 2 : 1);
+  int64_t n = 220 * 1024 / per_sm / stage;
+  while (n < 3 && per_sm > 1) n = 220 * 1024 / --per_sm / stage;
+  if (n < 2) return p;                                  // too long for two stages
+  p.ring = {(int)(n > kLnStages ? kLnStages : n), (uint32_t)stage, (uint32_t)row};
+  p.blocks = rows < (int64_t)sms * per_sm ? rows : (int64_t)sms * per_sm;
   return p;
 }
 static int64_t ln_parts(int64_t rows, int64_t d, int vec) {
@@ -435,37 +693,37 @@ static int64_t ln_parts(int64_t rows, int64_t d, int vec) {
   if (p.blocks > 0) return p.blocks;
   return rows < 512 ? (rows > 0 ? rows : 1) : 512;
 }
-// Vector width that rows of these strides and addresses allow.
-static int ln_vec(int64_t es, int64_t d, int64_t s1, int64_t s2, const void* p1, const void* p2,
-                  const void* p3, const void* w, const void* b) {
+// Whether rows of these strides and addresses are made of whole 16-byte vectors.
+static bool ln_whole(int64_t es, int64_t d, int64_t s1, int64_t s2, const void* p1, const void* p2,
+                     const void* p3, const void* w, const void* b) {
   const int64_t v = 16 / es;
   return d % v == 0 && s1 % v == 0 && s2 % v == 0 && aligned_to(p1, 16) && aligned_to(p2, 16) &&
-                 aligned_to(p3, 16) && aligned_to(w, 16) && aligned_to(b, 16)
-             ? (int)v
-             : 1;
+         aligned_to(p3, 16) && aligned_to(w, 16) && aligned_to(b, 16);
 }
 
-// Calls f.template operator()<K, G>() for the plan's team shape.
+static bool ln_allow_smem(const void* kernel, size_t bytes) {
+  return bytes <= 48 * 1024 ||
+         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) ==
+             cudaSuccess;
+}
 template <int VEC, class F>
 static void ln_shapes(const LnPlan& p, F f) {
   using std::integral_constant;
 #define QQT_LN(KK, GG) \
   if (p.k == KK && p.g == GG) return f(integral_constant<int, KK>{}, integral_constant<int, GG>{})
   QQT_LN(1, 8);
+  QQT_LN(2, 32);
+  QQT_LN(4, 0);
   if constexpr (VEC == 8) {
     QQT_LN(1, 16);
     QQT_LN(1, 32);
+    QQT_LN(2, 0);
   } else {
     QQT_LN(2, 8);
     QQT_LN(2, 16);
     QQT_LN(4, 32);
     QQT_LN(8, 0);
   }
-  if constexpr (VEC == 1) QQT_LN(16, 0);
-  QQT_LN(2, 32);
-  QQT_LN(1, 0);
-  QQT_LN(2, 0);
-  QQT_LN(4, 0);
 #undef QQT_LN
 }
 
@@ -475,11 +733,8 @@ using namespace qqt;
 
 extern "C" uint64_t qqt_layernorm_work_bytes(int64_t rows, int64_t d) {
   if (rows < 0 || d <= 0) return 0;
-  int64_t parts = 1;
-  for (int vec : {1, 4, 8}) {
-    const int64_t n = d % vec == 0 ? ln_parts(rows, d, vec) : 0;
-    parts = n > parts ? n : parts;
-  }
+  const int64_t p4 = ln_parts(rows, d, 4), p8 = ln_parts(rows, d, 8);
+  const int64_t parts = p4 > p8 ? p4 : p8;
   return (uint64_t)parts * 2 * (uint64_t)d * sizeof(float);
 }
 
@@ -494,24 +749,30 @@ extern "C" int qqt_layernorm_forward(const void* x, int32_t dtype, int64_t rows,
     using T = decltype(e);
     constexpr int V = 16 / sizeof(T);
     cudaStream_t st = (cudaStream_t)stream;
-    const int vec = ln_vec(sizeof(T), d, x_stride, 0, x, y, nullptr, w, b);
-    const LnPlan p = ln_plan(rows, d, vec, false);
+    const bool whole = ln_whole(sizeof(T), d, x_stride, 0, x, y, nullptr, w, b);
+    const LnPlan p = ln_plan(rows, d, V, false);
+    const T* xp = (const T*)x;
+    T* yp = (T*)y;
+    const unsigned blocks = (unsigned)p.blocks;
     if (p.blocks == 0) {
-      k_ln_long_fwd<T><<<(unsigned)rows, 1024, 0, st>>>((const T*)x, x_stride, d, w, b, eps, (T*)y,
-                                                        mean, rstd);
+      k_ln_long_fwd<T><<<(unsigned)rows, 1024, 0, st>>>(xp, x_stride, d, w, b, eps, yp, mean, rstd);
       return launch_status();
     }
-    auto run = [&](auto vv) {
-      ln_shapes<decltype(vv)::value>(p, [&](auto k, auto g) {
-        k_ln_fwd<T, decltype(vv)::value, decltype(k)::value, decltype(g)::value>
-            <<<(unsigned)p.blocks, p.threads, 0, st>>>((const T*)x, x_stride, rows, (int)d, w, b, eps,
-                                                       (T*)y, mean, rstd);
-      });
-    };
-    if (vec == 1)
-      run(std::integral_constant<int, 1>{});
-    else
-      run(std::integral_constant<int, V>{});
+    ln_shapes<V>(p, [&](auto kk, auto gg) {
+      constexpr int K = decltype(kk)::value, G = decltype(gg)::value;
+      if (!whole) {
+        k_ln_fwd<T, V, K, G, false><<<blocks, p.threads, 0, st>>>(xp, x_stride, rows, (int)d, w, b, eps,
+                                                                  yp, mean, rstd);
+      } else if constexpr (G == 0) {
+        const size_t smem = (size_t)p.ring.stages * p.ring.stage_bytes;
+        if (ln_allow_smem((const void*)k_ln_row_fwd<T, V, K>, smem))
+          k_ln_row_fwd<T, V, K><<<blocks, p.threads, smem, st>>>(xp, x_stride, rows, (int)d, w, b, eps,
+                                                                 yp, mean, rstd, p.ring);
+      } else {
+        k_ln_fwd<T, V, K, G, true><<<blocks, p.threads, 0, st>>>(xp, x_stride, rows, (int)d, w, b, eps,
+                                                                 yp, mean, rstd);
+      }
+    });
     return launch_status();
   });
 }
@@ -531,39 +792,39 @@ extern "C" int qqt_layernorm_backward(const void* dy, int64_t dy_stride, const v
     constexpr int V = 16 / sizeof(T);
     cudaStream_t st = (cudaStream_t)stream;
     float* part = sums ? (float*)work : nullptr;
-    const int vec = ln_vec(sizeof(T), d, x_stride, dy_stride, x, dy, dx, w, nullptr);
-    const LnPlan p = ln_plan(rows, d, vec, true);
-    int64_t parts = 0;
-    if (rows > 0 && (dx || sums)) {
-      if (p.blocks == 0) {
-        if (dx)
-          k_ln_long_dx<T><<<(unsigned)rows, 1024, 0, st>>>((const T*)dy, dy_stride, (const T*)x,
-                                                           x_stride, d, mean, rstd, w, (T*)dx);
-        if (sums) {
-          parts = ln_parts(rows, d, vec);
-          k_ln_long_part<T><<<dim3((unsigned)((d + 127) / 128), (unsigned)parts), 128, 0, st>>>(
-              (const T*)dy, dy_stride, (const T*)x, x_stride, rows, d, mean, rstd, part);
+    const bool whole = ln_whole(sizeof(T), d, x_stride, dy_stride, x, dy, dx, w, nullptr);
+    const LnPlan p = ln_plan(rows, d, V, true);
+    const T *xp = (const T*)x, *yp = (const T*)dy;
+    T* gp = (T*)dx;
+    const unsigned blocks = (unsigned)p.blocks;
+    const int64_t parts = rows > 0 ? ln_parts(rows, d, V) : 0;
+    if (rows > 0 && p.blocks == 0) {
+      if (dx)
+        k_ln_long_dx<T><<<(unsigned)rows, 1024, 0, st>>>(yp, dy_stride, xp, x_stride, d, mean, rstd, w,
+                                                         gp);
+      if (sums)
+        k_ln_long_part<T><<<dim3((unsigned)((d + 127) / 128), (unsigned)parts), 128, 0, st>>>(
+            yp, dy_stride, xp, x_stride, rows, d, mean, rstd, part);
+    } else if (rows > 0 && (dx || sums)) {
+      ln_shapes<V>(p, [&](auto kk, auto gg) {
+        constexpr int K = decltype(kk)::value, G = decltype(gg)::value;
+        size_t smem = G ? (size_t)(kLnWarpThreads / (G ? G : 1)) * 2 * d * 4 : 0;
+        if (!whole) {
+          k_ln_bwd<T, V, K, G, false><<<blocks, p.threads, smem, st>>>(
+              yp, dy_stride, xp, x_stride, rows, (int)d, mean, rstd, w, gp, part);
+        } else if constexpr (G == 0) {
+          smem = (size_t)p.ring.stages * p.ring.stage_bytes;
+          if (ln_allow_smem((const void*)k_ln_row_bwd<T, V, K>, smem))
+            k_ln_row_bwd<T, V, K><<<blocks, p.threads, smem, st>>>(
+                yp, dy_stride, xp, x_stride, rows, (int)d, mean, rstd, w, gp, part, p.ring);
+        } else {
+          k_ln_bwd<T, V, K, G, true><<<blocks, p.threads, smem, st>>>(
+              yp, dy_stride, xp, x_stride, rows, (int)d, mean, rstd, w, gp, part);
         }
-      } else {
-        parts = p.blocks;
-        auto run = [&](auto vv) {
-          ln_shapes<decltype(vv)::value>(p, [&](auto k, auto g) {
-            constexpr int G = decltype(g)::value;
-            const size_t smem = G ? (size_t)(kLnWarpThreads / (G ? G : 1)) * 2 * d * 4 : 0;
-            k_ln_bwd<T, decltype(vv)::value, decltype(k)::value, G>
-                <<<(unsigned)p.blocks, p.threads, smem, st>>>((const T*)dy, dy_stride, (const T*)x,
-                                                              x_stride, rows, (int)d, mean, rstd, w,
-                                                              (T*)dx, part);
-          });
-        };
-        if (vec == 1)
-          run(std::integral_constant<int, 1>{});
-        else
-          run(std::integral_constant<int, V>{});
-      }
+      });
     }
     if (sums)
-      k_ln_add<<<(unsigned)((2 * d + 31) / 32), 512, 0, st>>>(part, (int)parts, d, dw, db);
+      k_ln_add<<<(unsigned)((2 * d + 31) / 32), 1024, 0, st>>>(part, (int)parts, d, dw, db);
     return launch_status();
   });
 }

@@ -135,6 +135,49 @@ __device__ __forceinline__ Vec<T, VEC> vec_zero() {
 }
 static inline bool aligned_to(const void* p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
+// Rows staged by bulk copies: one mbarrier per stage, armed with the bytes of
+// its copies.  Waits are bounded; a wait that runs out is reported by the
+// device error word, and the kernel goes on to its end without further waits.
+constexpr uint32_t kStagePolls = 1u << 24;
+__device__ __forceinline__ uint32_t stage_addr(const void* p) {
+  return (uint32_t)__cvta_generic_to_shared(p);
+}
+__device__ __forceinline__ void stage_init(uint64_t* bar) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(stage_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void stage_init_done() {
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+}
+__device__ __forceinline__ void stage_arm(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(stage_addr(bar)),
+               "r"(bytes)
+               : "memory");
+}
+// bytes: a multiple of 16; both addresses on 16 bytes.
+__device__ __forceinline__ void stage_copy(void* dst, const void* src, uint32_t bytes,
+                                           uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          stage_addr(dst)),
+      "l"(src), "r"(bytes), "r"(stage_addr(bar))
+      : "memory");
+}
+__device__ __forceinline__ bool stage_wait(uint64_t* bar, uint32_t parity) {
+  for (uint32_t i = 0; i < kStagePolls; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(stage_addr(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+  }
+  flag_error(QQT_DEV_TIMEOUT);
+  return false;
+}
+
 // 2^x and 1/x by the special-function unit (relative errors of about 2^-22).
 __device__ __forceinline__ float ex2_approx(float x) {
   float r;
