@@ -12,26 +12,86 @@
 //   dz_j = [G (1[j = action] - p_j) + c p_j (log p_j + H_head)] / count
 //   G = (-A r where the clip is not binding) + beta (1 - exp(q))
 // Every sum is float32; the gradient is rounded once to the logits' type.
+//
+// By the number of logits V of a row:
+//  * up to kPlSmall: a thread per row, rows staged in shared memory so that
+//    loads and stores stay contiguous (the policy's 5 + 2 logits);
+//  * else a warp or a block per row: one pass keeps a running maximum and the
+//    two sums, rescaled when the maximum grows; a second pass, whose reads
+//    come from L2, writes the gradient.  Bound by the exponentials (two per
+//    logit on the special-function unit, 16 lanes a cycle and SM) and by
+//    memory at much the same time; the other arithmetic runs in pairs
+//    (f32x2).  A row may begin at any address: vectors are put together from
+//    two aligned ones, so the element a thread works on, and with it every
+//    sum, does not depend on alignment.
 
 #include "ops_common.cuh"
 
 namespace qqt {
 
+#ifndef PL_THREADS
+#define PL_THREADS 512
+#endif
+#ifndef PL_MINB
+#define PL_MINB 2
+#endif
+#ifndef PL_WARP
+#define PL_WARP 2048
+#endif
+constexpr int kPlSmall = 32;         // logits of a row that one thread handles
+constexpr int kPlSmallRows = 256;    // rows of such a block
+constexpr int kPlCounts = 64;        // blocks that count the mask's rows
+constexpr int kPlFold = 8192;        // rows up to which such a block counts them itself
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kFloor = -1.0e4f;    // z - m below it is as good as minus infinity
+
 struct HeadStat {
-  float m, log_s, ent, z_act;
-  bool ok;                  // some category is legal and the action is one of them
+  float m, inv_s, log_s, ent;
+  int act;                  // the action, -1 where it adds nothing
+  float z_act;
 };
 
-__global__ void k_pl_count(const uint8_t* __restrict__ mask, int64_t rows, float* __restrict__ out) {
-  __shared__ float buf[32];
-  int64_t n = 0;
-  if (mask)
-    for (int64_t r = threadIdx.x; r < rows; r += blockDim.x) n += mask[r] != 0;
-  const float c = mask ? block_sum((float)n, buf) : (float)rows;
-  if (threadIdx.x == 0) out[0] = c > 1.f ? c : 1.f;
+// Rows of the mask, at least 1; `counts`: the counting blocks' results.
+__device__ __forceinline__ float rows_counted(const QqtPolicyLoss& a, const int* counts) {
+  if (!a.mask) return fmaxf((float)a.rows, 1.f);
+  const int l = lane_id();
+  const int n = warp_sum(counts[l] + counts[l + 32]);
+  return fmaxf((float)n, 1.f);
 }
 
-// What a row adds to the sums, and its gradient's coefficients.
+__device__ __forceinline__ int count_bytes(const uint8_t* mask, int64_t first, int64_t step,
+                                           int64_t rows) {
+  int n = 0;
+  const bool whole = ((uintptr_t)mask & 15) == 0;
+  for (int64_t r = first * 16; r < rows; r += step * 16) {
+    if (whole && r + 16 <= rows) {
+      const uint4 v = *reinterpret_cast<const uint4*>(mask + r);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)      // bytes that are not 0
+        n += __popc(__vcmpne4(w[k], 0u) & 0x01010101u);
+    } else {
+      for (int64_t q = r; q < r + 16 && q < rows; ++q) n += mask[q] != 0;
+    }
+  }
+  return n;
+}
+
+__global__ void __launch_bounds__(512) k_pl_count(const uint8_t* __restrict__ mask, int64_t rows,
+                                                  int* __restrict__ counts) {
+  __shared__ int buf[16];
+  int n = count_bytes(mask, (int64_t)blockIdx.x * 512 + threadIdx.x, (int64_t)gridDim.x * 512, rows);
+  n = warp_sum(n);
+  if (lane_id() == 0) buf[warp_id()] = n;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    n = 0;
+    for (int k = 0; k < 16; ++k) n += buf[k];
+    counts[blockIdx.x] = n;
+  }
+}
+
+// What a row adds to the sums, and its gradient's coefficient.
 struct RowLoss {
   float pg, kl, clip, g;
 };
@@ -54,98 +114,490 @@ __device__ __forceinline__ RowLoss row_loss(float logp, float old, float a, floa
   return o;
 }
 
+
+__device__ __forceinline__ RowLoss loss_of(const QqtPolicyLoss& a, int64_t r, float logp, bool live) {
+  if (!live) return RowLoss{0.f, 0.f, 0.f, 0.f};
+  return row_loss(logp, a.old_logp[r], a.adv[r], a.ref_logp ? a.ref_logp[r] : 0.f,
+                  a.ref_logp != nullptr, a.clip_low, a.clip_high, a.kl_coef);
+}
+
+// log p of the head's action from its sums, and what the second pass needs.
+__device__ __forceinline__ float finish_head(HeadStat& k, float m, float s, float e, float z_act,
+                                             bool act_ok) {
+  const bool any = m != -INFINITY;
+  k.m = m;
+  k.inv_s = any ? 1.f / s : 0.f;
+  k.log_s = logf(s);
+  k.ent = any ? k.log_s - e * k.inv_s : 0.f;
+  k.z_act = z_act;
+  return any && act_ok && z_act != -INFINITY ? z_act - m - k.log_s : -INFINITY;
+}
+
+// The gradient at a logit t = z - m that is not the action's: with p = e / S,
+// scale (p (c (log p + H) - G)); the terms that may cancel are added before
+// the scale.  At the action's: scale (G (1 - p) + c p (log p + H)).
+struct HeadGrad {
+  float c_s, k_s, scale;               // e (c_s t + k_s) scale
+};
+__device__ __forceinline__ HeadGrad head_grad(const HeadStat& k, float g, float c, float scale) {
+  return HeadGrad{c * k.inv_s, (c * (k.ent - k.log_s) - g) * k.inv_s, scale};
+}
+__device__ __forceinline__ float action_grad(const HeadStat& k, float g, float c, float scale) {
+  const float lp = k.z_act - k.m - k.log_s, p = expf(lp);
+  return scale * fmaf(g, 1.f - p, p * (c * (lp + k.ent)));
+}
+
+// ---------------------------------------------------- few logits: thread per row
+
 template <class T>
-__global__ void k_pl_rows(QqtPolicyLoss a, const float* __restrict__ count, float* __restrict__ part) {
+__global__ void __launch_bounds__(kPlSmallRows)
+    k_pl_small(QqtPolicyLoss a, int V, const int* __restrict__ counts, float* __restrict__ part,
+               int one_block) {
+  extern __shared__ float zs[];          // [rows][pitch]
   __shared__ float buf[32];
-  const int64_t r = blockIdx.x;
-  const T* z = (const T*)a.logits + r * a.row_stride;
-  const uint8_t* legal = a.legal ? a.legal + r * a.legal_stride : nullptr;
+  __shared__ int n_mask;
+  const int pitch = V | 1;               // odd: threads on rows hit different banks
+  const int64_t r0 = (int64_t)blockIdx.x * kPlSmallRows;
+  const int n = a.rows - r0 < kPlSmallRows ? (int)(a.rows - r0) : kPlSmallRows;
+  const bool loss = a.old_logp != nullptr;
+  const bool fold = loss && a.mask && !counts;
+  int mine = 0;
+  if (fold) {
+    if (threadIdx.x == 0) n_mask = 0;
+    mine = warp_sum(count_bytes(a.mask, threadIdx.x, kPlSmallRows, a.rows));
+  }
+  {
+    int row = threadIdx.x / V, col = threadIdx.x % V;
+    const int dr = kPlSmallRows / V, dc = kPlSmallRows % V;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n * V; i += kPlSmallRows) {
+      float z = to_f(((const T*)a.logits)[(r0 + row) * a.row_stride + col]);
+      if (a.legal && !a.legal[(r0 + row) * a.legal_stride + col]) z = -INFINITY;
+      zs[row * pitch + col] = z;
+      row += dr;
+      col += dc;
+      if (col >= V) {
+        col -= V;
+        ++row;
+      }
+    }
+  }
+  __syncthreads();
+  if (fold && lane_id() == 0 && mine) atomicAdd(&n_mask, mine);   // whole numbers: any order
+  const bool on = threadIdx.x < n;
+  const int64_t r = r0 + threadIdx.x;
+  float* z = zs + threadIdx.x * pitch;
   HeadStat hs[QQT_MAX_HEADS];
   float logp = 0.f, ent = 0.f;
-  bool ok = true;
-  int at = 0;
-  for (int h = 0; h < a.n_heads; ++h) {
-    const int w = a.width[h];
-    const int64_t act = a.actions[r * a.action_stride + h];
-    float m = -INFINITY;
-    for (int j = threadIdx.x; j < w; j += blockDim.x)
-      if (!legal || legal[at + j]) m = max_nan(m, to_f(z[at + j]));
-    m = block_max_nan(m, buf);
-    float s = 0.f, e = 0.f;
-    for (int j = threadIdx.x; j < w; j += blockDim.x) {
-      if (legal && !legal[at + j]) continue;
-      const float t = to_f(z[at + j]) - m;
-      if (t == -INFINITY) continue;
-      const float x = expf(t);
-      s += x;
-      e = fmaf(x, t, e);
+  if (on) {
+    int at = 0;
+#pragma unroll 1
+    for (int h = 0; h < a.n_heads; ++h) {
+      const int w = a.width[h];
+      const int64_t act = a.actions[r * a.action_stride + h];
+      const bool in = act >= 0 && act < w;
+      if (!in) flag_error(QQT_DEV_BAD_ACTION);
+      float m = -INFINITY, s = 0.f, e = 0.f;
+      for (int j = 0; j < w; ++j) m = max_nan(m, z[at + j]);
+      for (int j = 0; j < w; ++j) {
+        const float t = max_nan(z[at + j] - m, kFloor), x = expf(t);
+        s += x;
+        e = fmaf(x, t, e);
+      }
+      HeadStat k;
+      k.act = in ? at + (int)act : -1;
+      logp += finish_head(k, m, s, e, in ? z[at + act] : -INFINITY, in);
+      ent += k.ent;
+      hs[h] = k;
+      at += w;
     }
-    s = block_sum(s, buf);
-    e = block_sum(e, buf);
-    HeadStat k;
+    if (a.logp) a.logp[r] = logp;
+    if (a.entropy) a.entropy[r] = ent;
+  }
+  if (!loss) return;
+  if (fold) __syncthreads();
+  const float count = fold ? fmaxf((float)n_mask, 1.f) : rows_counted(a, counts);
+  const bool live = on && logp != -INFINITY && (!a.mask || a.mask[r]);
+  const RowLoss l = loss_of(a, r, logp, live);
+  if (a.stats) {
+    const float v[4] = {l.pg, l.kl, live ? ent : 0.f, l.clip};
+    float sum[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sum[k] = block_sum(v[k], buf);
+    if (threadIdx.x == 0) {
+      if (one_block) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] /= count;
+        a.stats[0] = sum[0] + a.kl_coef * sum[1] - a.entropy_coef * sum[2];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) a.stats[1 + k] = sum[k];
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) part[blockIdx.x * 4 + k] = sum[k];
+      }
+    }
+  }
+  if (!a.dlogits) return;
+  const float scale = a.grad_scale / count * (a.upstream ? a.upstream[0] : 1.f);
+  if (on) {
+    int at = 0;
+#pragma unroll 1
+    for (int h = 0; h < a.n_heads; ++h) {
+      const int w = a.width[h];
+      const HeadStat k = hs[h];
+      const HeadGrad q = head_grad(k, l.g, a.entropy_coef, scale);
+      for (int j = 0; j < w; ++j) {
+        const float t = max_nan(z[at + j] - k.m, kFloor);
+        z[at + j] = live ? expf(t) * fmaf(q.c_s, t, q.k_s) * scale : 0.f;
+      }
+      if (live) z[k.act] = action_grad(k, l.g, a.entropy_coef, scale);
+      at += w;
+    }
+  }
+  __syncthreads();
+  {
+    int row = threadIdx.x / V, col = threadIdx.x % V;
+    const int dr = kPlSmallRows / V, dc = kPlSmallRows % V;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n * V; i += kPlSmallRows) {
+      ((T*)a.dlogits)[(r0 + row) * a.dlogits_stride + col] = from_f<T>(zs[row * pitch + col]);
+      row += dr;
+      col += dc;
+      if (col >= V) {
+        col -= V;
+        ++row;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------- many logits: team per row
+
+// Pairs of floats in one instruction each.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// The VEC elements from the s-th (0 < s < VEC) of the 2 VEC of a and b.
+template <class T, int VEC>
+__device__ __forceinline__ uint4 funnel(uint4 a, uint4 b, int s) {
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  const int words = sizeof(T) == 4 ? s : s >> 1;
+  if (words & 2) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  }
+  if (words & 1) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  }
+  if (sizeof(T) == 2) {
+    const int bits = (s & 1) * 16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], bits);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Vector j of the w elements from p, minus infinity past them.  sh: elements
+// between p and the 16-byte boundary below it.  Reads no element outside.
+template <class T, int VEC>
+__device__ __forceinline__ Vec<T, VEC> get_logits(const T* p, int sh, int j, int w) {
+  const int i = j * VEC;
+  uint4 r;
+  if (sh == 0 && i + VEC <= w) {
+    r = *reinterpret_cast<const uint4*>(p + i);
+  } else if (sh && i >= sh && i - sh + 2 * VEC <= w) {
+    const uint4* q = reinterpret_cast<const uint4*>(p + i - sh);
+    r = funnel<T, VEC>(q[0], q[1], sh);
+  } else {
+    float f[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) f[v] = i + v < w ? to_f(p[i + v]) : -INFINITY;
+    Vec<T, VEC> x;
+    x.put(f);
+    return x;
+  }
+  return *reinterpret_cast<const Vec<T, VEC>*>(&r);
+}
+
+// Stores vector j of the w elements from p; every lane of the warp calls it,
+// lane l with vector j0 + l.  on: the vector exists.  Where p is not on a
+// 16-byte boundary each lane stores the aligned word that its vector's first
+// elements and the lane below's last ones make up.
+template <class T, int VEC>
+__device__ __forceinline__ void put_grads(T* p, int sh, int j, int w, bool on, const float* f) {
+  Vec<T, VEC> x;
+  x.put(f);
+  const int i = j * VEC;
+  if (sh == 0) {
+    if (on && i + VEC <= w) {
+      st_vec(p + i, x);
+    } else if (on) {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v)
+        if (i + v < w) p[i + v] = from_f<T>(f[v]);
+    }
+    return;
+  }
+  const uint4 own = *reinterpret_cast<const uint4*>(&x);
+  uint4 below;
+  below.x = __shfl_up_sync(QQT_FULL, own.x, 1);
+  below.y = __shfl_up_sync(QQT_FULL, own.y, 1);
+  below.z = __shfl_up_sync(QQT_FULL, own.z, 1);
+  below.w = __shfl_up_sync(QQT_FULL, own.w, 1);
+  const bool above = __shfl_down_sync(QQT_FULL, (int)on, 1) && lane_id() < 31;
+  if (!on) return;
+  const int first = VEC - sh;            // elements of this vector in the word it shares below
+  const bool joined = lane_id() > 0 && i + first <= w;
+  if (joined)
+    *reinterpret_cast<uint4*>(p + i - sh) = funnel<T, VEC>(below, own, first);
+  // what no joined word takes: the last elements under a gap, the first without one below
+#pragma unroll
+  for (int v = 0; v < VEC; ++v)
+    if (i + v < w && ((v < first && !joined) || (v >= first && !above)))
+      p[i + v] = from_f<T>(f[v]);
+  // (a vector above that ends early does not join: its lane hands this one's last elements back)
+  if (lane_id() > 0 && !joined) {
+    const Vec<T, VEC> b = *reinterpret_cast<const Vec<T, VEC>*>(&below);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v)
+      if (v >= first) p[i - VEC + v] = from_f<T>(b.get(v));
+  }
+}
+
+template <class T>
+__device__ __forceinline__ int misfit(const T* p) {
+  return (int)(((uintptr_t)p & 15) / sizeof(T));
+}
+
+template <int VEC>
+__device__ __forceinline__ void bar_illegal(const uint8_t* legal, int j, int w, float* f) {
+  const int i = j * VEC;
+  const uint8_t* l = legal + i;
+  if (i + VEC <= w && ((uintptr_t)l & (VEC - 1)) == 0) {
+    uint32_t b[VEC / 4];
+    if constexpr (VEC == 8) {
+      const uint2 v = *reinterpret_cast<const uint2*>(l);
+      b[0] = v.x;
+      b[1] = v.y;
+    } else {
+      b[0] = *reinterpret_cast<const uint32_t*>(l);
+    }
+#pragma unroll
+    for (int v = 0; v < VEC; ++v)
+      if (!((b[v / 4] >> (v % 4 * 8)) & 0xff)) f[v] = -INFINITY;
+  } else {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v)
+      if (i + v < w && !l[v]) f[v] = -INFINITY;
+  }
+}
+
+// Maximum and sums over a team of a warp (WARP) or a block.
+template <bool WARP>
+__device__ __forceinline__ float team_max(float v, float* buf) {
+  return WARP ? warp_max_nan(v) : block_max_nan(v, buf);
+}
+template <bool WARP>
+__device__ __forceinline__ float team_add(float v, float* buf) {
+  return WARP ? warp_sum_f(v) : block_sum(v, buf);
+}
+
+template <class T, bool WARP, bool LEGAL>
+__global__ void __launch_bounds__(PL_THREADS, PL_MINB)
+    k_pl_rows(QqtPolicyLoss a, const int* __restrict__ counts, float* __restrict__ part) {
+  constexpr int VEC = 16 / sizeof(T), U = 4;
+  __shared__ float buf[32];
+  const int j0 = WARP ? 0 : (int)threadIdx.x - lane_id();   // the warp's first vector
+  const int step = WARP ? 32 : (int)blockDim.x;
+  const int64_t r = WARP ? (int64_t)blockIdx.x * (blockDim.x / 32) + warp_id() : (int64_t)blockIdx.x;
+  if (WARP && r >= a.rows) return;
+  const int lead = WARP ? lane_id() : (int)threadIdx.x;
+  const T* z = (const T*)a.logits + r * a.row_stride;
+  const uint8_t* legal = LEGAL ? a.legal + r * a.legal_stride : nullptr;
+  HeadStat hs[QQT_MAX_HEADS];
+  float logp = 0.f, ent = 0.f;
+  int at = 0;
+#pragma unroll 1
+  for (int h = 0; h < a.n_heads; ++h) {
+    const int w = a.width[h], nv = (w + VEC - 1) / VEC;
+    const T* p = z + at;
+    const int sh = misfit(p);
+    float m = -INFINITY;
+    uint64_t s2 = pair(0.f, 0.f), e2 = s2;
+#pragma unroll 1
+    for (int jb = j0; jb < nv; jb += step * U) {
+      float f[U][VEC];
+      {
+        Vec<T, VEC> c[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          c[u] = get_logits<T, VEC>(p, sh, jb + lane_id() + u * step, w);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) f[u][v] = c[u].get(v);
+      }
+      if (LEGAL)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (jb + lane_id() + u * step < nv) bar_illegal<VEC>(legal + at, jb + lane_id() + u * step, w, f[u]);
+      float mx = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) mx = max_nan(mx, f[u][v]);
+      if (mx == -INFINITY) continue;       // nothing legal so far
+      if (mx != m) {                       // rescale: e^(z - m) (z - m) moves with m too
+        const float dm = max_nan(m - mx, kFloor), sc = ex2_approx(dm * kLog2e);
+        const uint64_t sc2 = pair(sc, sc);
+        e2 = mul2(fma2(pair(dm, dm), s2, e2), sc2);
+        s2 = mul2(s2, sc2);
+        m = mx;
+      }
+      const uint64_t nm = pair(-m, -m), l2 = pair(kLog2e, kLog2e);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int v = 0; v < VEC; v += 2) {
+          float t0, t1, x0, x1;
+          unpair(add2(pair(f[u][v], f[u][v + 1]), nm), t0, t1);
+          const uint64_t t = pair(max_nan(t0, kFloor), max_nan(t1, kFloor));
+          unpair(mul2(t, l2), x0, x1);
+          const uint64_t x = pair(ex2_approx(x0), ex2_approx(x1));
+          s2 = add2(s2, x);
+          e2 = fma2(x, t, e2);
+        }
+    }
+    float s, e, hi;
+    unpair(s2, s, hi);
+    s += hi;
+    unpair(e2, e, hi);
+    e += hi;
+    const float top = team_max<WARP>(m, buf);
+    const float dm = m == -INFINITY ? kFloor : max_nan(m - top, kFloor);
+    const float sc = m == -INFINITY ? 0.f : ex2_approx(dm * kLog2e);
+    e = team_add<WARP>(sc * fmaf(dm, s, e), buf);
+    s = team_add<WARP>(sc * s, buf);
+    const int64_t act = a.actions[r * a.action_stride + h];
     const bool in = act >= 0 && act < w;
-    if (!in && threadIdx.x == 0) flag_error(QQT_DEV_BAD_ACTION);
-    k.z_act = in && (!legal || legal[at + act]) ? to_f(z[at + act]) : -INFINITY;
-    k.ok = m != -INFINITY && k.z_act != -INFINITY;
-    k.m = m;
-    k.log_s = logf(s);
-    k.ent = m == -INFINITY ? 0.f : k.log_s - e / s;
-    logp += k.ok ? k.z_act - m - k.log_s : -INFINITY;
+    if (!in && lead == 0) flag_error(QQT_DEV_BAD_ACTION);
+    HeadStat k;
+    k.act = in ? (int)act : -1;
+    logp += finish_head(k, top, s, e, in && !(LEGAL && !legal[at + act]) ? to_f(p[act]) : -INFINITY,
+                        in);
     ent += k.ent;
-    ok = ok && k.ok;
     hs[h] = k;
     at += w;
   }
-  if (threadIdx.x == 0) {
+  if (lead == 0) {
     if (a.logp) a.logp[r] = logp;
     if (a.entropy) a.entropy[r] = ent;
   }
   if (!a.old_logp) return;
-  const bool live = ok && (!a.mask || a.mask[r]);
-  RowLoss l{0.f, 0.f, 0.f, 0.f};
-  if (live)
-    l = row_loss(logp, a.old_logp[r], a.adv[r], a.ref_logp ? a.ref_logp[r] : 0.f,
-                 a.ref_logp != nullptr, a.clip_low, a.clip_high, a.kl_coef);
-  if (a.stats && threadIdx.x == 0) {
-    part[r * 4 + 0] = l.pg;
-    part[r * 4 + 1] = l.kl;
-    part[r * 4 + 2] = live ? ent : 0.f;
-    part[r * 4 + 3] = l.clip;
-  }
+  const bool live = logp != -INFINITY && (!a.mask || a.mask[r]);
+  const RowLoss l = loss_of(a, r, logp, live);
+  if (a.stats && lead == 0)
+    *reinterpret_cast<float4*>(part + r * 4) =
+        make_float4(l.pg, l.kl, live ? ent : 0.f, l.clip);
   if (!a.dlogits) return;
-  const float scale = a.grad_scale / count[0] * (a.upstream ? a.upstream[0] : 1.f);
+  const float scale =
+      a.grad_scale / rows_counted(a, counts) * (a.upstream ? a.upstream[0] : 1.f);
   T* dz = (T*)a.dlogits + r * a.dlogits_stride;
   at = 0;
+#pragma unroll 1
   for (int h = 0; h < a.n_heads; ++h) {
-    const int w = a.width[h];
+    const int w = a.width[h], nv = (w + VEC - 1) / VEC;
     const HeadStat k = hs[h];
-    const int64_t act = a.actions[r * a.action_stride + h];
-    for (int j = threadIdx.x; j < w; j += blockDim.x) {
-      float v = 0.f;
-      if (live && (!legal || legal[at + j])) {
-        // the terms that may cancel are added unscaled, the scale comes last
-        const float lp = to_f(z[at + j]) - k.m - k.log_s;
-        const float p = expf(lp);
-        const float q = lp == -INFINITY ? 0.f : a.entropy_coef * (lp + k.ent);
-        v = scale * (j == act ? fmaf(l.g, 1.f - p, p * q) : p * (q - l.g));
+    const T* p = z + at;
+    T* q = dz + at;
+    const int sh = misfit(p), qsh = misfit(q);
+    const HeadGrad g = head_grad(k, l.g, a.entropy_coef, scale);
+    const float ga = live ? action_grad(k, l.g, a.entropy_coef, scale) : 0.f;
+    const uint64_t nm = pair(-k.m, -k.m), l2 = pair(kLog2e, kLog2e), cs = pair(g.c_s, g.c_s),
+                   ks = pair(g.k_s, g.k_s), sc = pair(g.scale, g.scale);
+#pragma unroll 1
+    for (int jb = j0; jb < nv; jb += step * 2) {
+      Vec<T, VEC> c[2];
+      if (live)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          c[u] = get_logits<T, VEC>(p, sh, jb + lane_id() + u * step, w);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int j = jb + lane_id() + u * step;
+        float f[VEC];
+        if (live) {
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) f[v] = c[u].get(v);
+          if (LEGAL && j < nv) bar_illegal<VEC>(legal + at, j, w, f);
+#pragma unroll
+          for (int v = 0; v < VEC; v += 2) {
+            float t0, t1, x0, x1;
+            unpair(add2(pair(f[v], f[v + 1]), nm), t0, t1);
+            const uint64_t t = pair(max_nan(t0, kFloor), max_nan(t1, kFloor));
+            unpair(mul2(t, l2), x0, x1);
+            const uint64_t x = pair(ex2_approx(x0), ex2_approx(x1));
+            unpair(mul2(mul2(x, fma2(cs, t, ks)), sc), f[v], f[v + 1]);
+          }
+          if (j == k.act / VEC) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v)
+              if (j * VEC + v == k.act) f[v] = ga;
+          }
+        } else {
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) f[v] = 0.f;
+        }
+        put_grads<T, VEC>(q, qsh, j, w, j < nv, f);
       }
-      dz[at + j] = from_f<T>(v);
     }
     at += w;
   }
 }
 
-__global__ void k_pl_stats(const float* __restrict__ part, int64_t n, const float* __restrict__ count,
-                           float beta, float c, float* __restrict__ stats) {
+// Means over the counted rows from n partial sums, in a fixed order.
+__global__ void __launch_bounds__(1024)
+    k_pl_stats(QqtPolicyLoss a, const float* __restrict__ part, int64_t n,
+               const int* __restrict__ counts) {
   __shared__ float buf[32];
-  double s[4] = {0., 0., 0., 0.};
-  for (int64_t r = threadIdx.x; r < n; r += blockDim.x)
-    for (int k = 0; k < 4; ++k) s[k] += part[r * 4 + k];
-  float v[4];
-  for (int k = 0; k < 4; ++k) v[k] = block_sum((float)s[k], buf) / count[0];
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int64_t r = threadIdx.x; r < n; r += 1024) {
+    const float4 v = *reinterpret_cast<const float4*>(part + r * 4);
+    s[0] += v.x;
+    s[1] += v.y;
+    s[2] += v.z;
+    s[3] += v.w;
+  }
+  const float count = rows_counted(a, counts);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) s[k] = block_sum(s[k], buf) / count;
   if (threadIdx.x == 0) {
-    stats[0] = v[0] + beta * v[1] - c * v[2];
-    for (int k = 0; k < 4; ++k) stats[1 + k] = v[k];
+    a.stats[0] = s[0] + a.kl_coef * s[1] - a.entropy_coef * s[2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) a.stats[1 + k] = s[k];
   }
 }
 
@@ -153,8 +605,9 @@ __global__ void k_pl_stats(const float* __restrict__ part, int64_t n, const floa
 
 using namespace qqt;
 
+// 64 counts, then four partial sums a row (or a block of rows).
 extern "C" uint64_t qqt_policy_loss_work_bytes(int64_t rows) {
-  return rows < 0 ? 0 : 16 + (uint64_t)rows * 16;
+  return rows < 0 ? 0 : kPlCounts * 4 + (uint64_t)rows * 16;
 }
 
 extern "C" int qqt_policy_loss(const QqtPolicyLoss* a, qqt_stream_t stream) {
@@ -165,23 +618,48 @@ extern "C" int qqt_policy_loss(const QqtPolicyLoss* a, qqt_stream_t stream) {
     if (a->width[h] < 1) return QQT_E_ARG;
     v += a->width[h];
   }
-  if (v > 0x7fffffffll) return QQT_E_LIMIT;
+  if (v > 0x3fffffffll) return QQT_E_LIMIT;
   const bool loss = a->stats || a->dlogits;
   if (loss && !a->work) return QQT_E_ARG;
   if (a->rows > 0 && (!a->logits || !a->actions || (loss && (!a->old_logp || !a->adv))))
     return QQT_E_ARG;
+  if (!aligned_to(a->work, 16)) return QQT_E_ALIGN;
   cudaStream_t st = (cudaStream_t)stream;
-  float* count = (float*)a->work;
-  float* part = count + 4;
   QqtPolicyLoss args = *a;
   if (!loss) args.old_logp = nullptr;
-  if (loss) k_pl_count<<<1, 1024, 0, st>>>(a->mask, a->rows, count);
+  const bool small = v <= kPlSmall;
+  const int64_t blocks = (a->rows + kPlSmallRows - 1) / kPlSmallRows;
+  const bool one = small && blocks == 1;
+  int* counts = (int*)a->work;
+  float* part = loss ? (float*)(counts + kPlCounts) : nullptr;
+  if (loss && a->mask && !(small && a->rows <= kPlFold && blocks > 0 && (one || !a->stats)))
+    k_pl_count<<<kPlCounts, 512, 0, st>>>(a->mask, a->rows, counts);
+  else
+    counts = nullptr;
   if (a->rows > 0)
     with_dtype(a->dtype, [&](auto t) {
-      k_pl_rows<decltype(t)><<<(unsigned)a->rows, 256, 0, st>>>(args, count, part);
+      using T = decltype(t);
+      if (small) {
+        const size_t smem = (size_t)kPlSmallRows * (v | 1) * 4;
+        k_pl_small<T><<<(unsigned)blocks, kPlSmallRows, smem, st>>>(args, (int)v, counts, part, one);
+        return 0;
+      }
+      auto rows = [&](auto warp, auto legal) {
+        constexpr bool WARP = decltype(warp)::value;
+        const int threads = WARP ? 256 : v * (int64_t)sizeof(T) > 65536 * 2 ? PL_THREADS : 256;
+        const unsigned n = (unsigned)(WARP ? (a->rows + 7) / 8 : a->rows);
+        k_pl_rows<T, WARP, decltype(legal)::value><<<n, threads, 0, st>>>(args, counts, part);
+      };
+      using std::false_type;
+      using std::true_type;
+      const bool warp = v <= PL_WARP;
+      if (warp && a->legal) rows(true_type{}, true_type{});
+      if (warp && !a->legal) rows(true_type{}, false_type{});
+      if (!warp && a->legal) rows(false_type{}, true_type{});
+      if (!warp && !a->legal) rows(false_type{}, false_type{});
       return 0;
     });
-  if (a->stats)
-    k_pl_stats<<<1, 1024, 0, st>>>(part, a->rows, count, a->kl_coef, a->entropy_coef, a->stats);
+  if (a->stats && !one)
+    k_pl_stats<<<1, 1024, 0, st>>>(args, part, small ? blocks : a->rows, counts);
   return launch_status();
 }
