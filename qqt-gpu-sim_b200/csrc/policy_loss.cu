@@ -29,15 +29,10 @@
 
 namespace qqt {
 
-#ifndef PL_THREADS
-#define PL_THREADS 512
+#ifndef PL_W
+#define PL_W 256
 #endif
-#ifndef PL_MINB
-#define PL_MINB 2
-#endif
-#ifndef PL_WARP
-#define PL_WARP 2048
-#endif
+constexpr int kPlThreads = 512;      // largest block on a row
 constexpr int kPlSmall = 32;         // logits of a row that one thread handles
 constexpr int kPlSmallRows = 256;    // rows of such a block
 constexpr int kPlCounts = 64;        // blocks that count the mask's rows
@@ -340,12 +335,172 @@ __device__ __forceinline__ Vec<T, VEC> get_logits(const T* p, int sh, int j, int
   }
   return *reinterpret_cast<const Vec<T, VEC>*>(&r);
 }
+// Vectors j, j + step, ...  inner: none of the warp's is at an end of the row.
+template <class T, int VEC, int U>
+__device__ __forceinline__ void get_chunk(const T* p, int sh, int j, int step, int w, bool inner,
+                                          Vec<T, VEC>* c) {
+  if (inner && sh == 0) {
+    const uint4* q = reinterpret_cast<const uint4*>(p) + j;
+#pragma unroll
+    for (int u = 0; u < U; ++u, q += step) {
+      const uint4 r = *q;
+      c[u] = *reinterpret_cast<const Vec<T, VEC>*>(&r);
+    }
+  } else if (inner) {
+    const uint4* q = reinterpret_cast<const uint4*>(p - sh) + j;
+    uint4 lo[U], hi[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u, q += step) {
+      lo[u] = q[0];
+      hi[u] = q[1];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint4 r = funnel<T, VEC>(lo[u], hi[u], sh);
+      c[u] = *reinterpret_cast<const Vec<T, VEC>*>(&r);
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u) c[u] = get_logits<T, VEC>(p, sh, j + u * step, w);
+  }
+}
+
+// What is done to a vector before it is taken apart into floats: minus
+// infinity in illegal places, the maximum, and a finite floor (so that a
+// weight of 0 times z - m is 0).
+template <class T, int VEC>
+struct Logits;
+template <int VEC>
+struct Logits<float, VEC> {
+  static constexpr bool kSafe = false;   // z - m may be minus infinity
+  static constexpr float kBound = 0.f;
+  __device__ static __forceinline__ void bar(Vec<float, VEC>& x, const uint32_t* legal4) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v)
+      if (!((legal4[v / 4] >> (v % 4 * 8)) & 0xff)) x.v[v] = -INFINITY;
+  }
+  __device__ static __forceinline__ float top(float m, const Vec<float, VEC>& x) {
+#pragma unroll
+    for (int v = 0; v < VEC; v += 2)
+      asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(m), "f"(x.v[v]), "f"(x.v[v + 1]));
+    return m;
+  }
+  __device__ static __forceinline__ void lift(Vec<float, VEC>&) {}
+};
+template <class T>
+struct Half2;
+template <>
+struct Half2<__half> {
+  static constexpr uint32_t kNegInf = 0xfc00fc00u, kLowest = 0xfbfffbffu;
+  static constexpr float kBound = 3.0e4f;
+  __device__ static __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+};
+template <>
+struct Half2<__nv_bfloat16> {
+  static constexpr uint32_t kNegInf = 0xff80ff80u, kLowest = 0xff7fff7fu;
+  static constexpr float kBound = 1.0e30f;
+  __device__ static __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+};
+template <class T, int VEC>
+struct Logits16 {
+  // after lift() z - m is finite, and what was minus infinity still adds 0,
+  // while |m| is below kBound
+  static constexpr bool kSafe = true;
+  static constexpr float kBound = Half2<T>::kBound;
+  __device__ static __forceinline__ void bar(Vec<T, VEC>& x, const uint32_t* legal4) {
+#pragma unroll
+    for (int k = 0; k < VEC / 4; ++k) {
+      const uint32_t on = __vcmpne4(legal4[k], 0u);      // a byte of ones per legal place
+      const uint32_t lo = __byte_perm(on, 0, 0x1100), hi = __byte_perm(on, 0, 0x3322);
+      x.w[2 * k] = (x.w[2 * k] & lo) | (Half2<T>::kNegInf & ~lo);
+      x.w[2 * k + 1] = (x.w[2 * k + 1] & hi) | (Half2<T>::kNegInf & ~hi);
+    }
+  }
+  __device__ static __forceinline__ float top(float m, const Vec<T, VEC>& x) {
+    uint32_t t = x.w[0];
+#pragma unroll
+    for (int k = 1; k < VEC / 2; ++k) t = Half2<T>::max(t, x.w[k]);
+    Vec<T, 2> two;
+    two.w[0] = t;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(m), "f"(two.get(0)), "f"(two.get(1)));
+    return m;
+  }
+  __device__ static __forceinline__ void lift(Vec<T, VEC>& x) {
+#pragma unroll
+    for (int k = 0; k < VEC / 2; ++k) x.w[k] = Half2<T>::max(x.w[k], Half2<T>::kLowest);
+  }
+};
+template <int VEC>
+struct Logits<__half, VEC> : Logits16<__half, VEC> {};
+template <int VEC>
+struct Logits<__nv_bfloat16, VEC> : Logits16<__nv_bfloat16, VEC> {};
+
+template <class T, int VEC>
+__device__ __forceinline__ void bar_illegal(Vec<T, VEC>& x, const uint8_t* legal, int j, int w) {
+  const int i = j * VEC;
+  const uint8_t* l = legal + i;
+  uint32_t b[VEC / 4];
+  if (i + VEC <= w && ((uintptr_t)l & (VEC - 1)) == 0) {
+    if constexpr (VEC == 8) {
+      const uint2 v = *reinterpret_cast<const uint2*>(l);
+      b[0] = v.x;
+      b[1] = v.y;
+    } else {
+      b[0] = *reinterpret_cast<const uint32_t*>(l);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC / 4; ++k) {
+      b[k] = 0;
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        if (i + 4 * k + v < w && l[4 * k + v]) b[k] |= 0xffu << (8 * v);
+    }
+  }
+  Logits<T, VEC>::bar(x, b);
+}
+
+// z - m of a pair of places, as floats of at least kFloor where SAFE is not given.
+template <bool SAFE>
+__device__ __forceinline__ uint64_t below_top(float z0, float z1, uint64_t nm) {
+  const uint64_t t = add2(pair(z0, z1), nm);
+  if (SAFE) return t;
+  float t0, t1;
+  unpair(t, t0, t1);
+  return pair(max_nan(t0, kFloor), max_nan(t1, kFloor));
+}
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t t) {
+  float x0, x1;
+  unpair(mul2(t, pair(kLog2e, kLog2e)), x0, x1);
+  return pair(ex2_approx(x0), ex2_approx(x1));
+}
+template <class T, int VEC, int U, bool SAFE>
+__device__ __forceinline__ void add_exps(const Vec<T, VEC>* c, float m, uint64_t& s2, uint64_t& e2) {
+  const uint64_t nm = pair(-m, -m);
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int v = 0; v < VEC; v += 2) {
+      const uint64_t t = below_top<SAFE>(c[u].get(v), c[u].get(v + 1), nm);
+      const uint64_t x = exp2_pair(t);
+      s2 = add2(s2, x);
+      e2 = fma2(x, t, e2);
+    }
+}
 
 // Stores vector j of the w elements from p; every lane of the warp calls it,
-// lane l with vector j0 + l.  on: the vector exists.  Where p is not on a
-// 16-byte boundary each lane stores the aligned word that its vector's first
-// elements and the lane below's last ones make up.
-template <class T, int VEC>
+// and lane l of a team of G has vector j0 + l.  on: the vector exists.  Where p
+// is not on a 16-byte boundary each lane stores the aligned word that its
+// vector's first elements and the lane below's last ones make up.
+template <class T, int VEC, int G>
 __device__ __forceinline__ void put_grads(T* p, int sh, int j, int w, bool on, const float* f) {
   Vec<T, VEC> x;
   x.put(f);
@@ -358,28 +513,31 @@ __device__ __forceinline__ void put_grads(T* p, int sh, int j, int w, bool on, c
       for (int v = 0; v < VEC; ++v)
         if (i + v < w) p[i + v] = from_f<T>(f[v]);
     }
-    return;
   }
+  // (teams of a warp are on rows of their own alignment)
+  if (G == 32 ? sh == 0 : __all_sync(QQT_FULL, sh == 0)) return;
+  const int l = lane_id() % G;
   const uint4 own = *reinterpret_cast<const uint4*>(&x);
-  uint4 below;
-  below.x = __shfl_up_sync(QQT_FULL, own.x, 1);
-  below.y = __shfl_up_sync(QQT_FULL, own.y, 1);
-  below.z = __shfl_up_sync(QQT_FULL, own.z, 1);
-  below.w = __shfl_up_sync(QQT_FULL, own.w, 1);
-  const bool above = __shfl_down_sync(QQT_FULL, (int)on, 1) && lane_id() < 31;
-  if (!on) return;
-  const int first = VEC - sh;            // elements of this vector in the word it shares below
-  const bool joined = lane_id() > 0 && i + first <= w;
-  if (joined)
-    *reinterpret_cast<uint4*>(p + i - sh) = funnel<T, VEC>(below, own, first);
-  // what no joined word takes: the last elements under a gap, the first without one below
+  uint4 under;
+  under.x = __shfl_up_sync(QQT_FULL, own.x, 1);
+  under.y = __shfl_up_sync(QQT_FULL, own.y, 1);
+  under.z = __shfl_up_sync(QQT_FULL, own.z, 1);
+  under.w = __shfl_up_sync(QQT_FULL, own.w, 1);
+  const bool over = __shfl_down_sync(QQT_FULL, (int)on, 1) && l < G - 1;
+  if (!on || sh == 0) return;
+  const int first = VEC - sh;            // elements of this vector in the word it shares
+  const bool joined = l > 0 && i + first <= w;
+  if (joined) *reinterpret_cast<uint4*>(p + i - sh) = funnel<T, VEC>(under, own, first);
+  if (joined && over) return;
+  // what no joined word takes: first elements without a lane below, last ones
+  // without a lane above ...
 #pragma unroll
   for (int v = 0; v < VEC; ++v)
-    if (i + v < w && ((v < first && !joined) || (v >= first && !above)))
+    if (i + v < w && ((v < first && !joined) || (v >= first && !over)))
       p[i + v] = from_f<T>(f[v]);
-  // (a vector above that ends early does not join: its lane hands this one's last elements back)
-  if (lane_id() > 0 && !joined) {
-    const Vec<T, VEC> b = *reinterpret_cast<const Vec<T, VEC>*>(&below);
+  // ... and the last ones of the lane below a vector that ends before it can join
+  if (l > 0 && !joined) {
+    const Vec<T, VEC> b = *reinterpret_cast<const Vec<T, VEC>*>(&under);
 #pragma unroll
     for (int v = 0; v < VEC; ++v)
       if (v >= first) p[i - VEC + v] = from_f<T>(b.get(v));
@@ -391,49 +549,36 @@ __device__ __forceinline__ int misfit(const T* p) {
   return (int)(((uintptr_t)p & 15) / sizeof(T));
 }
 
-template <int VEC>
-__device__ __forceinline__ void bar_illegal(const uint8_t* legal, int j, int w, float* f) {
-  const int i = j * VEC;
-  const uint8_t* l = legal + i;
-  if (i + VEC <= w && ((uintptr_t)l & (VEC - 1)) == 0) {
-    uint32_t b[VEC / 4];
-    if constexpr (VEC == 8) {
-      const uint2 v = *reinterpret_cast<const uint2*>(l);
-      b[0] = v.x;
-      b[1] = v.y;
-    } else {
-      b[0] = *reinterpret_cast<const uint32_t*>(l);
-    }
-#pragma unroll
-    for (int v = 0; v < VEC; ++v)
-      if (!((b[v / 4] >> (v % 4 * 8)) & 0xff)) f[v] = -INFINITY;
-  } else {
-#pragma unroll
-    for (int v = 0; v < VEC; ++v)
-      if (i + v < w && !l[v]) f[v] = -INFINITY;
-  }
-}
-
-// Maximum and sums over a team of a warp (WARP) or a block.
-template <bool WARP>
+// Maximum and sums over a team of G lanes, or a block (G = 0).
+template <int G>
 __device__ __forceinline__ float team_max(float v, float* buf) {
-  return WARP ? warp_max_nan(v) : block_max_nan(v, buf);
+  if (G == 0) return block_max_nan(v, buf);
+#pragma unroll
+  for (int o = (G ? G : 32) / 2; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(QQT_FULL, v, o));
+  return v;
 }
-template <bool WARP>
+template <int G>
 __device__ __forceinline__ float team_add(float v, float* buf) {
-  return WARP ? warp_sum_f(v) : block_sum(v, buf);
+  if (G == 0) return block_sum(v, buf);
+#pragma unroll
+  for (int o = (G ? G : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(QQT_FULL, v, o);
+  return v;
 }
 
-template <class T, bool WARP, bool LEGAL>
-__global__ void __launch_bounds__(PL_THREADS, PL_MINB)
+template <class T, int G, bool LEGAL>
+__global__ void __launch_bounds__(kPlThreads, kPlThreads == 512 ? 2 : 1)
     k_pl_rows(QqtPolicyLoss a, const int* __restrict__ counts, float* __restrict__ part) {
-  constexpr int VEC = 16 / sizeof(T), U = 4;
+  constexpr int VEC = 16 / sizeof(T), U = 4, LANES = G ? G : 32;
+  using L = Logits<T, VEC>;
   __shared__ float buf[32];
-  const int j0 = WARP ? 0 : (int)threadIdx.x - lane_id();   // the warp's first vector
-  const int step = WARP ? 32 : (int)blockDim.x;
-  const int64_t r = WARP ? (int64_t)blockIdx.x * (blockDim.x / 32) + warp_id() : (int64_t)blockIdx.x;
-  if (WARP && r >= a.rows) return;
-  const int lead = WARP ? lane_id() : (int)threadIdx.x;
+  // this thread's first vector, the warp's first, and the step between vectors
+  const int tl = G ? lane_id() % LANES : (int)threadIdx.x;
+  const int wj = G ? 0 : (int)threadIdx.x - lane_id(), step = G ? G : (int)blockDim.x;
+  int64_t r = G ? (int64_t)blockIdx.x * (blockDim.x / LANES) + threadIdx.x / LANES
+                : (int64_t)blockIdx.x;
+  const bool exists = r < a.rows;
+  if (G && !exists) r = a.rows - 1;
+  const bool lead = tl == 0 && exists;
   const T* z = (const T*)a.logits + r * a.row_stride;
   const uint8_t* legal = LEGAL ? a.legal + r * a.legal_stride : nullptr;
   HeadStat hs[QQT_MAX_HEADS];
@@ -447,27 +592,18 @@ __global__ void __launch_bounds__(PL_THREADS, PL_MINB)
     float m = -INFINITY;
     uint64_t s2 = pair(0.f, 0.f), e2 = s2;
 #pragma unroll 1
-    for (int jb = j0; jb < nv; jb += step * U) {
-      float f[U][VEC];
-      {
-        Vec<T, VEC> c[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          c[u] = get_logits<T, VEC>(p, sh, jb + lane_id() + u * step, w);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) f[u][v] = c[u].get(v);
-      }
+    for (int jb = 0; jb + wj < nv; jb += step * U) {
+      Vec<T, VEC> c[U];
+      const int j = jb + tl;
+      const bool inner = jb + wj > 0 && (jb + wj + (U - 1) * step + LANES + 1) * VEC <= w;
+      get_chunk<T, VEC, U>(p, sh, j, step, w, inner, c);
       if (LEGAL)
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (jb + lane_id() + u * step < nv) bar_illegal<VEC>(legal + at, jb + lane_id() + u * step, w, f[u]);
+          if (j + u * step < nv) bar_illegal<T, VEC>(c[u], legal + at, j + u * step, w);
       float mx = m;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) mx = max_nan(mx, f[u][v]);
+      for (int u = 0; u < U; ++u) mx = L::top(mx, c[u]);
       if (mx == -INFINITY) continue;       // nothing legal so far
       if (mx != m) {                       // rescale: e^(z - m) (z - m) moves with m too
         const float dm = max_nan(m - mx, kFloor), sc = ex2_approx(dm * kLog2e);
@@ -476,33 +612,27 @@ __global__ void __launch_bounds__(PL_THREADS, PL_MINB)
         s2 = mul2(s2, sc2);
         m = mx;
       }
-      const uint64_t nm = pair(-m, -m), l2 = pair(kLog2e, kLog2e);
+      if (L::kSafe && fabsf(m) < L::kBound) {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int v = 0; v < VEC; v += 2) {
-          float t0, t1, x0, x1;
-          unpair(add2(pair(f[u][v], f[u][v + 1]), nm), t0, t1);
-          const uint64_t t = pair(max_nan(t0, kFloor), max_nan(t1, kFloor));
-          unpair(mul2(t, l2), x0, x1);
-          const uint64_t x = pair(ex2_approx(x0), ex2_approx(x1));
-          s2 = add2(s2, x);
-          e2 = fma2(x, t, e2);
-        }
+        for (int u = 0; u < U; ++u) L::lift(c[u]);
+        add_exps<T, VEC, U, L::kSafe>(c, m, s2, e2);
+      } else {
+        add_exps<T, VEC, U, false>(c, m, s2, e2);
+      }
     }
     float s, e, hi;
     unpair(s2, s, hi);
     s += hi;
     unpair(e2, e, hi);
     e += hi;
-    const float top = team_max<WARP>(m, buf);
+    const float top = team_max<G>(m, buf);
     const float dm = m == -INFINITY ? kFloor : max_nan(m - top, kFloor);
     const float sc = m == -INFINITY ? 0.f : ex2_approx(dm * kLog2e);
-    e = team_add<WARP>(sc * fmaf(dm, s, e), buf);
-    s = team_add<WARP>(sc * s, buf);
+    e = team_add<G>(sc * fmaf(dm, s, e), buf);
+    s = team_add<G>(sc * s, buf);
     const int64_t act = a.actions[r * a.action_stride + h];
     const bool in = act >= 0 && act < w;
-    if (!in && lead == 0) flag_error(QQT_DEV_BAD_ACTION);
+    if (!in && lead) flag_error(QQT_DEV_BAD_ACTION);
     HeadStat k;
     k.act = in ? (int)act : -1;
     logp += finish_head(k, top, s, e, in && !(LEGAL && !legal[at + act]) ? to_f(p[act]) : -INFINITY,
@@ -511,14 +641,14 @@ __global__ void __launch_bounds__(PL_THREADS, PL_MINB)
     hs[h] = k;
     at += w;
   }
-  if (lead == 0) {
+  if (lead) {
     if (a.logp) a.logp[r] = logp;
     if (a.entropy) a.entropy[r] = ent;
   }
   if (!a.old_logp) return;
   const bool live = logp != -INFINITY && (!a.mask || a.mask[r]);
   const RowLoss l = loss_of(a, r, logp, live);
-  if (a.stats && lead == 0)
+  if (a.stats && lead)
     *reinterpret_cast<float4*>(part + r * 4) =
         make_float4(l.pg, l.kl, live ? ent : 0.f, l.clip);
   if (!a.dlogits) return;
@@ -535,33 +665,31 @@ __global__ void __launch_bounds__(PL_THREADS, PL_MINB)
     const int sh = misfit(p), qsh = misfit(q);
     const HeadGrad g = head_grad(k, l.g, a.entropy_coef, scale);
     const float ga = live ? action_grad(k, l.g, a.entropy_coef, scale) : 0.f;
-    const uint64_t nm = pair(-k.m, -k.m), l2 = pair(kLog2e, kLog2e), cs = pair(g.c_s, g.c_s),
-                   ks = pair(g.k_s, g.k_s), sc = pair(g.scale, g.scale);
+    const int ja = k.act >= 0 ? k.act / VEC : -1;
+    const bool safe = L::kSafe && fabsf(k.m) < L::kBound;
+    const uint64_t nm = pair(-k.m, -k.m), cs = pair(g.c_s, g.c_s), ks = pair(g.k_s, g.k_s),
+                   sc = pair(g.scale, g.scale);
+    constexpr int U2 = 2;
 #pragma unroll 1
-    for (int jb = j0; jb < nv; jb += step * 2) {
-      Vec<T, VEC> c[2];
-      if (live)
+    for (int jb = 0; jb + wj < nv; jb += step * U2) {
+      Vec<T, VEC> c[U2];
+      const int j0 = jb + tl;
+      const bool inner = jb + wj > 0 && (jb + wj + (U2 - 1) * step + LANES + 1) * VEC <= w;
+      if (live) get_chunk<T, VEC, U2>(p, sh, j0, step, w, inner, c);
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          c[u] = get_logits<T, VEC>(p, sh, jb + lane_id() + u * step, w);
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int j = jb + lane_id() + u * step;
+      for (int u = 0; u < U2; ++u) {
+        const int j = j0 + u * step;
         float f[VEC];
         if (live) {
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) f[v] = c[u].get(v);
-          if (LEGAL && j < nv) bar_illegal<VEC>(legal + at, j, w, f);
+          if (LEGAL && j < nv) bar_illegal<T, VEC>(c[u], legal + at, j, w);
+          if (safe) L::lift(c[u]);
 #pragma unroll
           for (int v = 0; v < VEC; v += 2) {
-            float t0, t1, x0, x1;
-            unpair(add2(pair(f[v], f[v + 1]), nm), t0, t1);
-            const uint64_t t = pair(max_nan(t0, kFloor), max_nan(t1, kFloor));
-            unpair(mul2(t, l2), x0, x1);
-            const uint64_t x = pair(ex2_approx(x0), ex2_approx(x1));
-            unpair(mul2(mul2(x, fma2(cs, t, ks)), sc), f[v], f[v + 1]);
+            const float z0 = c[u].get(v), z1 = c[u].get(v + 1);
+            const uint64_t t = safe ? below_top<L::kSafe>(z0, z1, nm) : below_top<false>(z0, z1, nm);
+            unpair(mul2(mul2(exp2_pair(t), fma2(cs, t, ks)), sc), f[v], f[v + 1]);
           }
-          if (j == k.act / VEC) {
+          if (j == ja) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v)
               if (j * VEC + v == k.act) f[v] = ga;
@@ -570,7 +698,7 @@ __global__ void __launch_bounds__(PL_THREADS, PL_MINB)
 #pragma unroll
           for (int v = 0; v < VEC; ++v) f[v] = 0.f;
         }
-        put_grads<T, VEC>(q, qsh, j, w, j < nv, f);
+        put_grads<T, VEC, LANES>(q, qsh, j, w, j < nv && exists, f);
       }
     }
     at += w;
@@ -644,19 +772,27 @@ extern "C" int qqt_policy_loss(const QqtPolicyLoss* a, qqt_stream_t stream) {
         k_pl_small<T><<<(unsigned)blocks, kPlSmallRows, smem, st>>>(args, (int)v, counts, part, one);
         return 0;
       }
-      auto rows = [&](auto warp, auto legal) {
-        constexpr bool WARP = decltype(warp)::value;
-        const int threads = WARP ? 256 : v * (int64_t)sizeof(T) > 65536 * 2 ? PL_THREADS : 256;
-        const unsigned n = (unsigned)(WARP ? (a->rows + 7) / 8 : a->rows);
-        k_pl_rows<T, WARP, decltype(legal)::value><<<n, threads, 0, st>>>(args, counts, part);
+      // a team of 8 lanes holds rows of up to 32 vectors in one step, a warp
+      // rows of up to 256 in two, blocks the rest: 256 threads, 512 where a
+      // row is so long that the blocks of all SMs would read past L2
+      const int64_t bytes = v * (int64_t)sizeof(T);
+      const int g = bytes <= 32 * 16 ? 8 : bytes <= PL_W * 16 ? 32 : 0;
+      const int threads = g || bytes <= 128 * 1024 ? 256 : kPlThreads;
+      const int per = g ? threads / g : 1;
+      const unsigned n = (unsigned)((a->rows + per - 1) / per);
+      auto run = [&](auto gg) {
+        constexpr int G = decltype(gg)::value;
+        if (a->legal)
+          k_pl_rows<T, G, true><<<n, threads, 0, st>>>(args, counts, part);
+        else
+          k_pl_rows<T, G, false><<<n, threads, 0, st>>>(args, counts, part);
       };
-      using std::false_type;
-      using std::true_type;
-      const bool warp = v <= PL_WARP;
-      if (warp && a->legal) rows(true_type{}, true_type{});
-      if (warp && !a->legal) rows(true_type{}, false_type{});
-      if (!warp && a->legal) rows(false_type{}, true_type{});
-      if (!warp && !a->legal) rows(false_type{}, false_type{});
+      if (g == 8)
+        run(std::integral_constant<int, 8>{});
+      else if (g == 32)
+        run(std::integral_constant<int, 32>{});
+      else
+        run(std::integral_constant<int, 0>{});
       return 0;
     });
   if (a->stats && !one)
