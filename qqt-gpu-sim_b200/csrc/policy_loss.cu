@@ -39,11 +39,14 @@ constexpr int kPlCounts = 64;        // blocks that count the mask's rows
 constexpr int kPlFold = 8192;        // rows up to which such a block counts them itself
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFloor = -1.0e4f;    // z - m below it is as good as minus infinity
+constexpr float kRefMost = 1048576.f;   // largest |maximum| that the one-step exponents take
 
+// A head's sums: log p = t - log_s and p = e^t inv_s for t = z less the
+// reference that they were taken against.
 struct HeadStat {
-  float m, inv_s, log_s, ent;
-  int act;                  // the action, -1 where it adds nothing
-  float z_act;
+  float inv_s, log_s, ent;
+  float t_act;              // the action's t
+  int act;                  // the action, -1 where it is none of the head's
 };
 
 // Rows of the mask, at least 1; `counts`: the counting blocks' results.
@@ -110,35 +113,37 @@ __device__ __forceinline__ RowLoss row_loss(float logp, float old, float a, floa
 }
 
 
-__device__ __forceinline__ RowLoss loss_of(const QqtPolicyLoss& a, int64_t r, float logp, bool live) {
-  if (!live) return RowLoss{0.f, 0.f, 0.f, 0.f};
-  return row_loss(logp, a.old_logp[r], a.adv[r], a.ref_logp ? a.ref_logp[r] : 0.f,
-                  a.ref_logp != nullptr, a.clip_low, a.clip_high, a.kl_coef);
-}
-
-// log p of the head's action from its sums, and what the second pass needs.
-__device__ __forceinline__ float finish_head(HeadStat& k, float m, float s, float e, float z_act,
-                                             bool act_ok) {
-  const bool any = m != -INFINITY;
-  k.m = m;
-  k.inv_s = any ? 1.f / s : 0.f;
-  k.log_s = logf(s);
-  k.ent = any ? k.log_s - e * k.inv_s : 0.f;
-  k.z_act = z_act;
-  return any && act_ok && z_act != -INFINITY ? z_act - m - k.log_s : -INFINITY;
-}
-
-// The gradient at a logit t = z - m that is not the action's: with p = e / S,
-// scale (p (c (log p + H) - G)); the terms that may cancel are added before
-// the scale.  At the action's: scale (G (1 - p) + c p (log p + H)).
-struct HeadGrad {
-  float c_s, k_s, scale;               // e (c_s t + k_s) scale
+struct RowIn {
+  float old, adv, ref;
+  bool counts;
 };
-__device__ __forceinline__ HeadGrad head_grad(const HeadStat& k, float g, float c, float scale) {
-  return HeadGrad{c * k.inv_s, (c * (k.ent - k.log_s) - g) * k.inv_s, scale};
+__device__ __forceinline__ RowLoss loss_of(const QqtPolicyLoss& a, const RowIn& in, float logp,
+                                           bool live) {
+  if (!live) return RowLoss{0.f, 0.f, 0.f, 0.f};
+  return row_loss(logp, in.old, in.adv, in.ref, a.ref_logp != nullptr, a.clip_low, a.clip_high,
+                  a.kl_coef);
+}
+
+// log p of the head's action.  any: some category is legal.
+__device__ __forceinline__ float finish_head(HeadStat& k, bool any, float s, float log_s, float e,
+                                             float t_act, bool act_ok) {
+  k.inv_s = any ? 1.f / s : 0.f;
+  k.log_s = log_s;
+  k.ent = any ? log_s - e * k.inv_s : 0.f;
+  k.t_act = t_act;
+  return any && act_ok ? t_act - log_s : -INFINITY;
+}
+
+// The gradient at a logit that is not the action's, with p = e / S:
+// scale (p (c (log p + H) - G)) = scale e (c_s t + k_s); the terms that may
+// cancel are added before the scale.  At the action's:
+// scale (G (1 - p) + c p (log p + H)).
+__device__ __forceinline__ float head_c(const HeadStat& k, float c) { return c * k.inv_s; }
+__device__ __forceinline__ float head_k(const HeadStat& k, float g, float c) {
+  return (c * (k.ent - k.log_s) - g) * k.inv_s;
 }
 __device__ __forceinline__ float action_grad(const HeadStat& k, float g, float c, float scale) {
-  const float lp = k.z_act - k.m - k.log_s, p = expf(lp);
+  const float lp = k.t_act - k.log_s, p = expf(lp);
   return scale * fmaf(g, 1.f - p, p * (c * (lp + k.ent)));
 }
 
@@ -183,6 +188,7 @@ __global__ void __launch_bounds__(kPlSmallRows)
   const int64_t r = r0 + threadIdx.x;
   float* z = zs + threadIdx.x * pitch;
   HeadStat hs[QQT_MAX_HEADS];
+  float ms[QQT_MAX_HEADS];
   float logp = 0.f, ent = 0.f;
   if (on) {
     int at = 0;
@@ -201,7 +207,10 @@ __global__ void __launch_bounds__(kPlSmallRows)
       }
       HeadStat k;
       k.act = in ? at + (int)act : -1;
-      logp += finish_head(k, m, s, e, in ? z[at + act] : -INFINITY, in);
+      const float za = in ? z[at + act] : -INFINITY;
+      logp += finish_head(k, m != -INFINITY, s, logf(s), e, za - m, za != -INFINITY);
+      k.t_act = za == -INFINITY ? 0.f : za - m;
+      ms[h] = m;
       ent += k.ent;
       hs[h] = k;
       at += w;
@@ -212,8 +221,15 @@ __global__ void __launch_bounds__(kPlSmallRows)
   if (!loss) return;
   if (fold) __syncthreads();
   const float count = fold ? fmaxf((float)n_mask, 1.f) : rows_counted(a, counts);
-  const bool live = on && logp != -INFINITY && (!a.mask || a.mask[r]);
-  const RowLoss l = loss_of(a, r, logp, live);
+  RowIn row{0.f, 0.f, 0.f, true};
+  if (on) {
+    row.old = a.old_logp[r];
+    row.adv = a.adv[r];
+    if (a.ref_logp) row.ref = a.ref_logp[r];
+    if (a.mask) row.counts = a.mask[r] != 0;
+  }
+  const bool live = on && logp != -INFINITY && row.counts;
+  const RowLoss l = loss_of(a, row, logp, live);
   if (a.stats) {
     const float v[4] = {l.pg, l.kl, live ? ent : 0.f, l.clip};
     float sum[4];
@@ -240,10 +256,10 @@ __global__ void __launch_bounds__(kPlSmallRows)
     for (int h = 0; h < a.n_heads; ++h) {
       const int w = a.width[h];
       const HeadStat k = hs[h];
-      const HeadGrad q = head_grad(k, l.g, a.entropy_coef, scale);
+      const float m = ms[h], cs = head_c(k, a.entropy_coef), ks = head_k(k, l.g, a.entropy_coef);
       for (int j = 0; j < w; ++j) {
-        const float t = max_nan(z[at + j] - k.m, kFloor);
-        z[at + j] = live ? expf(t) * fmaf(q.c_s, t, q.k_s) * scale : 0.f;
+        const float t = max_nan(z[at + j] - m, kFloor);
+        z[at + j] = live ? expf(t) * fmaf(cs, t, ks) * scale : 0.f;
       }
       if (live) z[k.act] = action_grad(k, l.g, a.entropy_coef, scale);
       at += w;
@@ -269,26 +285,27 @@ __global__ void __launch_bounds__(kPlSmallRows)
 // ------------------------------------------------- many logits: team per row
 
 // Pairs of floats in one instruction each.
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-  uint64_t r;
+typedef uint64_t f32x2;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+  f32x2 r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
   return r;
 }
-__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
+__device__ __forceinline__ void unpair(f32x2 v, float& lo, float& hi) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
 }
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
@@ -314,28 +331,11 @@ __device__ __forceinline__ uint4 funnel(uint4 a, uint4 b, int s) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Vector j of the w elements from p, minus infinity past them.  sh: elements
-// between p and the 16-byte boundary below it.  Reads no element outside.
-template <class T, int VEC>
-__device__ __forceinline__ Vec<T, VEC> get_logits(const T* p, int sh, int j, int w) {
-  const int i = j * VEC;
-  uint4 r;
-  if (sh == 0 && i + VEC <= w) {
-    r = *reinterpret_cast<const uint4*>(p + i);
-  } else if (sh && i >= sh && i - sh + 2 * VEC <= w) {
-    const uint4* q = reinterpret_cast<const uint4*>(p + i - sh);
-    r = funnel<T, VEC>(q[0], q[1], sh);
-  } else {
-    float f[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) f[v] = i + v < w ? to_f(p[i + v]) : -INFINITY;
-    Vec<T, VEC> x;
-    x.put(f);
-    return x;
-  }
-  return *reinterpret_cast<const Vec<T, VEC>*>(&r);
-}
-// Vectors j, j + step, ...  inner: none of the warp's is at an end of the row.
+// Vectors j, j + step, ... of the w elements from p, minus infinity past them.
+// sh: elements between p and the 16-byte boundary below it.  inner: none of
+// the warp's vectors is at an end of the row.  Else all whole words are asked
+// for before the ends are seen to, which go element by element; nothing
+// outside the row is read.
 template <class T, int VEC, int U>
 __device__ __forceinline__ void get_chunk(const T* p, int sh, int j, int step, int w, bool inner,
                                           Vec<T, VEC>* c) {
@@ -346,7 +346,9 @@ __device__ __forceinline__ void get_chunk(const T* p, int sh, int j, int step, i
       const uint4 r = *q;
       c[u] = *reinterpret_cast<const Vec<T, VEC>*>(&r);
     }
-  } else if (inner) {
+    return;
+  }
+  if (inner) {
     const uint4* q = reinterpret_cast<const uint4*>(p - sh) + j;
     uint4 lo[U], hi[U];
 #pragma unroll
@@ -359,21 +361,62 @@ __device__ __forceinline__ void get_chunk(const T* p, int sh, int j, int step, i
       const uint4 r = funnel<T, VEC>(lo[u], hi[u], sh);
       c[u] = *reinterpret_cast<const Vec<T, VEC>*>(&r);
     }
-  } else {
+    return;
+  }
+  const int i0 = j * VEC, di = step * VEC;
+  bool ok[U];
+  if (sh == 0) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) c[u] = get_logits<T, VEC>(p, sh, j + u * step, w);
+    for (int u = 0; u < U; ++u) {
+      ok[u] = i0 + u * di + VEC <= w;
+      uint4 r = make_uint4(0, 0, 0, 0);
+      if (ok[u]) r = *reinterpret_cast<const uint4*>(p + (i0 + u * di));
+      c[u] = *reinterpret_cast<const Vec<T, VEC>*>(&r);
+    }
+  } else {
+    uint4 lo[U], hi[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * di - sh;
+      ok[u] = i >= 0 && i + 2 * VEC <= w;
+      lo[u] = hi[u] = make_uint4(0, 0, 0, 0);
+      if (ok[u]) {
+        const uint4* q = reinterpret_cast<const uint4*>(p + i);
+        lo[u] = q[0];
+        hi[u] = q[1];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint4 r = funnel<T, VEC>(lo[u], hi[u], sh);
+      c[u] = *reinterpret_cast<const Vec<T, VEC>*>(&r);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (!ok[u]) {
+      const int i = i0 + u * di;
+      float f[VEC];
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) f[v] = -INFINITY;
+      if (i < w) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v)
+          if (i + v < w) f[v] = to_f(p[i + v]);
+      }
+      c[u].put(f);
+    }
   }
 }
 
 // What is done to a vector before it is taken apart into floats: minus
-// infinity in illegal places, the maximum, and a finite floor (so that a
-// weight of 0 times z - m is 0).
+// infinity in illegal places, the maximum, and a finite floor whose e^t is 0
+// beside any maximum above -kLow (a weight of 0 times t is then 0).
 template <class T, int VEC>
 struct Logits;
 template <int VEC>
 struct Logits<float, VEC> {
-  static constexpr bool kSafe = false;   // z - m may be minus infinity
-  static constexpr float kBound = 0.f;
+  static constexpr float kLow = 1048576.f;
   __device__ static __forceinline__ void bar(Vec<float, VEC>& x, const uint32_t* legal4) {
 #pragma unroll
     for (int v = 0; v < VEC; ++v)
@@ -385,14 +428,17 @@ struct Logits<float, VEC> {
       asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(m), "f"(x.v[v]), "f"(x.v[v + 1]));
     return m;
   }
-  __device__ static __forceinline__ void lift(Vec<float, VEC>&) {}
+  __device__ static __forceinline__ void lift(Vec<float, VEC>& x) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) x.v[v] = max_nan(x.v[v], -1.0e30f);
+  }
 };
 template <class T>
 struct Half2;
 template <>
 struct Half2<__half> {
-  static constexpr uint32_t kNegInf = 0xfc00fc00u, kLowest = 0xfbfffbffu;
-  static constexpr float kBound = 3.0e4f;
+  static constexpr uint32_t kNegInf = 0xfc00fc00u, kFloor = 0xfbfffbffu;   // -65504
+  static constexpr float kLow = 3.0e4f;
   __device__ static __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -401,8 +447,8 @@ struct Half2<__half> {
 };
 template <>
 struct Half2<__nv_bfloat16> {
-  static constexpr uint32_t kNegInf = 0xff80ff80u, kLowest = 0xff7fff7fu;
-  static constexpr float kBound = 1.0e30f;
+  static constexpr uint32_t kNegInf = 0xff80ff80u, kFloor = 0xf149f149u;   // about -1e30
+  static constexpr float kLow = 1048576.f;
   __device__ static __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -411,10 +457,7 @@ struct Half2<__nv_bfloat16> {
 };
 template <class T, int VEC>
 struct Logits16 {
-  // after lift() z - m is finite, and what was minus infinity still adds 0,
-  // while |m| is below kBound
-  static constexpr bool kSafe = true;
-  static constexpr float kBound = Half2<T>::kBound;
+  static constexpr float kLow = Half2<T>::kLow;
   __device__ static __forceinline__ void bar(Vec<T, VEC>& x, const uint32_t* legal4) {
 #pragma unroll
     for (int k = 0; k < VEC / 4; ++k) {
@@ -435,7 +478,7 @@ struct Logits16 {
   }
   __device__ static __forceinline__ void lift(Vec<T, VEC>& x) {
 #pragma unroll
-    for (int k = 0; k < VEC / 2; ++k) x.w[k] = Half2<T>::max(x.w[k], Half2<T>::kLowest);
+    for (int k = 0; k < VEC / 2; ++k) x.w[k] = Half2<T>::max(x.w[k], Half2<T>::kFloor);
   }
 };
 template <int VEC>
@@ -468,32 +511,28 @@ __device__ __forceinline__ void bar_illegal(Vec<T, VEC>& x, const uint8_t* legal
   Logits<T, VEC>::bar(x, b);
 }
 
-// z - m of a pair of places, as floats of at least kFloor where SAFE is not given.
-template <bool SAFE>
-__device__ __forceinline__ uint64_t below_top(float z0, float z1, uint64_t nm) {
-  const uint64_t t = add2(pair(z0, z1), nm);
-  if (SAFE) return t;
-  float t0, t1;
-  unpair(t, t0, t1);
-  return pair(max_nan(t0, kFloor), max_nan(t1, kFloor));
+// Exponents are taken in base 2 against a whole number r near the maximum:
+// t = z log2 e - r in one fused step, r without a rounding of its own, and a
+// change of r scales the sums by an exact power of 2.
+template <class L>
+__device__ __forceinline__ float whole_ref(float m) {
+  return rintf(fminf(fmaxf(m, -L::kLow), kRefMost) * kLog2e);
 }
-__device__ __forceinline__ uint64_t exp2_pair(uint64_t t) {
+__device__ __forceinline__ f32x2 exp2_pair(f32x2 t) {
   float x0, x1;
-  unpair(mul2(t, pair(kLog2e, kLog2e)), x0, x1);
+  unpair(t, x0, x1);
   return pair(ex2_approx(x0), ex2_approx(x1));
 }
-template <class T, int VEC, int U, bool SAFE>
-__device__ __forceinline__ void add_exps(const Vec<T, VEC>* c, float m, uint64_t& s2, uint64_t& e2) {
-  const uint64_t nm = pair(-m, -m);
+template <class T, int VEC>
+__device__ __forceinline__ void add_exps(const Vec<T, VEC>& c, float ref, f32x2& s2, f32x2& e2) {
+  const f32x2 nr = pair(-ref, -ref), l2 = pair(kLog2e, kLog2e);
 #pragma unroll
-  for (int u = 0; u < U; ++u)
-#pragma unroll
-    for (int v = 0; v < VEC; v += 2) {
-      const uint64_t t = below_top<SAFE>(c[u].get(v), c[u].get(v + 1), nm);
-      const uint64_t x = exp2_pair(t);
-      s2 = add2(s2, x);
-      e2 = fma2(x, t, e2);
-    }
+  for (int v = 0; v < VEC; v += 2) {
+    const f32x2 t = fma2(pair(c.get(v), c.get(v + 1)), l2, nr);
+    const f32x2 x = exp2_pair(t);
+    s2 = add2(s2, x);
+    e2 = fma2(x, t, e2);
+  }
 }
 
 // Stores vector j of the w elements from p; every lane of the warp calls it,
@@ -501,9 +540,8 @@ __device__ __forceinline__ void add_exps(const Vec<T, VEC>* c, float m, uint64_t
 // is not on a 16-byte boundary each lane stores the aligned word that its
 // vector's first elements and the lane below's last ones make up.
 template <class T, int VEC, int G>
-__device__ __forceinline__ void put_grads(T* p, int sh, int j, int w, bool on, const float* f) {
-  Vec<T, VEC> x;
-  x.put(f);
+__device__ __forceinline__ void put_grads(T* p, int sh, int j, int w, bool on,
+                                          const Vec<T, VEC>& x) {
   const int i = j * VEC;
   if (sh == 0) {
     if (on && i + VEC <= w) {
@@ -511,7 +549,7 @@ __device__ __forceinline__ void put_grads(T* p, int sh, int j, int w, bool on, c
     } else if (on) {
 #pragma unroll
       for (int v = 0; v < VEC; ++v)
-        if (i + v < w) p[i + v] = from_f<T>(f[v]);
+        if (i + v < w) p[i + v] = from_f<T>(x.get(v));
     }
   }
   // (teams of a warp are on rows of their own alignment)
@@ -534,7 +572,7 @@ __device__ __forceinline__ void put_grads(T* p, int sh, int j, int w, bool on, c
 #pragma unroll
   for (int v = 0; v < VEC; ++v)
     if (i + v < w && ((v < first && !joined) || (v >= first && !over)))
-      p[i + v] = from_f<T>(f[v]);
+      p[i + v] = from_f<T>(x.get(v));
   // ... and the last ones of the lane below a vector that ends before it can join
   if (l > 0 && !joined) {
     const Vec<T, VEC> b = *reinterpret_cast<const Vec<T, VEC>*>(&under);
@@ -549,20 +587,73 @@ __device__ __forceinline__ int misfit(const T* p) {
   return (int)(((uintptr_t)p & 15) / sizeof(T));
 }
 
-// Maximum and sums over a team of G lanes, or a block (G = 0).
-template <int G>
-__device__ __forceinline__ float team_max(float v, float* buf) {
-  if (G == 0) return block_max_nan(v, buf);
-#pragma unroll
-  for (int o = (G ? G : 32) / 2; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(QQT_FULL, v, o));
-  return v;
+// Joins maximum, reference and sums over a team of G lanes, or a block (G =
+// 0): each side's sums are brought to the largest reference.
+struct Sums {
+  float m, r, s, e;
+};
+__device__ __forceinline__ void move_ref(Sums& q, float r) {
+  const float d = q.r - r, sc = ex2_approx(d);
+  q.e = sc * fmaf(d, q.s, q.e);
+  q.s = sc * q.s;
+  q.r = r;
 }
 template <int G>
-__device__ __forceinline__ float team_add(float v, float* buf) {
-  if (G == 0) return block_sum(v, buf);
+__device__ __forceinline__ void join_lanes(Sums& q) {
+  float r = q.r;
 #pragma unroll
-  for (int o = (G ? G : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(QQT_FULL, v, o);
-  return v;
+  for (int o = G / 2; o > 0; o >>= 1) {
+    q.m = max_nan(q.m, __shfl_xor_sync(QQT_FULL, q.m, o));
+    r = fmaxf(r, __shfl_xor_sync(QQT_FULL, r, o));
+  }
+  move_ref(q, r);
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) {
+    q.s += __shfl_xor_sync(QQT_FULL, q.s, o);
+    q.e += __shfl_xor_sync(QQT_FULL, q.e, o);
+  }
+}
+template <int G>
+__device__ __forceinline__ void join(Sums& q, float4* buf) {
+  join_lanes<G ? G : 32>(q);
+  if (G == 0) {
+    const int l = lane_id(), nw = blockDim.x >> 5;
+    if (l == 0) buf[warp_id()] = make_float4(q.m, q.r, q.s, q.e);
+    __syncthreads();
+    const bool one = l % 16 < nw;          // (both halves of the warp do the same)
+    const float4 v = buf[one ? l % 16 : 0];
+    q = Sums{v.x, v.y, one ? v.z : 0.f, one ? v.w : 0.f};
+    join_lanes<16>(q);
+  }
+}
+
+// The same sums against the maximum itself, element by element: for maxima
+// that the one-step exponents do not take, NaN among them.
+template <class T>
+__device__ __forceinline__ float plain_t(const T* p, const uint8_t* legal, int i, float m) {
+  const float z = legal && !legal[i] ? -INFINITY : to_f(p[i]);
+  return max_nan(z - m, kFloor);
+}
+template <class T, int G>
+__device__ __noinline__ void plain_sums(const T* p, const uint8_t* legal, int w, int tl, int step,
+                                        Sums& q, float* buf) {
+  float s = 0.f, e = 0.f;
+  for (int i = tl; i < w; i += step) {
+    const float t = plain_t(p, legal, i, q.m), x = expf(t);
+    s += x;
+    e = fmaf(x, t, e);
+  }
+#pragma unroll
+  for (int o = (G ? G : 32) / 2; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(QQT_FULL, s, o);
+    e += __shfl_xor_sync(QQT_FULL, e, o);
+  }
+  if (G == 0) {
+    s = block_sum(lane_id() == 0 ? s : 0.f, buf);
+    e = block_sum(lane_id() == 0 ? e : 0.f, buf);
+  }
+  q.s = s;
+  q.e = e;
 }
 
 template <class T, int G, bool LEGAL>
@@ -570,7 +661,8 @@ __global__ void __launch_bounds__(kPlThreads, kPlThreads == 512 ? 2 : 1)
     k_pl_rows(QqtPolicyLoss a, const int* __restrict__ counts, float* __restrict__ part) {
   constexpr int VEC = 16 / sizeof(T), U = 4, LANES = G ? G : 32;
   using L = Logits<T, VEC>;
-  __shared__ float buf[32];
+  __shared__ float4 buf[2][16];          // two heads in turn
+  __shared__ float plain_buf[32];
   // this thread's first vector, the warp's first, and the step between vectors
   const int tl = G ? lane_id() % LANES : (int)threadIdx.x;
   const int wj = G ? 0 : (int)threadIdx.x - lane_id(), step = G ? G : (int)blockDim.x;
@@ -579,64 +671,93 @@ __global__ void __launch_bounds__(kPlThreads, kPlThreads == 512 ? 2 : 1)
   const bool exists = r < a.rows;
   if (G && !exists) r = a.rows - 1;
   const bool lead = tl == 0 && exists;
+  // what the row's end needs is asked for at its start
+  RowIn in{0.f, 0.f, 0.f, true};
+  int n_counted = 0;
+  if (a.old_logp) {
+    in.old = a.old_logp[r];
+    in.adv = a.adv[r];
+    if (a.ref_logp) in.ref = a.ref_logp[r];
+    if (a.mask) {
+      in.counts = a.mask[r] != 0;
+      n_counted = counts[lane_id()] + counts[lane_id() + 32];
+    }
+  }
   const T* z = (const T*)a.logits + r * a.row_stride;
   const uint8_t* legal = LEGAL ? a.legal + r * a.legal_stride : nullptr;
   HeadStat hs[QQT_MAX_HEADS];
+  float refs[QQT_MAX_HEADS];
+  unsigned plain = 0;                    // heads whose sums are against the maximum itself
   float logp = 0.f, ent = 0.f;
   int at = 0;
 #pragma unroll 1
   for (int h = 0; h < a.n_heads; ++h) {
     const int w = a.width[h], nv = (w + VEC - 1) / VEC;
     const T* p = z + at;
+    const uint8_t* lg = LEGAL ? legal + at : nullptr;
     const int sh = misfit(p);
-    float m = -INFINITY;
-    uint64_t s2 = pair(0.f, 0.f), e2 = s2;
+    const int64_t act = a.actions[r * a.action_stride + h];
+    const bool in_head = act >= 0 && act < w;
+    const float z_act = in_head && !(LEGAL && !lg[act]) ? to_f(p[act]) : -INFINITY;
+    Sums q{-INFINITY, whole_ref<L>(-INFINITY), 0.f, 0.f};
+    f32x2 s2 = pair(0.f, 0.f), e2 = s2;
 #pragma unroll 1
     for (int jb = 0; jb + wj < nv; jb += step * U) {
       Vec<T, VEC> c[U];
       const int j = jb + tl;
-      const bool inner = jb + wj > 0 && (jb + wj + (U - 1) * step + LANES + 1) * VEC <= w;
-      get_chunk<T, VEC, U>(p, sh, j, step, w, inner, c);
+      const bool inner = (sh == 0 || jb + wj > 0) &&
+                         (jb + wj + (U - 1) * step + LANES + (sh ? 1 : 0)) * VEC <= w;
+      get_chunk<T, VEC, U>(p, sh, j, step, w, G == 8 ? false : inner, c);
       if (LEGAL)
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (j + u * step < nv) bar_illegal<T, VEC>(c[u], legal + at, j + u * step, w);
-      float mx = m;
+          if (j + u * step < nv) bar_illegal<T, VEC>(c[u], lg, j + u * step, w);
+      float m = q.m;
 #pragma unroll
-      for (int u = 0; u < U; ++u) mx = L::top(mx, c[u]);
-      if (mx == -INFINITY) continue;       // nothing legal so far
-      if (mx != m) {                       // rescale: e^(z - m) (z - m) moves with m too
-        const float dm = max_nan(m - mx, kFloor), sc = ex2_approx(dm * kLog2e);
-        const uint64_t sc2 = pair(sc, sc);
-        e2 = mul2(fma2(pair(dm, dm), s2, e2), sc2);
-        s2 = mul2(s2, sc2);
-        m = mx;
+      for (int u = 0; u < U; ++u) m = L::top(m, c[u]);
+      if (!(m <= q.m)) {
+        q.m = m;
+        const float ref = fmaxf(q.r, whole_ref<L>(m));
+        const float d = q.r - ref, sc = ex2_approx(d);
+        e2 = mul2(fma2(pair(d, d), s2, e2), pair(sc, sc));
+        s2 = mul2(s2, pair(sc, sc));
+        q.r = ref;
       }
-      if (L::kSafe && fabsf(m) < L::kBound) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) L::lift(c[u]);
-        add_exps<T, VEC, U, L::kSafe>(c, m, s2, e2);
-      } else {
-        add_exps<T, VEC, U, false>(c, m, s2, e2);
+      for (int u = 0; u < U; ++u) {
+        L::lift(c[u]);
+        add_exps<T, VEC>(c[u], q.r, s2, e2);
       }
     }
-    float s, e, hi;
-    unpair(s2, s, hi);
-    s += hi;
-    unpair(e2, e, hi);
-    e += hi;
-    const float top = team_max<G>(m, buf);
-    const float dm = m == -INFINITY ? kFloor : max_nan(m - top, kFloor);
-    const float sc = m == -INFINITY ? 0.f : ex2_approx(dm * kLog2e);
-    e = team_add<G>(sc * fmaf(dm, s, e), buf);
-    s = team_add<G>(sc * s, buf);
-    const int64_t act = a.actions[r * a.action_stride + h];
-    const bool in = act >= 0 && act < w;
-    if (!in && lead) flag_error(QQT_DEV_BAD_ACTION);
+    float hi;
+    unpair(s2, q.s, hi);
+    q.s += hi;
+    unpair(e2, q.e, hi);
+    q.e += hi;
+    join<G>(q, buf[h & 1]);
+    const bool any = q.m != -INFINITY;
+    const bool one_step = q.m >= -L::kLow && q.m <= kRefMost;
     HeadStat k;
-    k.act = in ? (int)act : -1;
-    logp += finish_head(k, top, s, e, in && !(LEGAL && !legal[at + act]) ? to_f(p[act]) : -INFINITY,
-                        in);
+    if (!in_head && lead) flag_error(QQT_DEV_BAD_ACTION);
+    k.act = in_head ? (int)act : -1;
+    float lp;
+    // (teams of one warp go together: whoever does not need it leaves it unused)
+    if (G == 8 ? __any_sync(QQT_FULL, any && !one_step) : any && !one_step) {
+      Sums qp = q;
+      plain_sums<T, G>(p, lg, w, tl, step, qp, plain_buf);
+      if (any && !one_step) q = qp;
+    }
+    if (any && !one_step) {
+      plain |= 1u << h;
+      lp = finish_head(k, any, q.s, logf(q.s), q.e, max_nan(z_act - q.m, kFloor),
+                       z_act != -INFINITY);
+      refs[h] = q.m;
+    } else {
+      const float ta = fmaf(max_nan(z_act, -1.0e30f), kLog2e, -q.r) * kLn2;
+      lp = finish_head(k, any, q.s, log2f(q.s) * kLn2, q.e * kLn2, ta, z_act != -INFINITY);
+      refs[h] = q.r;
+    }
+    logp += lp;
     ent += k.ent;
     hs[h] = k;
     at += w;
@@ -646,14 +767,14 @@ __global__ void __launch_bounds__(kPlThreads, kPlThreads == 512 ? 2 : 1)
     if (a.entropy) a.entropy[r] = ent;
   }
   if (!a.old_logp) return;
-  const bool live = logp != -INFINITY && (!a.mask || a.mask[r]);
-  const RowLoss l = loss_of(a, r, logp, live);
+  const bool live = logp != -INFINITY && in.counts;
+  const RowLoss l = loss_of(a, in, logp, live);
   if (a.stats && lead)
     *reinterpret_cast<float4*>(part + r * 4) =
         make_float4(l.pg, l.kl, live ? ent : 0.f, l.clip);
   if (!a.dlogits) return;
-  const float scale =
-      a.grad_scale / rows_counted(a, counts) * (a.upstream ? a.upstream[0] : 1.f);
+  const float n_rows = fmaxf((float)(a.mask ? warp_sum(n_counted) : a.rows), 1.f);
+  const float scale = a.grad_scale / n_rows * (a.upstream ? a.upstream[0] : 1.f);
   T* dz = (T*)a.dlogits + r * a.dlogits_stride;
   at = 0;
 #pragma unroll 1
@@ -661,46 +782,67 @@ __global__ void __launch_bounds__(kPlThreads, kPlThreads == 512 ? 2 : 1)
     const int w = a.width[h], nv = (w + VEC - 1) / VEC;
     const HeadStat k = hs[h];
     const T* p = z + at;
-    T* q = dz + at;
-    const int sh = misfit(p), qsh = misfit(q);
-    const HeadGrad g = head_grad(k, l.g, a.entropy_coef, scale);
-    const float ga = live ? action_grad(k, l.g, a.entropy_coef, scale) : 0.f;
-    const int ja = k.act >= 0 ? k.act / VEC : -1;
-    const bool safe = L::kSafe && fabsf(k.m) < L::kBound;
-    const uint64_t nm = pair(-k.m, -k.m), cs = pair(g.c_s, g.c_s), ks = pair(g.k_s, g.k_s),
-                   sc = pair(g.scale, g.scale);
-    constexpr int U2 = 2;
+    T* o = dz + at;
+    const uint8_t* lg = LEGAL ? legal + at : nullptr;
+    const int sh = misfit(p), osh = misfit(o);
+    const float cn = head_c(k, a.entropy_coef), kn = head_k(k, l.g, a.entropy_coef);
+    if (live && ((plain >> h) & 1)) {    // (G = 8: divergent, no lane needs another)
+      if (exists)
+        for (int i = tl; i < w; i += step) {
+          const float t = plain_t(p, lg, i, refs[h]);
+          if (i != k.act) o[i] = from_f<T>(expf(t) * fmaf(cn, t, kn) * scale);
+        }
+    }
+    const bool skip = live && ((plain >> h) & 1);
+    const float ref = refs[h];
+    const f32x2 nr = pair(-ref, -ref), l2 = pair(kLog2e, kLog2e), cs = pair(cn * kLn2, cn * kLn2),
+                ks = pair(kn, kn), sc = pair(scale, scale);
+    if (G == 8 || !skip) {
 #pragma unroll 1
-    for (int jb = 0; jb + wj < nv; jb += step * U2) {
-      Vec<T, VEC> c[U2];
-      const int j0 = jb + tl;
-      const bool inner = jb + wj > 0 && (jb + wj + (U2 - 1) * step + LANES + 1) * VEC <= w;
-      if (live) get_chunk<T, VEC, U2>(p, sh, j0, step, w, inner, c);
+      for (int jb = 0; jb + wj < nv; jb += step * U) {
+        const int j0 = jb + tl;
+        const int last = jb + wj + (U - 1) * step + LANES;
+        const bool whole = last * VEC <= w && exists && !skip;
+        const bool inner = G != 8 && (sh == 0 || jb + wj > 0) && (last + (sh ? 1 : 0)) * VEC <= w;
+        Vec<T, VEC> c[U];
+        if (live) get_chunk<T, VEC, U>(p, sh, j0, step, w, inner, c);
+        if (LEGAL && live)
 #pragma unroll
-      for (int u = 0; u < U2; ++u) {
-        const int j = j0 + u * step;
-        float f[VEC];
+          for (int u = 0; u < U; ++u)
+            if (j0 + u * step < nv) bar_illegal<T, VEC>(c[u], lg, j0 + u * step, w);
+        float f[U][VEC];
         if (live) {
-          if (LEGAL && j < nv) bar_illegal<T, VEC>(c[u], legal + at, j, w);
-          if (safe) L::lift(c[u]);
 #pragma unroll
-          for (int v = 0; v < VEC; v += 2) {
-            const float z0 = c[u].get(v), z1 = c[u].get(v + 1);
-            const uint64_t t = safe ? below_top<L::kSafe>(z0, z1, nm) : below_top<false>(z0, z1, nm);
-            unpair(mul2(mul2(exp2_pair(t), fma2(cs, t, ks)), sc), f[v], f[v + 1]);
-          }
-          if (j == ja) {
+          for (int u = 0; u < U; ++u) {
+            L::lift(c[u]);
 #pragma unroll
-            for (int v = 0; v < VEC; ++v)
-              if (j * VEC + v == k.act) f[v] = ga;
+            for (int v = 0; v < VEC; v += 2) {
+              const f32x2 t = fma2(pair(c[u].get(v), c[u].get(v + 1)), l2, nr);
+              unpair(mul2(mul2(exp2_pair(t), fma2(cs, t, ks)), sc), f[u][v], f[u][v + 1]);
+            }
+            c[u].put(f[u]);
           }
         } else {
 #pragma unroll
-          for (int v = 0; v < VEC; ++v) f[v] = 0.f;
+          for (int u = 0; u < U; ++u) c[u] = vec_zero<T, VEC>();
         }
-        put_grads<T, VEC, LANES>(q, qsh, j, w, j < nv && exists, f);
+        if (G != 8 && whole && osh == 0) {
+          uint4* q = reinterpret_cast<uint4*>(o) + j0;
+#pragma unroll
+          for (int u = 0; u < U; ++u, q += step) *q = *reinterpret_cast<const uint4*>(&c[u]);
+        } else {
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int j = j0 + u * step;
+            put_grads<T, VEC, LANES>(o, osh, j, w, j < nv && exists && !skip, c[u]);
+          }
+        }
       }
     }
+    // the action's own value, over what its vector's lane or the one above wrote
+    __syncwarp();
+    if (live && exists && k.act / VEC % step == tl)
+      o[k.act] = from_f<T>(action_grad(k, l.g, a.entropy_coef, scale));
     at += w;
   }
 }
