@@ -521,6 +521,12 @@ int qqt_recurrence_forward(const QqtSeq *x, const QqtSeq *gate, const QqtSeq *re
                            const float *h0, int32_t dtype, int64_t T, int64_t N, int64_t D,
                            const QqtSeq *h, float *h_last, float *carry, void *work,
                            qqt_stream_t stream);
+/* One tick: x, gate rows of N sequences -> h [N][D]; state -> state_out [N][D]
+ * float32 (they may be the same); reset (optional) uint8 (N). */
+int qqt_recurrence_step(const void *x, int64_t x_stride, const void *gate, int64_t gate_stride,
+                        const uint8_t *reset, int64_t reset_stride, const float *state,
+                        int32_t dtype, int64_t N, int64_t D, void *h, float *state_out,
+                        qqt_stream_t stream);
 /* dx, dgate (type dtype) and dh0 (optional) [N][D] for dh (optional) and
  * dh_last (optional) [N][D]. */
 int qqt_recurrence_backward(const QqtSeq *dh, const float *dh_last, const QqtSeq *x,

@@ -29,9 +29,6 @@
 
 namespace qqt {
 
-#ifndef PL_W
-#define PL_W 256
-#endif
 constexpr int kPlThreads = 512;      // largest block on a row
 constexpr int kPlSmall = 32;         // logits of a row that one thread handles
 constexpr int kPlSmallRows = 256;    // rows of such a block
@@ -285,30 +282,11 @@ __global__ void __launch_bounds__(kPlSmallRows)
 // ------------------------------------------------- many logits: team per row
 
 // Pairs of floats in one instruction each.
-typedef uint64_t f32x2;
-__device__ __forceinline__ f32x2 pair(float lo, float hi) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void unpair(f32x2 v, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
+typedef float2 f32x2;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) { return make_float2(lo, hi); }
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) { return __ffma2_rn(a, b, c); }
 
 // The VEC elements from the s-th (0 < s < VEC) of the 2 VEC of a and b.
 template <class T, int VEC>
@@ -519,9 +497,7 @@ __device__ __forceinline__ float whole_ref(float m) {
   return rintf(fminf(fmaxf(m, -L::kLow), kRefMost) * kLog2e);
 }
 __device__ __forceinline__ f32x2 exp2_pair(f32x2 t) {
-  float x0, x1;
-  unpair(t, x0, x1);
-  return pair(ex2_approx(x0), ex2_approx(x1));
+  return pair(ex2_approx(t.x), ex2_approx(t.y));
 }
 template <class T, int VEC>
 __device__ __forceinline__ void add_exps(const Vec<T, VEC>& c, float ref, f32x2& s2, f32x2& e2) {
@@ -729,11 +705,8 @@ __global__ void __launch_bounds__(kPlThreads, kPlThreads == 512 ? 2 : 1)
         add_exps<T, VEC>(c[u], q.r, s2, e2);
       }
     }
-    float hi;
-    unpair(s2, q.s, hi);
-    q.s += hi;
-    unpair(e2, q.e, hi);
-    q.e += hi;
+    q.s = s2.x + s2.y;
+    q.e = e2.x + e2.y;
     join<G>(q, buf[h & 1]);
     const bool any = q.m != -INFINITY;
     const bool one_step = q.m >= -L::kLow && q.m <= kRefMost;
@@ -818,7 +791,9 @@ __global__ void __launch_bounds__(kPlThreads, kPlThreads == 512 ? 2 : 1)
 #pragma unroll
             for (int v = 0; v < VEC; v += 2) {
               const f32x2 t = fma2(pair(c[u].get(v), c[u].get(v + 1)), l2, nr);
-              unpair(mul2(mul2(exp2_pair(t), fma2(cs, t, ks)), sc), f[u][v], f[u][v + 1]);
+              const f32x2 d = mul2(mul2(exp2_pair(t), fma2(cs, t, ks)), sc);
+              f[u][v] = d.x;
+              f[u][v + 1] = d.y;
             }
             c[u].put(f[u]);
           }
@@ -915,11 +890,14 @@ extern "C" int qqt_policy_loss(const QqtPolicyLoss* a, qqt_stream_t stream) {
         return 0;
       }
       // a team of 8 lanes holds rows of up to 32 vectors in one step, a warp
-      // rows of up to 256 in two, blocks the rest: 256 threads, 512 where a
-      // row is so long that the blocks of all SMs would read past L2
+      // walks over rows of up to 1024 (16384 rows x 8192 bf16: 148 us, 195 by
+      // blocks), blocks take the rest, larger ones for long rows, whose second
+      // reading then still finds them in L2 (8192 x 32000 bf16: 233 us with
+      // 256 threads, 292 with 512; 4096 x 32000 f32: 249 and 220).  The choice
+      // does not depend on what is asked for, so neither do a row's sums.
       const int64_t bytes = v * (int64_t)sizeof(T);
-      const int g = bytes <= 32 * 16 ? 8 : bytes <= PL_W * 16 ? 32 : 0;
-      const int threads = g || bytes <= 128 * 1024 ? 256 : kPlThreads;
+      const int g = bytes <= 32 * 16 ? 8 : bytes <= 1024 * 16 ? 32 : 0;
+      const int threads = g || bytes <= 80 * 1024 ? 256 : kPlThreads;
       const int per = g ? threads / g : 1;
       const unsigned n = (unsigned)((a->rows + per - 1) / per);
       auto run = [&](auto gg) {

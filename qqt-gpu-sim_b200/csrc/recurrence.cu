@@ -577,13 +577,6 @@ static int rec_vec(const RecArgs& a, int64_t es) {
 template <class T, bool BWD>
 static int rec_run(const RecArgs& a, void* work, cudaStream_t st) {
   const int vec = rec_vec(a, sizeof(T));
-  if (!BWD && a.nT == 1 && !a.carry) {
-    if (vec == 4)
-      k_rec_step<T, 4><<<(a.nC / 4 + 127) / 128, 128, 0, st>>>(a);
-    else
-      k_rec_step<T, 1><<<(a.nC + 127) / 128, 128, 0, st>>>(a);
-    return launch_status();
-  }
   if constexpr (sizeof(T) == 2 && !BWD) {
     if (vec == 4) return rec_walk<T, 4, BWD>(a, work, st);
   }
@@ -632,6 +625,34 @@ extern "C" int qqt_recurrence_forward(const QqtSeq* x, const QqtSeq* gate, const
   a.nC = (uint32_t)C;
   a.nD = (uint32_t)D;
   return with_dtype(dtype, [&](auto t) { return rec_run<decltype(t), false>(a, work, st); });
+}
+
+extern "C" int qqt_recurrence_step(const void* x, int64_t x_stride, const void* gate,
+                                   int64_t gate_stride, const uint8_t* reset, int64_t reset_stride,
+                                   const float* state, int32_t dtype, int64_t N, int64_t D, void* h,
+                                   float* state_out, qqt_stream_t stream) {
+  if (!dtype_ok(dtype) || !rec_sizes_ok(1, N, D)) return QQT_E_ARG;
+  if (N == 0) return QQT_OK;
+  if (!x || !gate || !state || !h || !state_out) return QQT_E_ARG;
+  RecArgs a{};
+  a.x = RecSeq{x, 0, x_stride};
+  a.g = RecSeq{gate, 0, gate_stride};
+  a.reset = RecSeq{reset, 0, reset_stride};
+  a.h = RecSeq{h, 0, D};
+  a.s0 = state;
+  a.s_end = state_out;
+  a.nT = 1;
+  a.nC = (uint32_t)(N * D);
+  a.nD = (uint32_t)D;
+  return with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (rec_vec(a, sizeof(T)) == 4)
+      k_rec_step<T, 4><<<(a.nC / 4 + 127) / 128, 128, 0, st>>>(a);
+    else
+      k_rec_step<T, 1><<<(a.nC + 127) / 128, 128, 0, st>>>(a);
+    return launch_status();
+  });
 }
 
 extern "C" int qqt_recurrence_backward(const QqtSeq* dh, const float* dh_last, const QqtSeq* x,

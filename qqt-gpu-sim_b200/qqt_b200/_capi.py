@@ -165,6 +165,8 @@ def lib():
             "qqt_recurrence_backward": (c_i32, [P(QqtSeq), c_p, P(QqtSeq), P(QqtSeq), P(QqtSeq),
                                                 c_p, c_i32, c_i64, c_i64, c_i64, P(QqtSeq),
                                                 P(QqtSeq), c_p, c_p, c_p]),
+            "qqt_recurrence_step": (c_i32, [c_p, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_i32, c_i64,
+                                            c_i64, c_p, c_p, c_p]),
             "qqt_recurrence_chunks": (c_i64, [c_i64]),
             "qqt_recurrence_work_bytes": (c_u64, [c_i64, c_i64, c_i64]),
             "qqt_policy_loss": (c_i32, [P(QqtPolicyLoss), c_p]),
@@ -220,24 +222,20 @@ def stream_ptr(device=None) -> int:
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
-def need(ok: bool, what: str, exc=ValueError) -> None:
-    """Argument check of the training operators."""
-    if not ok:
-        raise exc(what)
-
-
-def need_cuda(*tensors) -> None:
-    """All given tensors (None allowed) on one CUDA device, the current one
-    (kernels launch on its current stream)."""
-    dev = tensors[0].device
+def launch_stream(first: torch.Tensor, *others) -> int:
+    """The current stream's handle, once all given tensors (None allowed) are
+    on one CUDA device, the current one (kernels launch there)."""
+    dev = first.device
     if dev.type != "cuda":
         raise ValueError(f"tensors must be on a CUDA device, got {dev}")
-    for t in tensors:
-        if t is not None and t.device != dev:
+    i = dev.index
+    for t in others:
+        if t is not None and t.get_device() != i:
             raise ValueError(f"tensors on different devices: {dev} and {t.device}")
-    if dev.index != torch.cuda.current_device():
+    if i != torch.cuda.current_device():
         raise ValueError(f"tensors on {dev}, but the current device is "
                          f"cuda:{torch.cuda.current_device()}")
+    return torch._C._cuda_getCurrentRawStream(i)
 
 
 def device_error() -> int:

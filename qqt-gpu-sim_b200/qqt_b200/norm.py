@@ -15,35 +15,42 @@ import torch.nn as nn
 
 from . import _capi as capi
 
+_F32 = torch.float32
 
-def _rows(t: torch.Tensor, d: int):
+
+def _rows(t: torch.Tensor, d: int) -> torch.Tensor:
     """t as (rows, d) with a unit inner stride: a view where the layout allows
     one, else a copy."""
-    r = t.reshape(-1, d) if t.numel() else t.new_empty((t.numel() // d, d))
-    if d > 1 and r.stride(1) != 1:
-        r = r.contiguous()
-    return r
+    if t.dim() != 2 or t.shape[1] != d:
+        t = t.reshape(-1, d) if t.numel() else t.new_empty((t.numel() // d, d))
+    return t if d == 1 or t.stride(1) == 1 else t.contiguous()
 
 
-def _check(x, weight, bias, what="x"):
-    capi.need(x.dtype in capi.DTYPES, f"{what} must be float32, float16 or bfloat16, got {x.dtype}",
-              TypeError)
-    capi.need(weight.dtype == torch.float32 and (bias is None or bias.dtype == torch.float32),
-              "weight and bias must be float32", TypeError)
-    nd = weight.dim()
-    capi.need(nd >= 1 and weight.numel() > 0, "weight must have at least one value")
-    capi.need(x.dim() >= nd and x.shape[x.dim() - nd:] == weight.shape,
-              f"{what} of shape {tuple(x.shape)} does not end in {tuple(weight.shape)}")
-    capi.need(bias is None or bias.shape == weight.shape, "bias and weight differ in shape")
+def _check(x, weight, bias) -> int:
+    """The element type's code; raises on arguments that do not go together."""
+    code = capi.DTYPES.get(x.dtype)
+    if code is None:
+        raise TypeError(f"x must be float32, float16 or bfloat16, got {x.dtype}")
+    if weight.dtype is not _F32 or (bias is not None and bias.dtype is not _F32):
+        raise TypeError("weight and bias must be float32")
+    ws, nd = weight.shape, weight.dim()
+    if nd < 1 or weight.numel() == 0:
+        raise ValueError("weight must have at least one value")
+    if x.shape[-nd:] != ws:
+        raise ValueError(f"x of shape {tuple(x.shape)} does not end in {tuple(ws)}")
+    if bias is not None and bias.shape != ws:
+        raise ValueError("bias and weight differ in shape")
+    return code
 
 
 def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
                        eps: float = 1e-5, stats: bool = True):
     """(y, mean, rstd): y of x's shape and type, contiguous; mean and rstd
     float32, one per row (None with stats=False)."""
-    _check(x, weight, bias)
-    capi.need(eps >= 0, "eps must not be negative")
-    capi.need_cuda(x, weight, bias)
+    code = _check(x, weight, bias)
+    if not eps >= 0:
+        raise ValueError("eps must not be negative")
+    stream = capi.launch_stream(x, weight, bias)
     d = weight.numel()
     xr = _rows(x, d)
     w = weight.contiguous()
@@ -52,11 +59,14 @@ def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     mean = rstd = None
     if stats:
-        mean, rstd = torch.empty((2, n), dtype=torch.float32, device=x.device)
-    capi.check(capi.lib().qqt_layernorm_forward(
-        xr.data_ptr(), capi.DTYPES[x.dtype], n, d, xr.stride(0), w.data_ptr(), capi.ptr(b), eps,
-        y.data_ptr(), capi.ptr(mean), capi.ptr(rstd), capi.stream_ptr(x.device)),
-        "qqt_layernorm_forward")
+        mean = torch.empty(n, dtype=_F32, device=x.device)
+        rstd = torch.empty(n, dtype=_F32, device=x.device)
+    rc = capi.lib().qqt_layernorm_forward(
+        xr.data_ptr(), code, n, d, xr.stride(0), w.data_ptr(), None if b is None else b.data_ptr(),
+        eps, y.data_ptr(), None if mean is None else mean.data_ptr(),
+        None if rstd is None else rstd.data_ptr(), stream)
+    if rc:
+        capi.check(rc, "qqt_layernorm_forward")
     return y, mean, rstd
 
 
@@ -64,26 +74,29 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
                         weight: torch.Tensor, need_dx: bool = True, need_dw: bool = True):
     """(dx, dweight, dbias) for dL/dy = dy; dx has x's type, dweight and dbias
     are float32 of the weight's shape (None where not needed)."""
-    _check(x, weight, None)
-    capi.need(dy.shape == x.shape and dy.dtype == x.dtype, "dy must have x's shape and type")
+    code = _check(x, weight, None)
+    if dy.shape != x.shape or dy.dtype is not x.dtype:
+        raise ValueError("dy must have x's shape and type")
     d = weight.numel()
     n = x.numel() // d
-    capi.need(mean.shape == (n,) and rstd.shape == (n,) and mean.dtype == torch.float32
-              and rstd.dtype == torch.float32 and mean.is_contiguous() and rstd.is_contiguous(),
-              "mean and rstd must be the forward pass's")
-    capi.need_cuda(x, dy, mean, rstd, weight)
+    for t in (mean, rstd):
+        if t.dim() != 1 or t.shape[0] != n or t.dtype is not _F32 or not t.is_contiguous():
+            raise ValueError("mean and rstd must be the forward pass's")
+    stream = capi.launch_stream(x, dy, mean, rstd, weight)
+    dev, L = x.device, capi.lib()
     xr, dyr, w = _rows(x, d), _rows(dy, d), weight.contiguous()
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_dx else None
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_dx else None
     dw = db = work = None
-    L = capi.lib()
     if need_dw:
-        dw, db = torch.empty((2,) + tuple(weight.shape), dtype=torch.float32, device=x.device)
-        work = torch.empty(int(L.qqt_layernorm_work_bytes(n, d)), dtype=torch.uint8,
-                           device=x.device)
-    capi.check(L.qqt_layernorm_backward(
-        dyr.data_ptr(), dyr.stride(0), xr.data_ptr(), xr.stride(0), capi.DTYPES[x.dtype], n, d,
-        mean.data_ptr(), rstd.data_ptr(), w.data_ptr(), capi.ptr(dx), capi.ptr(dw), capi.ptr(db),
-        capi.ptr(work), capi.stream_ptr(x.device)), "qqt_layernorm_backward")
+        dw = torch.empty(weight.shape, dtype=_F32, device=dev)
+        db = torch.empty(weight.shape, dtype=_F32, device=dev)
+        work = torch.empty(L.qqt_layernorm_work_bytes(n, d), dtype=torch.uint8, device=dev)
+    rc = L.qqt_layernorm_backward(
+        dyr.data_ptr(), dyr.stride(0), xr.data_ptr(), xr.stride(0), code, n, d, mean.data_ptr(),
+        rstd.data_ptr(), w.data_ptr(), capi.ptr(dx), capi.ptr(dw), capi.ptr(db), capi.ptr(work),
+        stream)
+    if rc:
+        capi.check(rc, "qqt_layernorm_backward")
     return dx, dw, db
 
 
@@ -106,10 +119,10 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
                eps: float = 1e-5) -> torch.Tensor:
     """(x - mean) / sqrt(var + eps) * weight + bias over the weight's trailing
     dimensions of x; differentiable in x, weight and bias."""
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
-                                    or (bias is not None and bias.requires_grad)):
+    if (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)) \
+            and torch.is_grad_enabled():
         return _LayerNorm.apply(x, weight, bias, eps)
-    return layer_norm_forward(x, weight, bias, eps, stats=False)[0]
+    return layer_norm_forward(x, weight, bias, eps, False)[0]
 
 
 class LayerNorm(nn.Module):

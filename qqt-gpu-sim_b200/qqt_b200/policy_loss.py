@@ -25,86 +25,105 @@ import torch
 from . import _capi as capi
 
 
-def _bytes(t: torch.Tensor) -> torch.Tensor:
-    return t.view(torch.uint8) if t.dtype == torch.bool else t
+_F32 = torch.float32
+_FLAGS = (torch.bool, torch.uint8)
 
 
 def _args(logits, actions, legal, heads):
-    """Checked arguments shared by every entry: a filled QqtPolicyLoss and the
-    tensors it points into."""
-    capi.need(logits.dtype in capi.DTYPES,
-              f"logits must be float32, float16 or bfloat16, got {logits.dtype}", TypeError)
-    capi.need(logits.dim() == 2 and logits.shape[1] > 0,
-              f"logits must be (N, V), got {tuple(logits.shape)}")
+    """(QqtPolicyLoss, N, V, stream, tensors it points into) of the arguments
+    that every entry shares; raises on those that do not go together."""
+    code = capi.DTYPES.get(logits.dtype)
+    if code is None:
+        raise TypeError(f"logits must be float32, float16 or bfloat16, got {logits.dtype}")
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError(f"logits must be (N, V), got {tuple(logits.shape)}")
     n, v = logits.shape
-    heads = (v,) if heads is None else tuple(int(w) for w in heads)
-    capi.need(0 < len(heads) <= capi.MAX_HEADS, f"1 to {capi.MAX_HEADS} heads, got {len(heads)}")
-    capi.need(min(heads) > 0 and sum(heads) == v, f"heads {heads} do not add up to {v} logits")
-    capi.need(actions.dtype == torch.int64, "actions must be int64", TypeError)
+    heads = (v,) if heads is None else tuple(heads)
+    nh = len(heads)
+    if not 0 < nh <= capi.MAX_HEADS:
+        raise ValueError(f"1 to {capi.MAX_HEADS} heads, got {nh}")
+    if min(heads) <= 0 or sum(heads) != v:
+        raise ValueError(f"heads {heads} do not add up to {v} logits")
+    if actions.dtype is not torch.int64:
+        raise TypeError("actions must be int64")
     if actions.dim() == 1:
         actions = actions[:, None]
-    capi.need(actions.shape == (n, len(heads)),
-              f"actions must be (N, heads) = {(n, len(heads))}, got {tuple(actions.shape)}")
+    if actions.shape != (n, nh):
+        raise ValueError(f"actions must be (N, heads) = {(n, nh)}, got {tuple(actions.shape)}")
     if legal is not None:
-        capi.need(legal.dtype in (torch.bool, torch.uint8), "legal must be bool or uint8", TypeError)
-        capi.need(legal.shape == (n, v), f"legal must be (N, V), got {tuple(legal.shape)}")
-        legal = _bytes(legal)
+        if legal.dtype not in _FLAGS:
+            raise TypeError("legal must be bool or uint8")
+        if legal.shape != (n, v):
+            raise ValueError(f"legal must be (N, V) = {(n, v)}, got {tuple(legal.shape)}")
         if v > 1 and legal.stride(1) != 1:
             legal = legal.contiguous()
-    capi.need_cuda(logits, actions, legal)
+    stream = capi.launch_stream(logits, actions, legal)
     if v > 1 and logits.stride(1) != 1:
         logits = logits.contiguous()
-    if len(heads) > 1 and actions.stride(1) != 1:
+    if nh > 1 and actions.stride(1) != 1:
         actions = actions.contiguous()
-    a = capi.QqtPolicyLoss(logits.data_ptr(), logits.stride(0), n, capi.ptr(legal),
+    a = capi.QqtPolicyLoss(logits.data_ptr(), logits.stride(0), n,
+                           None if legal is None else legal.data_ptr(),
                            0 if legal is None else legal.stride(0), actions.data_ptr(),
                            actions.stride(0))
-    a.dtype, a.n_heads = capi.DTYPES[logits.dtype], len(heads)
-    a.width[:len(heads)] = heads
-    a.grad_scale = 1.0
-    return a, (logits, actions, legal)
+    a.dtype, a.n_heads, a.grad_scale = code, nh, 1.0
+    a.width[:nh] = heads
+    return a, n, v, stream, (logits, actions, legal)
+
+
+def _row_values(t, n, dev, what):
+    if t.dtype is not _F32:
+        raise TypeError(f"{what} must be float32")
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{what} must be (N,) = {(n,)}, got {tuple(t.shape)}")
+    if t.device != dev:
+        raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+    return t if t.stride(0) == 1 else t.contiguous()
 
 
 def _loss_args(a, n, dev, old_logp, advantage, ref_logp, mask, clip, kl_coef, entropy_coef):
-    keep = []
-    for name, field, t in (("old_logp", "old_logp", old_logp), ("advantage", "adv", advantage),
-                           ("ref_logp", "ref_logp", ref_logp)):
-        if t is None and name == "ref_logp":
-            capi.need(kl_coef == 0, "a KL term needs ref_logp")
-            continue
-        capi.need(t.dtype == torch.float32, f"{name} must be float32", TypeError)
-        capi.need(t.shape == (n,), f"{name} must be (N,) = {(n,)}, got {tuple(t.shape)}")
-        t = t.contiguous()
-        setattr(a, field, t.data_ptr())
-        keep.append(t)
+    """Fills in the loss's arguments; returns the tensors they point into."""
+    old_logp = _row_values(old_logp, n, dev, "old_logp")
+    advantage = _row_values(advantage, n, dev, "advantage")
+    a.old_logp, a.adv = old_logp.data_ptr(), advantage.data_ptr()
+    if ref_logp is not None:
+        ref_logp = _row_values(ref_logp, n, dev, "ref_logp")
+        a.ref_logp = ref_logp.data_ptr()
+    elif kl_coef != 0:
+        raise ValueError("a KL term needs ref_logp")
     if mask is not None:
-        capi.need(mask.dtype in (torch.bool, torch.uint8), "mask must be bool or uint8", TypeError)
-        capi.need(mask.shape == (n,), f"mask must be (N,) = {(n,)}, got {tuple(mask.shape)}")
-        mask = _bytes(mask).contiguous()
+        if mask.dtype not in _FLAGS:
+            raise TypeError("mask must be bool or uint8")
+        if mask.dim() != 1 or mask.shape[0] != n:
+            raise ValueError(f"mask must be (N,) = {(n,)}, got {tuple(mask.shape)}")
+        if mask.device != dev:
+            raise ValueError(f"tensors on different devices: {dev} and {mask.device}")
+        mask = mask if mask.stride(0) == 1 else mask.contiguous()
         a.mask = mask.data_ptr()
-        keep.append(mask)
     lo, hi = clip if isinstance(clip, (tuple, list)) else (clip, clip)
-    capi.need(0 <= lo <= 1 and hi >= 0, f"clip must be in [0, 1] below and not negative above: {clip}")
+    if not (0 <= lo <= 1 and hi >= 0):
+        raise ValueError(f"clip must be in [0, 1] below and not negative above: {clip}")
     a.clip_low, a.clip_high, a.kl_coef, a.entropy_coef = lo, hi, kl_coef, entropy_coef
-    for t in keep:
-        capi.need(t.device == dev, f"tensors on different devices: {dev} and {t.device}")
-    work = torch.empty(int(capi.lib().qqt_policy_loss_work_bytes(n)), dtype=torch.uint8, device=dev)
+    work = torch.empty(capi.lib().qqt_policy_loss_work_bytes(n), dtype=torch.uint8, device=dev)
     a.work = work.data_ptr()
-    return keep + [work]
+    return old_logp, advantage, ref_logp, mask, work
 
 
-def _launch(a, dev):
-    capi.check(capi.lib().qqt_policy_loss(a, capi.stream_ptr(dev)), "qqt_policy_loss")
+def _launch(a, stream):
+    rc = capi.lib().qqt_policy_loss(a, stream)
+    if rc:
+        capi.check(rc, "qqt_policy_loss")
 
 
 def policy_logp(logits: torch.Tensor, actions: torch.Tensor, legal: torch.Tensor | None = None,
                 heads=None):
     """(logp, entropy), float32 (N,), of `actions` (N,) or (N, heads) int64
     under the masked heads; not differentiable."""
-    a, keep = _args(logits, actions, legal, heads)
-    logp, ent = torch.empty((2, logits.shape[0]), dtype=torch.float32, device=logits.device)
+    a, n, _, stream, keep = _args(logits, actions, legal, heads)
+    logp = torch.empty(n, dtype=_F32, device=logits.device)
+    ent = torch.empty(n, dtype=_F32, device=logits.device)
     a.logp, a.entropy = logp.data_ptr(), ent.data_ptr()
-    _launch(a, logits.device)
+    _launch(a, stream)
     return logp, ent
 
 
@@ -118,18 +137,17 @@ def policy_loss_and_grad(logits: torch.Tensor, actions: torch.Tensor, old_logp: 
     (N,); dlogits (N, V) of the logits' type = grad_scale * dloss/dlogits
     (grad_scale: the loss scaling of float16 training).  clip: one width or
     (below, above)."""
-    a, keep = _args(logits, actions, legal, heads)
-    n, v = logits.shape
+    a, n, v, stream, keep = _args(logits, actions, legal, heads)
     dev = logits.device
     keep = keep, _loss_args(a, n, dev, old_logp, advantage, ref_logp, mask, clip, kl_coef,
                             entropy_coef)
-    logp = torch.empty(n, dtype=torch.float32, device=dev)
-    stats = torch.empty(5, dtype=torch.float32, device=dev)
+    logp = torch.empty(n, dtype=_F32, device=dev)
+    stats = torch.empty(5, dtype=_F32, device=dev)
     dz = torch.empty((n, v), dtype=logits.dtype, device=dev)
     a.logp, a.stats, a.dlogits, a.dlogits_stride = (logp.data_ptr(), stats.data_ptr(),
                                                     dz.data_ptr(), v)
     a.grad_scale = grad_scale
-    _launch(a, dev)
+    _launch(a, stream)
     return stats, logp, dz
 
 
@@ -137,13 +155,13 @@ class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, actions, old_logp, advantage, ref_logp, legal, mask, opts):
         heads, clip, kl_coef, entropy_coef = opts
-        a, keep = _args(logits, actions, legal, heads)
+        a, n, v, stream, keep = _args(logits, actions, legal, heads)
         dev = logits.device
-        keep = keep, _loss_args(a, logits.shape[0], dev, old_logp, advantage, ref_logp, mask, clip,
+        keep = keep, _loss_args(a, n, dev, old_logp, advantage, ref_logp, mask, clip,
                                 kl_coef, entropy_coef)
-        stats = torch.empty(5, dtype=torch.float32, device=dev)
+        stats = torch.empty(5, dtype=_F32, device=dev)
         a.stats = stats.data_ptr()
-        _launch(a, dev)
+        _launch(a, stream)
         ctx.save_for_backward(logits, actions, old_logp, advantage, ref_logp, legal, mask)
         ctx.opts = opts
         # two outputs, no shared storage: the loss carries the gradient, the
@@ -156,14 +174,14 @@ class _PolicyLoss(torch.autograd.Function):
     def backward(ctx, dloss, _):
         logits, actions, old_logp, advantage, ref_logp, legal, mask = ctx.saved_tensors
         heads, clip, kl_coef, entropy_coef = ctx.opts
-        a, keep = _args(logits, actions, legal, heads)
+        a, n, v, stream, keep = _args(logits, actions, legal, heads)
         dev = logits.device
-        keep = keep, _loss_args(a, logits.shape[0], dev, old_logp, advantage, ref_logp, mask, clip,
+        keep = keep, _loss_args(a, n, dev, old_logp, advantage, ref_logp, mask, clip,
                                 kl_coef, entropy_coef)
         up = dloss.to(torch.float32).contiguous()
         dz = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-        a.upstream, a.dlogits, a.dlogits_stride = up.data_ptr(), dz.data_ptr(), logits.shape[1]
-        _launch(a, dev)
+        a.upstream, a.dlogits, a.dlogits_stride = up.data_ptr(), dz.data_ptr(), v
+        _launch(a, stream)
         return dz, None, None, None, None, None, None, None
 
 

@@ -24,6 +24,10 @@ import torch
 from . import _capi as capi
 
 
+_F32 = torch.float32
+_FLAGS = (torch.bool, torch.uint8)
+
+
 def _unit(t: torch.Tensor) -> torch.Tensor:
     return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
@@ -41,28 +45,39 @@ def _like(x: torch.Tensor) -> torch.Tensor:
     return torch.empty((t, n, d), dtype=x.dtype, device=x.device)
 
 
-def _check(x, gate, h0, reset):
-    capi.need(x.dtype in capi.DTYPES, f"x must be float32, float16 or bfloat16, got {x.dtype}",
-              TypeError)
-    capi.need(gate.dtype == x.dtype, "gate must have x's type", TypeError)
-    capi.need(x.dim() == 3 and x.shape[2] > 0 and gate.shape == x.shape,
-              f"x and gate must be (T, N, D) alike, got {tuple(x.shape)} and {tuple(gate.shape)}")
-    _check_state(h0, x.shape[1:], "h0")
+def _check(x, gate, state, reset, dims, what) -> int:
+    """The element type's code; raises on arguments that do not go together.
+    dims: x's dimensions (3, or 2 for one tick)."""
+    code = capi.DTYPES.get(x.dtype)
+    if code is None:
+        raise TypeError(f"x must be float32, float16 or bfloat16, got {x.dtype}")
+    if gate.dtype is not x.dtype:
+        raise TypeError("gate must have x's type")
+    shape = x.shape
+    if len(shape) != dims or shape[-1] == 0 or gate.shape != shape:
+        raise ValueError(f"x and gate must be {'(T, N, D)' if dims == 3 else '(N, D)'} alike, got "
+                         f"{tuple(shape)} and {tuple(gate.shape)}")
+    if state is not None:
+        if state.dtype is not _F32:
+            raise TypeError(f"{what} must be float32")
+        if state.shape != shape[-2:]:
+            raise ValueError(f"{what} must be (N, D) = {tuple(shape[-2:])}, got "
+                             f"{tuple(state.shape)}")
     if reset is not None:
-        capi.need(reset.dtype in (torch.bool, torch.uint8), "reset must be bool or uint8",
-                  TypeError)
-        capi.need(reset.shape == x.shape[:2],
-                  f"reset must be (T, N) = {tuple(x.shape[:2])}, got {tuple(reset.shape)}")
-
-
-def _check_state(s, shape, what):
-    if s is not None:
-        capi.need(s.dtype == torch.float32, f"{what} must be float32", TypeError)
-        capi.need(s.shape == shape, f"{what} must be (N, D) = {tuple(shape)}, got {tuple(s.shape)}")
+        if reset.dtype not in _FLAGS:
+            raise TypeError("reset must be bool or uint8")
+        if reset.shape != shape[:-1]:
+            raise ValueError(f"reset must be {tuple(shape[:-1])}, got {tuple(reset.shape)}")
+    return code
 
 
 def _work(L, t, n, d, dev):
-    return torch.empty(int(L.qqt_recurrence_work_bytes(t, n, d)), dtype=torch.uint8, device=dev)
+    """(tensor, address) of the workspace, (None, None) where none is needed."""
+    nb = L.qqt_recurrence_work_bytes(t, n, d)
+    if nb == 0:
+        return None, None
+    w = torch.empty(nb, dtype=torch.uint8, device=dev)
+    return w, w.data_ptr()
 
 
 def gated_recurrence_forward(x: torch.Tensor, gate: torch.Tensor, h0: torch.Tensor | None = None,
@@ -71,23 +86,23 @@ def gated_recurrence_forward(x: torch.Tensor, gate: torch.Tensor, h0: torch.Tens
     float32, saved (chunks, N, D) float32 for `gated_recurrence_backward`
     (None with save=False).  h0 None is zero; reset (T, N) drops the state
     that would enter a tick."""
-    _check(x, gate, h0, reset)
-    capi.need_cuda(x, gate, h0, reset)
+    code = _check(x, gate, h0, reset, 3, "h0")
+    stream = capi.launch_stream(x, gate, h0, reset)
     t, n, d = x.shape
     dev, L = x.device, capi.lib()
     x, gate = _unit(x), _unit(gate)
     h0 = None if h0 is None else h0.contiguous()
     h = _like(x)
-    last = torch.empty((n, d), dtype=torch.float32, device=dev)
+    last = torch.empty((n, d), dtype=_F32, device=dev)
     saved = None
     if save:
-        saved = torch.empty((int(L.qqt_recurrence_chunks(t)), n, d), dtype=torch.float32,
-                            device=dev)
-    work = _work(L, t, n, d, dev)
-    capi.check(L.qqt_recurrence_forward(
-        _seq(x), _seq(gate), _seq(reset), capi.ptr(h0), capi.DTYPES[x.dtype], t, n, d, _seq(h),
-        last.data_ptr(), capi.ptr(saved), work.data_ptr(), capi.stream_ptr(dev)),
-        "qqt_recurrence_forward")
+        saved = torch.empty((L.qqt_recurrence_chunks(t), n, d), dtype=_F32, device=dev)
+    work, wp = _work(L, t, n, d, dev)
+    rc = L.qqt_recurrence_forward(
+        _seq(x), _seq(gate), _seq(reset), capi.ptr(h0), code, t, n, d, _seq(h), last.data_ptr(),
+        capi.ptr(saved), wp, stream)
+    if rc:
+        capi.check(rc, "qqt_recurrence_forward")
     return h, last, saved
 
 
@@ -96,27 +111,27 @@ def gated_recurrence_backward(dh: torch.Tensor | None, dh_last: torch.Tensor | N
                               reset: torch.Tensor | None = None):
     """(dx, dgate, dh0) for dL/dh = dh and dL/dh_last = dh_last (either may be
     None, zero); saved is the forward pass's."""
-    _check(x, gate, None, reset)
+    code = _check(x, gate, dh_last, reset, 3, "dh_last")
     t, n, d = x.shape
-    _check_state(dh_last, x.shape[1:], "dh_last")
-    capi.need(dh is None or (dh.shape == x.shape and dh.dtype == x.dtype),
-              "dh must have x's shape and type")
+    if dh is not None and (dh.shape != x.shape or dh.dtype is not x.dtype):
+        raise ValueError("dh must have x's shape and type")
     L = capi.lib()
-    capi.need(saved is not None and saved.dtype == torch.float32 and saved.is_contiguous()
-              and saved.shape == (int(L.qqt_recurrence_chunks(t)), n, d),
-              "saved must be the forward pass's")
-    capi.need_cuda(x, gate, saved, dh, dh_last, reset)
+    if saved is None or saved.dtype is not _F32 or not saved.is_contiguous() \
+            or saved.shape != (L.qqt_recurrence_chunks(t), n, d):
+        raise ValueError("saved must be the forward pass's")
+    stream = capi.launch_stream(x, gate, saved, dh, dh_last, reset)
     dev = x.device
     x, gate = _unit(x), _unit(gate)
     dh = None if dh is None else _unit(dh)
     dh_last = None if dh_last is None else dh_last.contiguous()
     dx, dg = _like(x), _like(x)
-    dh0 = torch.empty((n, d), dtype=torch.float32, device=dev)
-    work = _work(L, t, n, d, dev)
-    capi.check(L.qqt_recurrence_backward(
-        _seq(dh), capi.ptr(dh_last), _seq(x), _seq(gate), _seq(reset), saved.data_ptr(),
-        capi.DTYPES[x.dtype], t, n, d, _seq(dx), _seq(dg), dh0.data_ptr(), work.data_ptr(),
-        capi.stream_ptr(dev)), "qqt_recurrence_backward")
+    dh0 = torch.empty((n, d), dtype=_F32, device=dev)
+    work, wp = _work(L, t, n, d, dev)
+    rc = L.qqt_recurrence_backward(
+        _seq(dh), capi.ptr(dh_last), _seq(x), _seq(gate), _seq(reset), saved.data_ptr(), code, t, n,
+        d, _seq(dx), _seq(dg), dh0.data_ptr(), wp, stream)
+    if rc:
+        capi.check(rc, "qqt_recurrence_backward")
     return dx, dg, dh0
 
 
@@ -152,21 +167,25 @@ def gated_recurrence_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tens
     """One tick: (h, new state) for x, gate (N, D), state (N, D) float32 and
     reset (N,).  state_out receives the new state (it may be `state` itself:
     the rollout's in-place form); by default it is a new tensor."""
-    capi.need(x.dim() == 2, f"x must be (N, D), got {tuple(x.shape)}")
-    x3, g3 = x[None], gate[None]
-    r2 = None if reset is None else reset[None]
-    _check(x3, g3, state, r2)
-    capi.need(state is not None and state.is_contiguous(), "state must be contiguous")
-    _check_state(state_out, x.shape, "state_out")
-    capi.need(state_out is None or state_out.is_contiguous(), "state_out must be contiguous")
-    capi.need_cuda(x, gate, state, reset, state_out)
+    code = _check(x, gate, state, reset, 2, "state")
+    if state is None or not state.is_contiguous():
+        raise ValueError("state must be contiguous")
+    if state_out is None:
+        out = torch.empty_like(state)
+    elif state_out.dtype is not _F32:
+        raise TypeError("state_out must be float32")
+    elif state_out.shape != state.shape or not state_out.is_contiguous():
+        raise ValueError(f"state_out must be a contiguous {tuple(state.shape)}")
+    else:
+        out = state_out
+    stream = capi.launch_stream(x, gate, state, reset, out)
     n, d = x.shape
-    dev, L = x.device, capi.lib()
-    x3, g3 = _unit(x3), _unit(g3)
-    h = torch.empty((1, n, d), dtype=x.dtype, device=dev)
-    out = torch.empty_like(state) if state_out is None else state_out
-    work = _work(L, 1, n, d, dev)
-    capi.check(L.qqt_recurrence_forward(
-        _seq(x3), _seq(g3), _seq(r2), state.data_ptr(), capi.DTYPES[x.dtype], 1, n, d, _seq(h),
-        out.data_ptr(), None, work.data_ptr(), capi.stream_ptr(dev)), "qqt_recurrence_forward")
-    return h[0], out
+    x, gate = _unit(x), _unit(gate)
+    h = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    rc = capi.lib().qqt_recurrence_step(
+        x.data_ptr(), x.stride(0), gate.data_ptr(), gate.stride(0),
+        None if reset is None else reset.data_ptr(), 0 if reset is None else reset.stride(0),
+        state.data_ptr(), code, n, d, h.data_ptr(), out.data_ptr(), stream)
+    if rc:
+        capi.check(rc, "qqt_recurrence_step")
+    return h, out
