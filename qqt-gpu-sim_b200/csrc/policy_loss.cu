@@ -46,6 +46,15 @@ struct HeadStat {
   int act;                  // the action, -1 where it is none of the head's
 };
 
+// The counting, the row and the summing kernel overlap: each is launched while
+// the one before still runs, and waits for it where it needs its results.
+__device__ __forceinline__ void wait_for_counts() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void let_next_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // Rows of the mask, at least 1; `counts`: the counting blocks' results.
 __device__ __forceinline__ float rows_counted(const QqtPolicyLoss& a, const int* counts) {
   if (!a.mask) return fmaxf((float)a.rows, 1.f);
@@ -75,6 +84,7 @@ __device__ __forceinline__ int count_bytes(const uint8_t* mask, int64_t first, i
 __global__ void __launch_bounds__(512) k_pl_count(const uint8_t* __restrict__ mask, int64_t rows,
                                                   int* __restrict__ counts) {
   __shared__ int buf[16];
+  let_next_start();
   int n = count_bytes(mask, (int64_t)blockIdx.x * 512 + threadIdx.x, (int64_t)gridDim.x * 512, rows);
   n = warp_sum(n);
   if (lane_id() == 0) buf[warp_id()] = n;
@@ -146,59 +156,130 @@ __device__ __forceinline__ float action_grad(const HeadStat& k, float g, float c
 
 // ---------------------------------------------------- few logits: thread per row
 
+// Copies n elements from p to floats, or floats to p, by 16-byte vectors; p on
+// 16 bytes.
 template <class T>
+__device__ __forceinline__ void stage_in(const T* p, int n, float* to) {
+  constexpr int VEC = 16 / sizeof(T);
+  for (int i = threadIdx.x * VEC; i + VEC <= n; i += kPlSmallRows * VEC) {
+    const Vec<T, VEC> x = ld_vec<T, VEC>(p + i);
+#pragma unroll
+    for (int v = 0; v < VEC; v += 4)
+      *reinterpret_cast<float4*>(to + i + v) =
+          make_float4(x.get(v), x.get(v + 1), x.get(v + 2), x.get(v + 3));
+  }
+  const int i = n / VEC * VEC + threadIdx.x;
+  if (i < n) to[i] = to_f(p[i]);
+}
+template <class T>
+__device__ __forceinline__ void stage_out(T* p, int n, const float* from) {
+  constexpr int VEC = 16 / sizeof(T);
+  for (int i = threadIdx.x * VEC; i + VEC <= n; i += kPlSmallRows * VEC) {
+    float f[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) f[v] = from[i + v];
+    Vec<T, VEC> x;
+    x.put(f);
+    st_vec(p + i, x);
+  }
+  const int i = n / VEC * VEC + threadIdx.x;
+  if (i < n) p[i] = from_f<T>(from[i]);
+}
+
+// Rows are V | 1 floats apart in shared memory: threads on rows hit different
+// banks.  Where V is odd and the rows lie one after the other, the block's
+// rows are one run of memory that is copied as it is.
+// NH: the number of heads where it is 1 or 2 (what is kept per head then stays
+// in registers), QQT_MAX_HEADS for any.
+template <class T, int NH>
 __global__ void __launch_bounds__(kPlSmallRows)
     k_pl_small(QqtPolicyLoss a, int V, const int* __restrict__ counts, float* __restrict__ part,
                int one_block) {
-  extern __shared__ float zs[];          // [rows][pitch]
-  __shared__ float buf[32];
+  extern __shared__ __align__(16) float zs[];
+  __shared__ float buf[4][32];
   __shared__ int n_mask;
-  const int pitch = V | 1;               // odd: threads on rows hit different banks
+  const int pitch = V | 1;
   const int64_t r0 = (int64_t)blockIdx.x * kPlSmallRows;
   const int n = a.rows - r0 < kPlSmallRows ? (int)(a.rows - r0) : kPlSmallRows;
   const bool loss = a.old_logp != nullptr;
   const bool fold = loss && a.mask && !counts;
+  const bool on = threadIdx.x < n;
+  const int64_t r = r0 + threadIdx.x;
+  RowIn row{0.f, 0.f, 0.f, true};
+  if (loss && on) {
+    row.old = a.old_logp[r];
+    row.adv = a.adv[r];
+    if (a.ref_logp) row.ref = a.ref_logp[r];
+    if (a.mask) row.counts = a.mask[r] != 0;
+  }
   int mine = 0;
   if (fold) {
     if (threadIdx.x == 0) n_mask = 0;
     mine = warp_sum(count_bytes(a.mask, threadIdx.x, kPlSmallRows, a.rows));
   }
-  {
-    int row = threadIdx.x / V, col = threadIdx.x % V;
+  const T* zp = (const T*)a.logits + r0 * a.row_stride;
+  uint8_t* legal = (uint8_t*)(zs + kPlSmallRows * pitch);
+  if ((V & 1) && a.row_stride == V && ((uintptr_t)zp & 15) == 0) {
+    stage_in(zp, n * V, zs);
+  } else {
+    int q = threadIdx.x / V, col = threadIdx.x % V;
     const int dr = kPlSmallRows / V, dc = kPlSmallRows % V;
 #pragma unroll 4
     for (int i = threadIdx.x; i < n * V; i += kPlSmallRows) {
-      float z = to_f(((const T*)a.logits)[(r0 + row) * a.row_stride + col]);
-      if (a.legal && !a.legal[(r0 + row) * a.legal_stride + col]) z = -INFINITY;
-      zs[row * pitch + col] = z;
-      row += dr;
+      zs[q * pitch + col] = to_f(zp[q * a.row_stride + col]);
+      q += dr;
       col += dc;
       if (col >= V) {
         col -= V;
-        ++row;
+        ++q;
+      }
+    }
+  }
+  if (a.legal) {
+    const uint8_t* lp = a.legal + r0 * a.legal_stride;
+    if (a.legal_stride == V && ((uintptr_t)lp & 15) == 0) {
+      for (int i = threadIdx.x * 16; i + 16 <= n * V; i += kPlSmallRows * 16)
+        *reinterpret_cast<uint4*>(legal + i) = *reinterpret_cast<const uint4*>(lp + i);
+      const int i = n * V / 16 * 16 + threadIdx.x;
+      if (i < n * V) legal[i] = lp[i];
+    } else {
+      int q = threadIdx.x / V, col = threadIdx.x % V;
+      const int dr = kPlSmallRows / V, dc = kPlSmallRows % V;
+#pragma unroll 4
+      for (int i = threadIdx.x; i < n * V; i += kPlSmallRows) {
+        legal[i] = lp[q * a.legal_stride + col];
+        q += dr;
+        col += dc;
+        if (col >= V) {
+          col -= V;
+          ++q;
+        }
       }
     }
   }
   __syncthreads();
   if (fold && lane_id() == 0 && mine) atomicAdd(&n_mask, mine);   // whole numbers: any order
-  const bool on = threadIdx.x < n;
-  const int64_t r = r0 + threadIdx.x;
   float* z = zs + threadIdx.x * pitch;
-  HeadStat hs[QQT_MAX_HEADS];
-  float ms[QQT_MAX_HEADS];
+  const uint8_t* lg = legal + threadIdx.x * V;
+  HeadStat hs[NH];
+  float ms[NH];
   float logp = 0.f, ent = 0.f;
   if (on) {
     int at = 0;
-#pragma unroll 1
-    for (int h = 0; h < a.n_heads; ++h) {
+#pragma unroll(NH <= 2 ? NH : 1)
+    for (int h = 0; h < (NH <= 2 ? NH : a.n_heads); ++h) {
       const int w = a.width[h];
       const int64_t act = a.actions[r * a.action_stride + h];
       const bool in = act >= 0 && act < w;
       if (!in) flag_error(QQT_DEV_BAD_ACTION);
       float m = -INFINITY, s = 0.f, e = 0.f;
-      for (int j = 0; j < w; ++j) m = max_nan(m, z[at + j]);
-      for (int j = 0; j < w; ++j) {
-        const float t = max_nan(z[at + j] - m, kFloor), x = expf(t);
+      for (int j = at; j < at + w; ++j) {
+        if (a.legal && !lg[j]) z[j] = -INFINITY;
+        m = max_nan(m, z[j]);
+      }
+#pragma unroll 4
+      for (int j = at; j < at + w; ++j) {
+        const float t = max_nan(z[j] - m, kFloor), x = ex2_approx(t * kLog2e);
         s += x;
         e = fmaf(x, t, e);
       }
@@ -217,31 +298,34 @@ __global__ void __launch_bounds__(kPlSmallRows)
   }
   if (!loss) return;
   if (fold) __syncthreads();
+  wait_for_counts();
   const float count = fold ? fmaxf((float)n_mask, 1.f) : rows_counted(a, counts);
-  RowIn row{0.f, 0.f, 0.f, true};
-  if (on) {
-    row.old = a.old_logp[r];
-    row.adv = a.adv[r];
-    if (a.ref_logp) row.ref = a.ref_logp[r];
-    if (a.mask) row.counts = a.mask[r] != 0;
-  }
   const bool live = on && logp != -INFINITY && row.counts;
   const RowLoss l = loss_of(a, row, logp, live);
   if (a.stats) {
     const float v[4] = {l.pg, l.kl, live ? ent : 0.f, l.clip};
-    float sum[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) sum[k] = block_sum(v[k], buf);
-    if (threadIdx.x == 0) {
-      if (one_block) {
+    for (int k = 0; k < 4; ++k) {
+      const float x = warp_sum_f(v[k]);
+      if (lane_id() == 0) buf[k][warp_id()] = x;
+    }
+    __syncthreads();
+    if (warp_id() == 0) {
+      float sum[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) sum[k] /= count;
-        a.stats[0] = sum[0] + a.kl_coef * sum[1] - a.entropy_coef * sum[2];
+      for (int k = 0; k < 4; ++k)
+        sum[k] = warp_sum_f(lane_id() < kPlSmallRows / 32 ? buf[k][lane_id()] : 0.f);
+      if (lane_id() == 0) {
+        if (one_block) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) a.stats[1 + k] = sum[k];
-      } else {
+          for (int k = 0; k < 4; ++k) sum[k] /= count;
+          a.stats[0] = sum[0] + a.kl_coef * sum[1] - a.entropy_coef * sum[2];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) part[blockIdx.x * 4 + k] = sum[k];
+          for (int k = 0; k < 4; ++k) a.stats[1 + k] = sum[k];
+        } else {
+          *reinterpret_cast<float4*>(part + (int64_t)blockIdx.x * 4) =
+              make_float4(sum[0], sum[1], sum[2], sum[3]);
+        }
       }
     }
   }
@@ -249,31 +333,35 @@ __global__ void __launch_bounds__(kPlSmallRows)
   const float scale = a.grad_scale / count * (a.upstream ? a.upstream[0] : 1.f);
   if (on) {
     int at = 0;
-#pragma unroll 1
-    for (int h = 0; h < a.n_heads; ++h) {
+#pragma unroll(NH <= 2 ? NH : 1)
+    for (int h = 0; h < (NH <= 2 ? NH : a.n_heads); ++h) {
       const int w = a.width[h];
       const HeadStat k = hs[h];
       const float m = ms[h], cs = head_c(k, a.entropy_coef), ks = head_k(k, l.g, a.entropy_coef);
-      for (int j = 0; j < w; ++j) {
-        const float t = max_nan(z[at + j] - m, kFloor);
-        z[at + j] = live ? expf(t) * fmaf(cs, t, ks) * scale : 0.f;
+#pragma unroll 4
+      for (int j = at; j < at + w; ++j) {
+        const float t = max_nan(z[j] - m, kFloor);
+        z[j] = live ? ex2_approx(t * kLog2e) * fmaf(cs, t, ks) * scale : 0.f;
       }
       if (live) z[k.act] = action_grad(k, l.g, a.entropy_coef, scale);
       at += w;
     }
   }
   __syncthreads();
-  {
-    int row = threadIdx.x / V, col = threadIdx.x % V;
+  T* op = (T*)a.dlogits + r0 * a.dlogits_stride;
+  if ((V & 1) && a.dlogits_stride == V && ((uintptr_t)op & 15) == 0) {
+    stage_out(op, n * V, zs);
+  } else {
+    int q = threadIdx.x / V, col = threadIdx.x % V;
     const int dr = kPlSmallRows / V, dc = kPlSmallRows % V;
 #pragma unroll 4
     for (int i = threadIdx.x; i < n * V; i += kPlSmallRows) {
-      ((T*)a.dlogits)[(r0 + row) * a.dlogits_stride + col] = from_f<T>(zs[row * pitch + col]);
-      row += dr;
+      op[q * a.dlogits_stride + col] = from_f<T>(zs[q * pitch + col]);
+      q += dr;
       col += dc;
       if (col >= V) {
         col -= V;
-        ++row;
+        ++q;
       }
     }
   }
@@ -651,13 +739,12 @@ __global__ void __launch_bounds__(kPlThreads, kPlThreads == 512 ? 2 : 1)
   RowIn in{0.f, 0.f, 0.f, true};
   int n_counted = 0;
   if (a.old_logp) {
+    wait_for_counts();
+    if (a.mask) n_counted = counts[lane_id()] + counts[lane_id() + 32];
     in.old = a.old_logp[r];
     in.adv = a.adv[r];
     if (a.ref_logp) in.ref = a.ref_logp[r];
-    if (a.mask) {
-      in.counts = a.mask[r] != 0;
-      n_counted = counts[lane_id()] + counts[lane_id() + 32];
-    }
+    if (a.mask) in.counts = a.mask[r] != 0;
   }
   const T* z = (const T*)a.logits + r * a.row_stride;
   const uint8_t* legal = LEGAL ? a.legal + r * a.legal_stride : nullptr;
@@ -826,8 +913,9 @@ __global__ void __launch_bounds__(kPlThreads, kPlThreads == 512 ? 2 : 1)
 __global__ void __launch_bounds__(1024)
     k_pl_stats(QqtPolicyLoss a, const float* __restrict__ part, int64_t n,
                const int* __restrict__ counts) {
-  __shared__ float buf[32];
+  __shared__ float buf[4][32];
   float s[4] = {0.f, 0.f, 0.f, 0.f};
+  wait_for_counts();
 #pragma unroll 4
   for (int64_t r = threadIdx.x; r < n; r += 1024) {
     const float4 v = *reinterpret_cast<const float4*>(part + r * 4);
@@ -836,10 +924,17 @@ __global__ void __launch_bounds__(1024)
     s[2] += v.z;
     s[3] += v.w;
   }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    s[k] = warp_sum_f(s[k]);
+    if (lane_id() == 0) buf[k][warp_id()] = s[k];
+  }
+  __syncthreads();
+  if (warp_id() > 0) return;
   const float count = rows_counted(a, counts);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) s[k] = block_sum(s[k], buf) / count;
-  if (threadIdx.x == 0) {
+  for (int k = 0; k < 4; ++k) s[k] = warp_sum_f(buf[k][lane_id()]) / count;
+  if (lane_id() == 0) {
     a.stats[0] = s[0] + a.kl_coef * s[1] - a.entropy_coef * s[2];
 #pragma unroll
     for (int k = 0; k < 4; ++k) a.stats[1 + k] = s[k];
@@ -849,6 +944,24 @@ __global__ void __launch_bounds__(1024)
 }  // namespace qqt
 
 using namespace qqt;
+
+// early: the kernel before it in the stream is one of this call's, and this one
+// may start while that one still runs.
+template <class... P, class... A>
+static void pl_launch(void (*kernel)(P...), unsigned blocks, unsigned threads, size_t smem,
+                      cudaStream_t st, bool early, A... args) {
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = blocks;
+  cfg.blockDim = threads;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = early ? 1 : 0;
+  (void)cudaLaunchKernelEx(&cfg, kernel, P(args)...);   // (launch_status reports a failure)
+}
 
 // 64 counts, then four partial sums a row (or a block of rows).
 extern "C" uint64_t qqt_policy_loss_work_bytes(int64_t rows) {
@@ -885,8 +998,17 @@ extern "C" int qqt_policy_loss(const QqtPolicyLoss* a, qqt_stream_t stream) {
     with_dtype(a->dtype, [&](auto t) {
       using T = decltype(t);
       if (small) {
-        const size_t smem = (size_t)kPlSmallRows * (v | 1) * 4;
-        k_pl_small<T><<<(unsigned)blocks, kPlSmallRows, smem, st>>>(args, (int)v, counts, part, one);
+        const size_t smem = (size_t)kPlSmallRows * ((v | 1) * 4 + (a->legal ? v : 0));
+        auto run = [&](auto nh) {
+          pl_launch(k_pl_small<T, decltype(nh)::value>, (unsigned)blocks, kPlSmallRows, smem, st,
+                    counts != nullptr, args, (int)v, counts, part, (int)one);
+        };
+        if (a->n_heads == 1)
+          run(std::integral_constant<int, 1>{});
+        else if (a->n_heads == 2)
+          run(std::integral_constant<int, 2>{});
+        else
+          run(std::integral_constant<int, QQT_MAX_HEADS>{});
         return 0;
       }
       // a team of 8 lanes holds rows of up to 32 vectors in one step, a warp
@@ -903,9 +1025,9 @@ extern "C" int qqt_policy_loss(const QqtPolicyLoss* a, qqt_stream_t stream) {
       auto run = [&](auto gg) {
         constexpr int G = decltype(gg)::value;
         if (a->legal)
-          k_pl_rows<T, G, true><<<n, threads, 0, st>>>(args, counts, part);
+          pl_launch(k_pl_rows<T, G, true>, n, threads, 0, st, counts != nullptr, args, counts, part);
         else
-          k_pl_rows<T, G, false><<<n, threads, 0, st>>>(args, counts, part);
+          pl_launch(k_pl_rows<T, G, false>, n, threads, 0, st, counts != nullptr, args, counts, part);
       };
       if (g == 8)
         run(std::integral_constant<int, 8>{});
@@ -916,6 +1038,6 @@ extern "C" int qqt_policy_loss(const QqtPolicyLoss* a, qqt_stream_t stream) {
       return 0;
     });
   if (a->stats && !one)
-    k_pl_stats<<<1, 1024, 0, st>>>(args, part, small ? blocks : a->rows, counts);
+    pl_launch(k_pl_stats, 1, 1024, 0, st, a->rows > 0, args, part, small ? blocks : a->rows, counts);
   return launch_status();
 }
