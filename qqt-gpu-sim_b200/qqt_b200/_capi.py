@@ -160,11 +160,11 @@ def lib():
             "qqt_layernorm_backward": (c_i32, [c_p, c_i64, c_p, c_i64, c_i32, c_i64, c_i64, c_p,
                                                c_p, c_p, c_p, c_p, c_p, c_p, c_p]),
             "qqt_layernorm_work_bytes": (c_u64, [c_i64, c_i64]),
-            "qqt_recurrence_forward": (c_i32, [P(QqtSeq), P(QqtSeq), P(QqtSeq), c_p, c_i32, c_i64,
-                                               c_i64, c_i64, P(QqtSeq), c_p, c_p, c_p, c_p]),
-            "qqt_recurrence_backward": (c_i32, [P(QqtSeq), c_p, P(QqtSeq), P(QqtSeq), P(QqtSeq),
-                                                c_p, c_i32, c_i64, c_i64, c_i64, P(QqtSeq),
-                                                P(QqtSeq), c_p, c_p, c_p]),
+            # (QqtSeq operands by address: several may lie in one array)
+            "qqt_recurrence_forward": (c_i32, [c_p, c_p, c_p, c_p, c_i32, c_i64, c_i64, c_i64, c_p,
+                                               c_p, c_p, c_p, c_p]),
+            "qqt_recurrence_backward": (c_i32, [c_p, c_p, c_p, c_p, c_p, c_p, c_i32, c_i64, c_i64,
+                                                c_i64, c_p, c_p, c_p, c_p, c_p]),
             "qqt_recurrence_step": (c_i32, [c_p, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_i32, c_i64,
                                             c_i64, c_p, c_p, c_p]),
             "qqt_recurrence_chunks": (c_i64, [c_i64]),
@@ -225,15 +225,14 @@ DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 def launch_stream(first: torch.Tensor, *others) -> int:
     """The current stream's handle, once all given tensors (None allowed) are
     on one CUDA device, the current one (kernels launch there)."""
-    dev = first.device
-    if dev.type != "cuda":
-        raise ValueError(f"tensors must be on a CUDA device, got {dev}")
-    i = dev.index
+    if not first.is_cuda:
+        raise ValueError(f"tensors must be on a CUDA device, got {first.device}")
+    i = first.get_device()
     for t in others:
         if t is not None and t.get_device() != i:
-            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
-    if i != torch.cuda.current_device():
-        raise ValueError(f"tensors on {dev}, but the current device is "
+            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
+    if i != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors on {first.device}, but the current device is "
                          f"cuda:{torch.cuda.current_device()}")
     return torch._C._cuda_getCurrentRawStream(i)
 

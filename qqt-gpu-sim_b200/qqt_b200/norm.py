@@ -56,11 +56,11 @@ def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor
     w = weight.contiguous()
     b = None if bias is None else bias.contiguous()
     n = xr.shape[0]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
     mean = rstd = None
     if stats:
-        mean = torch.empty(n, dtype=_F32, device=x.device)
-        rstd = torch.empty(n, dtype=_F32, device=x.device)
+        mean = w.new_empty(n)
+        rstd = torch.empty_like(mean)
     rc = capi.lib().qqt_layernorm_forward(
         xr.data_ptr(), code, n, d, xr.stride(0), w.data_ptr(), None if b is None else b.data_ptr(),
         eps, y.data_ptr(), None if mean is None else mean.data_ptr(),
@@ -83,14 +83,15 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
         if t.dim() != 1 or t.shape[0] != n or t.dtype is not _F32 or not t.is_contiguous():
             raise ValueError("mean and rstd must be the forward pass's")
     stream = capi.launch_stream(x, dy, mean, rstd, weight)
-    dev, L = x.device, capi.lib()
+    L = capi.lib()
     xr, dyr, w = _rows(x, d), _rows(dy, d), weight.contiguous()
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_dx else None
+    dx = None
+    if need_dx:
+        dx = torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
     dw = db = work = None
     if need_dw:
-        dw = torch.empty(weight.shape, dtype=_F32, device=dev)
-        db = torch.empty(weight.shape, dtype=_F32, device=dev)
-        work = torch.empty(L.qqt_layernorm_work_bytes(n, d), dtype=torch.uint8, device=dev)
+        dw, db = torch.empty_like(w), torch.empty_like(w)
+        work = w.new_empty(L.qqt_layernorm_work_bytes(n, d) // 4)
     rc = L.qqt_layernorm_backward(
         dyr.data_ptr(), dyr.stride(0), xr.data_ptr(), xr.stride(0), code, n, d, mean.data_ptr(),
         rstd.data_ptr(), w.data_ptr(), capi.ptr(dx), capi.ptr(dw), capi.ptr(db), capi.ptr(work),

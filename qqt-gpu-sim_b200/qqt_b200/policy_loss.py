@@ -104,7 +104,7 @@ def _loss_args(a, n, dev, old_logp, advantage, ref_logp, mask, clip, kl_coef, en
     if not (0 <= lo <= 1 and hi >= 0):
         raise ValueError(f"clip must be in [0, 1] below and not negative above: {clip}")
     a.clip_low, a.clip_high, a.kl_coef, a.entropy_coef = lo, hi, kl_coef, entropy_coef
-    work = torch.empty(capi.lib().qqt_policy_loss_work_bytes(n), dtype=torch.uint8, device=dev)
+    work = advantage.new_empty(capi.lib().qqt_policy_loss_work_bytes(n) // 4)
     a.work = work.data_ptr()
     return old_logp, advantage, ref_logp, mask, work
 
@@ -120,8 +120,8 @@ def policy_logp(logits: torch.Tensor, actions: torch.Tensor, legal: torch.Tensor
     """(logp, entropy), float32 (N,), of `actions` (N,) or (N, heads) int64
     under the masked heads; not differentiable."""
     a, n, _, stream, keep = _args(logits, actions, legal, heads)
-    logp = torch.empty(n, dtype=_F32, device=logits.device)
-    ent = torch.empty(n, dtype=_F32, device=logits.device)
+    logp = logits.new_empty(n, dtype=_F32)
+    ent = torch.empty_like(logp)
     a.logp, a.entropy = logp.data_ptr(), ent.data_ptr()
     _launch(a, stream)
     return logp, ent
@@ -141,9 +141,9 @@ def policy_loss_and_grad(logits: torch.Tensor, actions: torch.Tensor, old_logp: 
     dev = logits.device
     keep = keep, _loss_args(a, n, dev, old_logp, advantage, ref_logp, mask, clip, kl_coef,
                             entropy_coef)
-    logp = torch.empty(n, dtype=_F32, device=dev)
-    stats = torch.empty(5, dtype=_F32, device=dev)
-    dz = torch.empty((n, v), dtype=logits.dtype, device=dev)
+    logp = logits.new_empty(n, dtype=_F32)
+    stats = logp.new_empty(5)
+    dz = torch.empty_like(logits) if logits.is_contiguous() else logits.new_empty((n, v))
     a.logp, a.stats, a.dlogits, a.dlogits_stride = (logp.data_ptr(), stats.data_ptr(),
                                                     dz.data_ptr(), v)
     a.grad_scale = grad_scale
@@ -159,7 +159,7 @@ class _PolicyLoss(torch.autograd.Function):
         dev = logits.device
         keep = keep, _loss_args(a, n, dev, old_logp, advantage, ref_logp, mask, clip,
                                 kl_coef, entropy_coef)
-        stats = torch.empty(5, dtype=_F32, device=dev)
+        stats = logits.new_empty(5, dtype=_F32)
         a.stats = stats.data_ptr()
         _launch(a, stream)
         ctx.save_for_backward(logits, actions, old_logp, advantage, ref_logp, legal, mask)
@@ -179,7 +179,7 @@ class _PolicyLoss(torch.autograd.Function):
         keep = keep, _loss_args(a, n, dev, old_logp, advantage, ref_logp, mask, clip,
                                 kl_coef, entropy_coef)
         up = dloss.to(torch.float32).contiguous()
-        dz = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        dz = logits.new_empty((n, v))
         a.upstream, a.dlogits, a.dlogits_stride = up.data_ptr(), dz.data_ptr(), v
         _launch(a, stream)
         return dz, None, None, None, None, None, None, None

@@ -32,17 +32,19 @@ def _unit(t: torch.Tensor) -> torch.Tensor:
     return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
-def _seq(t: torch.Tensor | None):
-    return None if t is None else ctypes.byref(capi.QqtSeq(t.data_ptr(), t.stride(0), t.stride(1)))
-
-
-def _like(x: torch.Tensor) -> torch.Tensor:
-    """An empty (T, N, D) in x's order: batch-first where x's time steps lie
-    closer together than its sequences."""
-    t, n, d = x.shape
-    if t > 1 and n > 1 and x.stride(0) < x.stride(1):
-        return torch.empty((n, t, d), dtype=x.dtype, device=x.device).transpose(0, 1)
-    return torch.empty((t, n, d), dtype=x.dtype, device=x.device)
+def _seqs(*tensors):
+    """The tensors as one array of QqtSeq and its entries' addresses (None for
+    a tensor that is None); the array has to live until the call is done."""
+    v = []
+    for t in tensors:
+        if t is None:
+            v += (0, 0, 0)
+        else:
+            st = t.stride()
+            v += (t.data_ptr(), st[0], st[1])
+    a = (ctypes.c_int64 * len(v))(*v)
+    base = ctypes.addressof(a)
+    return a, [None if t is None else base + 24 * i for i, t in enumerate(tensors)]
 
 
 def _check(x, gate, state, reset, dims, what) -> int:
@@ -71,12 +73,12 @@ def _check(x, gate, state, reset, dims, what) -> int:
     return code
 
 
-def _work(L, t, n, d, dev):
+def _work(L, t, n, d, like):
     """(tensor, address) of the workspace, (None, None) where none is needed."""
     nb = L.qqt_recurrence_work_bytes(t, n, d)
     if nb == 0:
         return None, None
-    w = torch.empty(nb, dtype=torch.uint8, device=dev)
+    w = like.new_empty(nb // 4)
     return w, w.data_ptr()
 
 
@@ -89,18 +91,16 @@ def gated_recurrence_forward(x: torch.Tensor, gate: torch.Tensor, h0: torch.Tens
     code = _check(x, gate, h0, reset, 3, "h0")
     stream = capi.launch_stream(x, gate, h0, reset)
     t, n, d = x.shape
-    dev, L = x.device, capi.lib()
+    L = capi.lib()
     x, gate = _unit(x), _unit(gate)
     h0 = None if h0 is None else h0.contiguous()
-    h = _like(x)
-    last = torch.empty((n, d), dtype=_F32, device=dev)
-    saved = None
-    if save:
-        saved = torch.empty((L.qqt_recurrence_chunks(t), n, d), dtype=_F32, device=dev)
-    work, wp = _work(L, t, n, d, dev)
-    rc = L.qqt_recurrence_forward(
-        _seq(x), _seq(gate), _seq(reset), capi.ptr(h0), code, t, n, d, _seq(h), last.data_ptr(),
-        capi.ptr(saved), wp, stream)
+    h = torch.empty_like(x)                    # (dense, in the order of x's strides)
+    last = x.new_empty((n, d), dtype=_F32)
+    saved = last.new_empty((L.qqt_recurrence_chunks(t), n, d)) if save else None
+    work, wp = _work(L, t, n, d, last)
+    keep, (xs, gs, rs, hs) = _seqs(x, gate, reset, h)
+    rc = L.qqt_recurrence_forward(xs, gs, rs, None if h0 is None else h0.data_ptr(), code, t, n, d,
+                                  hs, last.data_ptr(), capi.ptr(saved), wp, stream)
     if rc:
         capi.check(rc, "qqt_recurrence_forward")
     return h, last, saved
@@ -120,16 +120,15 @@ def gated_recurrence_backward(dh: torch.Tensor | None, dh_last: torch.Tensor | N
             or saved.shape != (L.qqt_recurrence_chunks(t), n, d):
         raise ValueError("saved must be the forward pass's")
     stream = capi.launch_stream(x, gate, saved, dh, dh_last, reset)
-    dev = x.device
     x, gate = _unit(x), _unit(gate)
     dh = None if dh is None else _unit(dh)
     dh_last = None if dh_last is None else dh_last.contiguous()
-    dx, dg = _like(x), _like(x)
-    dh0 = torch.empty((n, d), dtype=_F32, device=dev)
-    work, wp = _work(L, t, n, d, dev)
-    rc = L.qqt_recurrence_backward(
-        _seq(dh), capi.ptr(dh_last), _seq(x), _seq(gate), _seq(reset), saved.data_ptr(), code, t, n,
-        d, _seq(dx), _seq(dg), dh0.data_ptr(), wp, stream)
+    dx, dg = torch.empty_like(x), torch.empty_like(x)
+    dh0 = saved.new_empty((n, d))
+    work, wp = _work(L, t, n, d, saved)
+    keep, (hs, xs, gs, rs, dxs, dgs) = _seqs(dh, x, gate, reset, dx, dg)
+    rc = L.qqt_recurrence_backward(hs, capi.ptr(dh_last), xs, gs, rs, saved.data_ptr(), code, t, n,
+                                   d, dxs, dgs, dh0.data_ptr(), wp, stream)
     if rc:
         capi.check(rc, "qqt_recurrence_backward")
     return dx, dg, dh0
@@ -181,7 +180,7 @@ def gated_recurrence_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tens
     stream = capi.launch_stream(x, gate, state, reset, out)
     n, d = x.shape
     x, gate = _unit(x), _unit(gate)
-    h = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    h = x.new_empty((n, d))
     rc = capi.lib().qqt_recurrence_step(
         x.data_ptr(), x.stride(0), gate.data_ptr(), gate.stride(0),
         None if reset is None else reset.data_ptr(), 0 if reset is None else reset.stride(0),
