@@ -553,6 +553,7 @@ __global__ void __launch_bounds__(1024) k_ln_add(const float* __restrict__ part,
   const int64_t c = (int64_t)blockIdx.x * 32 + lane_id();
   const float* p = part + (int64_t)warp_id() * 2 * d + c;
   float s = 0.f;
+  before_me_done();
   if (c < 2 * d) {
 #pragma unroll 16
     for (int r = warp_id(); r < n_part; r += 32, p += 64 * d) s += *p;
@@ -824,7 +825,8 @@ extern "C" int qqt_layernorm_backward(const void* dy, int64_t dy_stride, const v
       });
     }
     if (sums)
-      k_ln_add<<<(unsigned)((2 * d + 31) / 32), 1024, 0, st>>>(part, (int)parts, d, dw, db);
+      launch_early(k_ln_add, dim3((unsigned)((2 * d + 31) / 32)), dim3(1024), 0, st, rows > 0, part,
+                   (int)parts, d, dw, db);
     return launch_status();
   });
 }

@@ -231,7 +231,33 @@ __device__ __forceinline__ float block_max_nan(float v, float* buf) {
   return v;
 }
 
-static inline int elem_bytes(int32_t dtype) { return dtype == QQT_F32 ? 4 : 2; }
+// Kernels of one call launched while the one before still runs: such a kernel
+// waits for that one's results with before_me_done(); let_next_start() allows
+// the next to be launched before this one ends.
+__device__ __forceinline__ void before_me_done() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void let_next_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+// early: the kernel before it in the stream is one of the same call's.  A
+// failure is left for launch_status.
+template <class... P, class... A>
+static void launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                         bool early, A... args) {
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = early ? 1 : 0;
+  (void)cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 static inline bool dtype_ok(int32_t dtype) { return dtype >= QQT_F32 && dtype <= QQT_BF16; }
 
 // Runs f(T{}) with the element type of `dtype`.

@@ -46,15 +46,6 @@ struct HeadStat {
   int act;                  // the action, -1 where it is none of the head's
 };
 
-// The counting, the row and the summing kernel overlap: each is launched while
-// the one before still runs, and waits for it where it needs its results.
-__device__ __forceinline__ void wait_for_counts() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-__device__ __forceinline__ void let_next_start() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-
 // Rows of the mask, at least 1; `counts`: the counting blocks' results.
 __device__ __forceinline__ float rows_counted(const QqtPolicyLoss& a, const int* counts) {
   if (!a.mask) return fmaxf((float)a.rows, 1.f);
@@ -298,7 +289,7 @@ __global__ void __launch_bounds__(kPlSmallRows)
   }
   if (!loss) return;
   if (fold) __syncthreads();
-  wait_for_counts();
+  before_me_done();
   const float count = fold ? fmaxf((float)n_mask, 1.f) : rows_counted(a, counts);
   const bool live = on && logp != -INFINITY && row.counts;
   const RowLoss l = loss_of(a, row, logp, live);
@@ -739,7 +730,7 @@ __global__ void __launch_bounds__(kPlThreads, kPlThreads == 512 ? 2 : 1)
   RowIn in{0.f, 0.f, 0.f, true};
   int n_counted = 0;
   if (a.old_logp) {
-    wait_for_counts();
+    before_me_done();
     if (a.mask) n_counted = counts[lane_id()] + counts[lane_id() + 32];
     in.old = a.old_logp[r];
     in.adv = a.adv[r];
@@ -915,7 +906,7 @@ __global__ void __launch_bounds__(1024)
                const int* __restrict__ counts) {
   __shared__ float buf[4][32];
   float s[4] = {0.f, 0.f, 0.f, 0.f};
-  wait_for_counts();
+  before_me_done();
 #pragma unroll 4
   for (int64_t r = threadIdx.x; r < n; r += 1024) {
     const float4 v = *reinterpret_cast<const float4*>(part + r * 4);
@@ -944,24 +935,6 @@ __global__ void __launch_bounds__(1024)
 }  // namespace qqt
 
 using namespace qqt;
-
-// early: the kernel before it in the stream is one of this call's, and this one
-// may start while that one still runs.
-template <class... P, class... A>
-static void pl_launch(void (*kernel)(P...), unsigned blocks, unsigned threads, size_t smem,
-                      cudaStream_t st, bool early, A... args) {
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = blocks;
-  cfg.blockDim = threads;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = at;
-  cfg.numAttrs = early ? 1 : 0;
-  (void)cudaLaunchKernelEx(&cfg, kernel, P(args)...);   // (launch_status reports a failure)
-}
 
 // 64 counts, then four partial sums a row (or a block of rows).
 extern "C" uint64_t qqt_policy_loss_work_bytes(int64_t rows) {
@@ -1000,7 +973,7 @@ extern "C" int qqt_policy_loss(const QqtPolicyLoss* a, qqt_stream_t stream) {
       if (small) {
         const size_t smem = (size_t)kPlSmallRows * ((v | 1) * 4 + (a->legal ? v : 0));
         auto run = [&](auto nh) {
-          pl_launch(k_pl_small<T, decltype(nh)::value>, (unsigned)blocks, kPlSmallRows, smem, st,
+          launch_early(k_pl_small<T, decltype(nh)::value>, dim3(blocks), dim3(kPlSmallRows), smem, st,
                     counts != nullptr, args, (int)v, counts, part, (int)one);
         };
         if (a->n_heads == 1)
@@ -1025,9 +998,9 @@ extern "C" int qqt_policy_loss(const QqtPolicyLoss* a, qqt_stream_t stream) {
       auto run = [&](auto gg) {
         constexpr int G = decltype(gg)::value;
         if (a->legal)
-          pl_launch(k_pl_rows<T, G, true>, n, threads, 0, st, counts != nullptr, args, counts, part);
+          launch_early(k_pl_rows<T, G, true>, dim3(n), dim3(threads), 0, st, counts != nullptr, args, counts, part);
         else
-          pl_launch(k_pl_rows<T, G, false>, n, threads, 0, st, counts != nullptr, args, counts, part);
+          launch_early(k_pl_rows<T, G, false>, dim3(n), dim3(threads), 0, st, counts != nullptr, args, counts, part);
       };
       if (g == 8)
         run(std::integral_constant<int, 8>{});
@@ -1038,6 +1011,6 @@ extern "C" int qqt_policy_loss(const QqtPolicyLoss* a, qqt_stream_t stream) {
       return 0;
     });
   if (a->stats && !one)
-    pl_launch(k_pl_stats, 1, 1024, 0, st, a->rows > 0, args, part, small ? blocks : a->rows, counts);
+    launch_early(k_pl_stats, dim3(1), dim3(1024), 0, st, a->rows > 0, args, part, small ? blocks : a->rows, counts);
   return launch_status();
 }

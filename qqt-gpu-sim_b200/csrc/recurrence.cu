@@ -170,6 +170,7 @@ __global__ void __launch_bounds__(kSeqThreads, kFwdBlocks) k_rec_seq_fwd(RecArgs
   const int64_t ticks = a.nT - first < a.seg ? a.nT - first : a.seg;
   const T *xp = at<T>(a.x, p, first), *gp = at<T>(a.g, p, first);
   T* hp = at<T>(a.h, p, first);
+  if (a.enters) before_me_done();
   const float* from = a.enters ? a.enters + (int64_t)blockIdx.y * a.nC : a.s0;
   Vec<float, VEC> s = from ? ld_vec<float, VEC>(from + p.c) : vec_zero<float, VEC>();
   float* cp = a.carry ? a.carry + first / kRecU * a.nC + p.c : nullptr;
@@ -293,6 +294,7 @@ __global__ void __launch_bounds__(kSeqThreads, kBwdBlocks) k_rec_seq_bwd(RecArgs
   const int64_t full = end / kRecU;    // (batches are counted from tick 0)
   const int rem = (int)(end % kRecU);
   const bool has_dh = a.h.p != nullptr;
+  if (a.enters) before_me_done();
   const float* from = a.enters ? a.enters + (int64_t)blockIdx.y * a.nC : a.s0;
   Vec<float, VEC> acc = from ? ld_vec<float, VEC>(from + p.c) : vec_zero<float, VEC>();
   Vec<T, VEC> x[kRecU], g[kRecU], dh[kRecU];
@@ -368,7 +370,12 @@ __global__ void __launch_bounds__(kSeqThreads, kBwdBlocks) k_rec_seq_bwd(RecArgs
 // ------------------------------------------------------------- segments
 
 // The pair of a segment of VEC channels: (A, B) of the state, or, with BWD,
-// (A, G) of the gradient, scanned from the segment's last tick down.
+// (A, G) of the gradient.  The segment is gone through against the direction
+// of the walk that follows, which then finds what was read last -- the ticks
+// it begins with -- still in L2.  P is the product of the gates between the
+// tick and the segment's exit, so B = sum P' i x over the ticks, P' before the
+// tick's own gate, and G = sum P dh with it.  What lies beyond a reset never
+// comes through: P is -0 from there on, and nothing more is added.
 template <class T, int VEC, bool BWD>
 __device__ __forceinline__ void pair_tick(const Vec<T, VEC>& x, const Vec<T, VEC>& g, bool r,
                                           float* A, float* B) {
@@ -376,9 +383,14 @@ __device__ __forceinline__ void pair_tick(const Vec<T, VEC>& x, const Vec<T, VEC
   for (int v = 0; v < VEC; ++v) {
     float f, i;
     gates<T>(g.get(v), f, i);
-    B[v] = BWD ? f * (x.get(v) + B[v]) : fmaf(f, r ? 0.f : B[v], i * x.get(v));
-    if (BWD && r) B[v] = 0.f;
-    A[v] = r || drops(A[v]) ? -0.f : A[v] * f;
+    const bool gone = drops(A[v]);
+    if (BWD) {
+      A[v] = r || gone ? -0.f : A[v] * f;
+      B[v] = drops(A[v]) ? B[v] : fmaf(A[v], x.get(v), B[v]);
+    } else {
+      B[v] = gone ? B[v] : fmaf(A[v], i * x.get(v), B[v]);
+      A[v] = r || gone ? -0.f : A[v] * f;
+    }
   }
 }
 
@@ -400,34 +412,26 @@ __global__ void __launch_bounds__(kSeqThreads, kFwdBlocks) k_rec_sum(RecArgs a) 
 #pragma unroll
   for (int u = 0; u < kRecU; ++u) x[u] = vec_zero<T, VEC>();
   const int64_t full = end / kRecU, b0 = first / kRecU;   // batches counted from tick 0
-  const int rem = (int)(end % kRecU);
-  if (BWD && rem) {                  // (only the last segment ends inside a batch)
-    load_ticks<T, VEC>(at<T>(a.g, p, full * kRecU), a.g.ts, rem, g);
-    if (has_in) load_ticks<T, VEC>(at<T>(in, p, full * kRecU), in.ts, rem, x);
-    const unsigned rst = load_resets(a, p, full * kRecU);
-#pragma unroll
-    for (int u = kRecU - 1; u >= 0; --u)
-      if (u < rem) pair_tick<T, VEC, BWD>(x[u], g[u], (rst >> u) & 1, A, B);
-  }
+  const int rem = (int)(end % kRecU);                      // (only in the last segment: BWD)
   if (full > b0) {
-    const int64_t dir = BWD ? -1 : 1;
-    int64_t b = BWD ? full - 1 : b0;
+    const int64_t dir = BWD ? 1 : -1;
+    int64_t b = BWD ? b0 : full - 1;
     const T* gp = at<T>(a.g, p, b * kRecU);
     const T* xp = has_in ? at<T>(in, p, b * kRecU) : nullptr;
     load_ticks<T, VEC>(gp, a.g.ts, kRecU, g);
     if (has_in) load_ticks<T, VEC>(xp, in.ts, kRecU, x);
     unsigned rst = load_resets(a, p, b * kRecU);
-    // from here on the pointers are at the scan's first tick of the next batch
+    // from here on the pointers are at the first tick of the next batch
     const int64_t gs = dir * a.g.ts, xs = dir * in.ts;
-    const T* gn = BWD ? gp - a.g.ts : gp + kRecU * a.g.ts;
-    const T* xn = BWD ? xp - in.ts : xp + kRecU * in.ts;
+    const T* gn = BWD ? gp + kRecU * a.g.ts : gp - a.g.ts;
+    const T* xn = BWD ? xp + kRecU * in.ts : xp - in.ts;
     for (int64_t left = full - b0; left > 0; --left) {
       const bool more = left > 1;
       b += dir;
       const unsigned rst_next = more ? load_resets(a, p, b * kRecU) : 0;
 #pragma unroll
       for (int j = 0; j < kRecU; ++j) {
-        const int u = BWD ? kRecU - 1 - j : j;
+        const int u = BWD ? j : kRecU - 1 - j;
         pair_tick<T, VEC, BWD>(x[u], g[u], (rst >> u) & 1, A, B);
         if (more) {
           g[u] = ld_vec<T, VEC>(gn);
@@ -438,6 +442,14 @@ __global__ void __launch_bounds__(kSeqThreads, kFwdBlocks) k_rec_sum(RecArgs a) 
       }
       rst = rst_next;
     }
+  }
+  if (BWD && rem) {
+    load_ticks<T, VEC>(at<T>(a.g, p, full * kRecU), a.g.ts, rem, g);
+    if (has_in) load_ticks<T, VEC>(at<T>(in, p, full * kRecU), in.ts, rem, x);
+    const unsigned rst = load_resets(a, p, full * kRecU);
+#pragma unroll
+    for (int u = 0; u < kRecU; ++u)
+      if (u < rem) pair_tick<T, VEC, BWD>(x[u], g[u], (rst >> u) & 1, A, B);
   }
   if (!p.on) return;
 #pragma unroll
@@ -453,6 +465,7 @@ template <bool BWD>
 __global__ void __launch_bounds__(1024) k_rec_join(RecArgs a, int segs) {
   __shared__ float sA[32][33], sB[32][33];
   const int l = lane_id(), w = warp_id();
+  before_me_done();
   const uint32_t c0 = blockIdx.x * 32 + l;
   const bool on = c0 < a.nC;
   const uint32_t c = on ? c0 : a.nC - 1;
@@ -555,12 +568,13 @@ static int rec_walk(RecArgs a, void* work, cudaStream_t st) {
     a.pair = (float2*)work;
     a.enters = (float*)(a.pair + (int64_t)(cut.segs - 1) * a.nC);
     k_rec_sum<T, VEC, BWD><<<dim3(blocks, cut.segs - 1), kSeqThreads, 0, st>>>(a);
-    k_rec_join<BWD><<<(a.nC + 31) / 32, 1024, 0, st>>>(a, cut.segs);
+    launch_early(k_rec_join<BWD>, dim3((a.nC + 31) / 32), dim3(1024), 0, st, true, a, cut.segs);
   }
+  const bool early = cut.segs > 1;
   if (BWD)
-    k_rec_seq_bwd<T, VEC><<<dim3(blocks, cut.segs), kSeqThreads, 0, st>>>(a);
+    launch_early(k_rec_seq_bwd<T, VEC>, dim3(blocks, cut.segs), dim3(kSeqThreads), 0, st, early, a);
   else
-    k_rec_seq_fwd<T, VEC><<<dim3(blocks, cut.segs), kSeqThreads, 0, st>>>(a);
+    launch_early(k_rec_seq_fwd<T, VEC>, dim3(blocks, cut.segs), dim3(kSeqThreads), 0, st, early, a);
   return launch_status();
 }
 
