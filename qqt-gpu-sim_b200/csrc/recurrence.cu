@@ -376,20 +376,21 @@ __global__ void __launch_bounds__(kSeqThreads, kBwdBlocks) k_rec_seq_bwd(RecArgs
 // tick and the segment's exit, so B = sum P' i x over the ticks, P' before the
 // tick's own gate, and G = sum P dh with it.  What lies beyond a reset never
 // comes through: P is -0 from there on, and nothing more is added.
-template <class T, int VEC, bool BWD>
+// CLEAN: no lane has met a reset.
+template <class T, int VEC, bool BWD, bool CLEAN>
 __device__ __forceinline__ void pair_tick(const Vec<T, VEC>& x, const Vec<T, VEC>& g, bool r,
                                           float* A, float* B) {
 #pragma unroll
   for (int v = 0; v < VEC; ++v) {
     float f, i;
     gates<T>(g.get(v), f, i);
-    const bool gone = drops(A[v]);
+    const bool gone = !CLEAN && drops(A[v]);
     if (BWD) {
-      A[v] = r || gone ? -0.f : A[v] * f;
-      B[v] = drops(A[v]) ? B[v] : fmaf(A[v], x.get(v), B[v]);
+      A[v] = !CLEAN && (r || gone) ? -0.f : A[v] * f;
+      B[v] = !CLEAN && drops(A[v]) ? B[v] : fmaf(A[v], x.get(v), B[v]);
     } else {
       B[v] = gone ? B[v] : fmaf(A[v], i * x.get(v), B[v]);
-      A[v] = r || gone ? -0.f : A[v] * f;
+      A[v] = !CLEAN && (r || gone) ? -0.f : A[v] * f;
     }
   }
 }
@@ -413,6 +414,7 @@ __global__ void __launch_bounds__(kSeqThreads, kFwdBlocks) k_rec_sum(RecArgs a) 
   for (int u = 0; u < kRecU; ++u) x[u] = vec_zero<T, VEC>();
   const int64_t full = end / kRecU, b0 = first / kRecU;   // batches counted from tick 0
   const int rem = (int)(end % kRecU);                      // (only in the last segment: BWD)
+  bool done = false;
   if (full > b0) {
     const int64_t dir = BWD ? 1 : -1;
     int64_t b = BWD ? b0 : full - 1;
@@ -429,27 +431,37 @@ __global__ void __launch_bounds__(kSeqThreads, kFwdBlocks) k_rec_sum(RecArgs a) 
       const bool more = left > 1;
       b += dir;
       const unsigned rst_next = more ? load_resets(a, p, b * kRecU) : 0;
+      auto batch = [&](auto clean) {
 #pragma unroll
-      for (int j = 0; j < kRecU; ++j) {
-        const int u = BWD ? j : kRecU - 1 - j;
-        pair_tick<T, VEC, BWD>(x[u], g[u], (rst >> u) & 1, A, B);
-        if (more) {
-          g[u] = ld_vec<T, VEC>(gn);
-          if (has_in) x[u] = ld_vec<T, VEC>(xn);
+        for (int j = 0; j < kRecU; ++j) {
+          const int u = BWD ? j : kRecU - 1 - j;
+          pair_tick<T, VEC, BWD, decltype(clean)::value>(x[u], g[u], (rst >> u) & 1, A, B);
+          if (more) {
+            g[u] = ld_vec<T, VEC>(gn);
+            if (has_in) x[u] = ld_vec<T, VEC>(xn);
+          }
+          gn += gs;
+          xn += xs;
         }
-        gn += gs;
-        xn += xs;
+      };
+      if (__all_sync(QQT_FULL, rst == 0 && !drops(A[0])))
+        batch(std::true_type{});
+      else
+        batch(std::false_type{});
+      if (__all_sync(QQT_FULL, drops(A[0]))) {   // nothing more comes through
+        done = true;
+        break;
       }
       rst = rst_next;
     }
   }
-  if (BWD && rem) {
+  if (BWD && rem && !done) {
     load_ticks<T, VEC>(at<T>(a.g, p, full * kRecU), a.g.ts, rem, g);
     if (has_in) load_ticks<T, VEC>(at<T>(in, p, full * kRecU), in.ts, rem, x);
     const unsigned rst = load_resets(a, p, full * kRecU);
 #pragma unroll
     for (int u = 0; u < kRecU; ++u)
-      if (u < rem) pair_tick<T, VEC, BWD>(x[u], g[u], (rst >> u) & 1, A, B);
+      if (u < rem) pair_tick<T, VEC, BWD, false>(x[u], g[u], (rst >> u) & 1, A, B);
   }
   if (!p.on) return;
 #pragma unroll
@@ -471,16 +483,17 @@ __global__ void __launch_bounds__(1024) k_rec_join(RecArgs a, int segs) {
   const uint32_t c = on ? c0 : a.nC - 1;
   const int per = (segs + 31) / 32;
   const int k0 = w * per, k1 = k0 + per < segs ? k0 + per : segs;
-  constexpr int Q = 8;
-  auto pair_of = [&](int k) {        // that of the k-th segment along the scan
-    return a.pair[(int64_t)(BWD ? segs - 2 - k : k) * a.nC + c];
+  constexpr int Q = 16;              // of a share's pairs, the last ones read stay in registers
+  float2 v[Q];
+  auto read = [&](int k) {           // those of the segments from the k-th along the scan
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+      if (k + q < k1 && k + q + 1 < segs)
+        v[q] = a.pair[(int64_t)(BWD ? segs - 2 - (k + q) : k + q) * a.nC + c];
   };
   float A = 1.f, B = 0.f;
   for (int k = k0; k < k1; k += Q) {
-    float2 v[Q];
-#pragma unroll
-    for (int q = 0; q < Q; ++q)
-      if (k + q < k1 && k + q + 1 < segs) v[q] = pair_of(k + q);
+    read(k);
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       if (k + q < k1 && k + q + 1 < segs) {
@@ -494,7 +507,7 @@ __global__ void __launch_bounds__(1024) k_rec_join(RecArgs a, int segs) {
   __syncthreads();
   if (w == 0) {
     float s = a.s0 ? a.s0[c] : 0.f;
-#pragma unroll 8
+#pragma unroll
     for (int q = 0; q < 32; ++q) {
       const float nA = sA[q][l], nB = sB[q][l];
       sB[q][l] = s;
@@ -504,10 +517,7 @@ __global__ void __launch_bounds__(1024) k_rec_join(RecArgs a, int segs) {
   __syncthreads();
   float s = sB[w][l];
   for (int k = k0; k < k1; k += Q) {
-    float2 v[Q];
-#pragma unroll
-    for (int q = 0; q < Q; ++q)
-      if (k + q < k1 && k + q + 1 < segs) v[q] = pair_of(k + q);
+    if (per > Q) read(k);
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       if (k + q < k1) {
