@@ -35,6 +35,12 @@ constexpr int kLnRowThreads16 = 768, kLnRowThreads32 = 512;
 // keeps 2 e sums besides its operands.
 __host__ __device__ constexpr int ln_max_threads(int e) { return e == 16 ? 768 : 512; }
 
+// 1 / sqrt(v) of the unit with one Newton step: float32 accuracy.
+__device__ __forceinline__ float ln_rstd(float v) {
+  const float r = rsqrtf(v);
+  return r * fmaf(-0.5f * v * r, r, 1.5f);
+}
+
 // Sums of N values over a team of G lanes (G <= 32), or over the block (G =
 // 0; buf holds 2 x N x 32 floats, used in turn so that one barrier is enough).
 template <int G, int N>
@@ -128,13 +134,73 @@ __device__ __forceinline__ void ln_load(const T* p, const LnTeam& t, int nv, int
     out[k] = on && j < nv ? ln_get<T, VEC, WHOLE>(p, j, d) : vec_zero<T, VEC>();
   }
 }
+// The steps of both passes on one vector, two values at a time.
+// Sums f, and its square once it is centred.
+template <int VEC>
+__device__ __forceinline__ void ln_sum(const float* f, f32x2& s) {
+#pragma unroll
+  for (int v = 0; v < VEC; v += 2) s = add2(s, pair(f[v], f[v + 1]));
+}
+template <int VEC>
+__device__ __forceinline__ void ln_centre(float* f, float mu, f32x2& s) {
+  const f32x2 m = pair(-mu, -mu);
+#pragma unroll
+  for (int v = 0; v < VEC; v += 2) {
+    const f32x2 c = add2(pair(f[v], f[v + 1]), m);
+    f[v] = c.x;
+    f[v + 1] = c.y;
+    s = fma2(c, c, s);
+  }
+}
 // The scaled and shifted row.
 template <int VEC>
 __device__ __forceinline__ void ln_scale(const float* c, float rs, const Vec<float, VEC>& w,
                                          bool has_b, const Vec<float, VEC>& b, float* o) {
+  const f32x2 r = pair(rs, rs);
 #pragma unroll
-  for (int v = 0; v < VEC; ++v)
-    o[v] = has_b ? fmaf(c[v] * rs, w.get(v), b.get(v)) : c[v] * rs * w.get(v);
+  for (int v = 0; v < VEC; v += 2) {
+    const f32x2 x = mul2(pair(c[v], c[v + 1]), r), wv = pair(w.get(v), w.get(v + 1));
+    const f32x2 y = has_b ? fma2(x, wv, pair(b.get(v), b.get(v + 1))) : mul2(x, wv);
+    o[v] = y.x;
+    o[v + 1] = y.y;
+  }
+}
+// Backward, first half: the sums of dy xh and dy (columns), of q and q xh (row).
+template <class T, int VEC>
+__device__ __forceinline__ void ln_gather(const Vec<T, VEC>& cx, const Vec<T, VEC>& cy,
+                                          const float* w, float mu, float rs, float* aw, float* ab,
+                                          f32x2& s1, f32x2& s2) {
+  const f32x2 m = pair(-mu, -mu), r = pair(rs, rs);
+#pragma unroll
+  for (int v = 0; v < VEC; v += 2) {
+    const f32x2 g = pair(cy.get(v), cy.get(v + 1));
+    const f32x2 xh = mul2(add2(pair(cx.get(v), cx.get(v + 1)), m), r);
+    const f32x2 q = mul2(g, pair(w[v], w[v + 1]));
+    const f32x2 nb = add2(pair(ab[v], ab[v + 1]), g), nw = fma2(g, xh, pair(aw[v], aw[v + 1]));
+    ab[v] = nb.x;
+    ab[v + 1] = nb.y;
+    aw[v] = nw.x;
+    aw[v + 1] = nw.y;
+    s1 = add2(s1, q);
+    s2 = fma2(q, xh, s2);
+  }
+}
+// Second half: dx = rs q - rs m1 - (x - mu) rs^2 m2, m1 and m2 the row's means.
+template <class T, int VEC>
+__device__ __forceinline__ void ln_spread(const Vec<T, VEC>& cx, const Vec<T, VEC>& cy,
+                                          const float* w, float mu, float rs, float m1, float m2,
+                                          float* o) {
+  const f32x2 m = pair(-mu, -mu), r = pair(rs, rs);
+  const float a = -rs * m1, b = -rs * rs * m2;
+  const f32x2 c1 = pair(a, a), c2 = pair(b, b);
+#pragma unroll
+  for (int v = 0; v < VEC; v += 2) {
+    const f32x2 q = mul2(pair(cy.get(v), cy.get(v + 1)), pair(w[v], w[v + 1]));
+    const f32x2 x = add2(pair(cx.get(v), cx.get(v + 1)), m);
+    const f32x2 y = fma2(q, r, fma2(x, c2, c1));
+    o[v] = y.x;
+    o[v + 1] = y.y;
+  }
 }
 
 template <class T, int VEC, int K, int G, bool WHOLE>
@@ -155,30 +221,34 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K))
   for (int64_t lr = lead; lr < rows; lr += t.rows_step) {
     const bool on = t.row < rows;
     float f[K][VEC];
-    float s[1] = {0.f};
+    f32x2 s2 = pair(0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k) {
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        f[k][v] = c[k].get(v);
-        s[0] += f[k][v];
-      }
+      for (int v = 0; v < VEC; ++v) f[k][v] = c[k].get(v);
+      ln_sum<VEC>(f[k], s2);
+    }
+    float s[1] = {s2.x + s2.y};
     // the next row's values are on their way meanwhile
     const int64_t next = t.row + t.rows_step;
     ln_load<T, VEC, K, WHOLE>(x + next * xs, t, nv, d, next < rows, c);
     team_sum<G, 1>(s, buf, turn);
     const float mu = s[0] * inv_d;
-    s[0] = 0.f;
+    s2 = pair(0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (t.j + k * t.step < nv)
+    for (int k = 0; k < K; ++k) {
+      const int j = t.j + k * t.step;
+      if (j < nv) {
+        if (!WHOLE && (j + 1) * VEC > d)   // what pads the row's last vector adds nothing
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          f[k][v] = WHOLE || (t.j + k * t.step) * VEC + v < d ? f[k][v] - mu : 0.f;
-          s[0] = fmaf(f[k][v], f[k][v], s[0]);
-        }
+          for (int v = 0; v < VEC; ++v)
+            if (j * VEC + v >= d) f[k][v] = mu;
+        ln_centre<VEC>(f[k], mu, s2);
+      }
+    }
+    s[0] = s2.x + s2.y;
     team_sum<G, 1>(s, buf, turn);
-    const float rs = 1.f / sqrtf(s[0] * inv_d + eps);
+    const float rs = ln_rstd(s[0] * inv_d + eps);
     if (on) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
@@ -218,9 +288,8 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K), 
   for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int v = 0; v < VEC; ++v) aw[k][v] = ab[k][v] = 0.f;
-  // Few elements: the scaled values stay for the second half and the next row
-  // is loaded meanwhile.  Many: they are made again from the packed operands.
-  constexpr bool KEEP = VEC * K <= 8;
+  // Few elements: the next row is loaded while this one is finished.
+  constexpr bool AHEAD = VEC * K <= 8;
   Vec<T, VEC> cx[K], cy[K];
   ln_load<T, VEC, K, WHOLE>(x + t.row * xs, t, nv, d, t.row < rows, cx);
   ln_load<T, VEC, K, WHOLE>(dy + t.row * dys, t, nv, d, t.row < rows, cy);
@@ -228,26 +297,21 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K), 
   for (int64_t lr = lead; lr < rows; lr += t.rows_step) {
     const bool on = t.row < rows;
     const float m0 = mu, r0 = rs;
-    float xk[KEEP ? K : 1][VEC], qk[KEEP ? K : 1][VEC];
-    float s[2] = {0.f, 0.f};
+    f32x2 s1 = pair(0.f, 0.f), s2 = s1;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int j = t.j + k * t.step;
       if (j < nv) {
         const Vec<float, VEC> wv = ln_param<VEC, WHOLE>(w, j, d);
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          const float g = cy[k].get(v), xh = (cx[k].get(v) - m0) * r0, q = g * wv.get(v);
-          ab[k][v] += g;
-          aw[k][v] = fmaf(g, xh, aw[k][v]);
-          s[0] += q;
-          s[1] = fmaf(q, xh, s[1]);
-          if (KEEP) {
-            xk[KEEP ? k : 0][v] = xh;
-            qk[KEEP ? k : 0][v] = q;
-          }
-        }
+        ln_gather<T, VEC>(cx[k], cy[k], wv.v, m0, r0, aw[k], ab[k], s1, s2);
       }
+    }
+    float s[2] = {s1.x + s1.y, s2.x + s2.y};
+    Vec<T, VEC> px[K], py[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      px[k] = cx[k];
+      py[k] = cy[k];
     }
     const int64_t next = t.row + t.rows_step;
     auto load_next = [&] {
@@ -258,7 +322,7 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K), 
         rs = rstd[next];
       }
     };
-    if (KEEP || !dx) load_next();
+    if (AHEAD || !dx) load_next();
     if (dx) {
       team_sum<G, 2>(s, buf, turn);
       const float m1 = s[0] * inv_d, m2 = s[1] * inv_d;
@@ -267,20 +331,12 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K), 
         const int j = t.j + k * t.step;
         if (on && j < nv) {
           float o[VEC];
-          if (KEEP) {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v)
-              o[v] = r0 * (fmaf(-xk[KEEP ? k : 0][v], m2, qk[KEEP ? k : 0][v]) - m1);
-          } else {
-            const Vec<float, VEC> wv = ln_param<VEC, WHOLE>(w, j, d);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v)
-              o[v] = r0 * (fmaf(-(cx[k].get(v) - m0) * r0, m2, cy[k].get(v) * wv.get(v)) - m1);
-          }
+          const Vec<float, VEC> wv = ln_param<VEC, WHOLE>(w, j, d);
+          ln_spread<T, VEC>(px[k], py[k], wv.v, m0, r0, m1, m2, o);
           ln_put<T, VEC, WHOLE>(dx + t.row * d, j, d, o);
         }
       }
-      if (!KEEP) load_next();
+      if (!AHEAD) load_next();
     }
     t.row = next;
   }
@@ -375,33 +431,28 @@ __global__ void __launch_bounds__(ln_max_threads(VEC* K))
     if (alive) alive = stage_wait(&bar[s], parity);
     const T* in = (const T*)(stage + (size_t)s * ring.stage_bytes);
     float f[K][VEC];
-    float sum[1] = {0.f};
+    f32x2 s2 = pair(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int j = threadIdx.x + k * blockDim.x;
       if (j < nv) {
         const Vec<T, VEC> c = ld_vec<T, VEC>(in + j * VEC);
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          f[k][v] = c.get(v);
-          sum[0] += f[k][v];
-        }
+        for (int v = 0; v < VEC; ++v) f[k][v] = c.get(v);
+        ln_sum<VEC>(f[k], s2);
       }
     }
+    float sum[1] = {s2.x + s2.y};
     team_sum<0, 1>(sum, buf, turn);        // (its barrier: everyone has read the stage)
     if (threadIdx.x == 0) fetch(row + (int64_t)ring.stages * gridDim.x, s);
     const float mu = sum[0] * inv_d;
-    sum[0] = 0.f;
+    s2 = pair(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < K; ++k)
-      if (threadIdx.x + k * blockDim.x < nv)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          f[k][v] -= mu;
-          sum[0] = fmaf(f[k][v], f[k][v], sum[0]);
-        }
+      if (threadIdx.x + k * blockDim.x < nv) ln_centre<VEC>(f[k], mu, s2);
+    sum[0] = s2.x + s2.y;
     team_sum<0, 1>(sum, buf, turn);
-    const float rs = 1.f / sqrtf(sum[0] * inv_d + eps);
+    const float rs = ln_rstd(sum[0] * inv_d + eps);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int j = threadIdx.x + k * blockDim.x;
@@ -480,25 +531,18 @@ __global__ void __launch_bounds__(ln_max_threads(VEC* K))
     if (alive) alive = stage_wait(&bar[s], parity);
     const T* ix = (const T*)(stage + (size_t)s * ring.stage_bytes);
     const T* iy = (const T*)((const unsigned char*)ix + ring.stage_bytes / 2);
-    float sum[2] = {0.f, 0.f};
+    f32x2 s1 = pair(0.f, 0.f), s2 = s1;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int j = threadIdx.x + k * blockDim.x;
       if (j < nv) {
-        const Vec<T, VEC> cx = ld_vec<T, VEC>(ix + j * VEC), cy = ld_vec<T, VEC>(iy + j * VEC);
         Vec<float, VEC> wv;
         if (!WREG) wv = ln_param<VEC, true>(w, j, d);
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          const float g = cy.get(v), xh = (cx.get(v) - m0) * r0;
-          const float q = g * (WREG ? wr[WREG ? k : 0][v] : wv.get(v));
-          ab[k][v] += g;
-          aw[k][v] = fmaf(g, xh, aw[k][v]);
-          sum[0] += q;
-          sum[1] = fmaf(q, xh, sum[1]);
-        }
+        ln_gather<T, VEC>(ld_vec<T, VEC>(ix + j * VEC), ld_vec<T, VEC>(iy + j * VEC),
+                          WREG ? wr[WREG ? k : 0] : wv.v, m0, r0, aw[k], ab[k], s1, s2);
       }
     }
+    float sum[2] = {s1.x + s1.y, s2.x + s2.y};
     if (dx)
       team_sum<0, 2>(sum, buf, turn);      // (its barrier: the row before is done with)
     else
@@ -511,15 +555,11 @@ __global__ void __launch_bounds__(ln_max_threads(VEC* K))
       for (int k = 0; k < K; ++k) {
         const int j = threadIdx.x + k * blockDim.x;
         if (j < nv) {
-          const Vec<T, VEC> cx = ld_vec<T, VEC>(ix + j * VEC), cy = ld_vec<T, VEC>(iy + j * VEC);
           Vec<float, VEC> wv;
           if (!WREG) wv = ln_param<VEC, true>(w, j, d);
           float o[VEC];
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) {
-            const float q = cy.get(v) * (WREG ? wr[WREG ? k : 0][v] : wv.get(v));
-            o[v] = r0 * (fmaf(-(cx.get(v) - m0) * r0, m2, q) - m1);
-          }
+          ln_spread<T, VEC>(ld_vec<T, VEC>(ix + j * VEC), ld_vec<T, VEC>(iy + j * VEC),
+                            WREG ? wr[WREG ? k : 0] : wv.v, m0, r0, m1, m2, o);
           ln_put<T, VEC, true>(dx + row * d, j, d, o);
         }
       }

@@ -135,6 +135,13 @@ __device__ __forceinline__ Vec<T, VEC> vec_zero() {
 }
 static inline bool aligned_to(const void* p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
+// Pairs of floats, one instruction for both.
+typedef float2 f32x2;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) { return make_float2(lo, hi); }
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) { return __ffma2_rn(a, b, c); }
+
 // Rows staged by bulk copies: one mbarrier per stage, armed with the bytes of
 // its copies.  Waits are bounded; a wait that runs out is reported by the
 // device error word, and the kernel goes on to its end without further waits.

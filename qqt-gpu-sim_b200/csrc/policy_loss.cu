@@ -360,13 +360,6 @@ __global__ void __launch_bounds__(kPlSmallRows)
 
 // ------------------------------------------------- many logits: team per row
 
-// Pairs of floats in one instruction each.
-typedef float2 f32x2;
-__device__ __forceinline__ f32x2 pair(float lo, float hi) { return make_float2(lo, hi); }
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) { return __fadd2_rn(a, b); }
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) { return __fmul2_rn(a, b); }
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) { return __ffma2_rn(a, b, c); }
-
 // The VEC elements from the s-th (0 < s < VEC) of the 2 VEC of a and b.
 template <class T, int VEC>
 __device__ __forceinline__ uint4 funnel(uint4 a, uint4 b, int s) {
