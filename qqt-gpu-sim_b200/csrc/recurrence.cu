@@ -49,21 +49,50 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   return r;
 }
 template <class T>
-__device__ __forceinline__ void gates(float gate, float& f, float& i) {
+__device__ __forceinline__ void gates(f32x2 gate, f32x2& f, f32x2& i) {
   constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-  float e;
+  f32x2 e;
   if constexpr (sizeof(T) == 4) {
-    const float g = max_nan(min_nan(gate, 120.f), -86.f);
-    const float p = g * kLog2e;
-    // g log2 e - p: the product's rounding and log2 e's own tail
-    const float lost = fmaf(g, 1.9259629911e-8f, fmaf(g, kLog2e, -p));
-    e = ex2_approx(-p);
-    e = fmaf(e, -kLn2 * lost, e);
+    const f32x2 g = pair(max_nan(min_nan(gate.x, 120.f), -86.f), max_nan(min_nan(gate.y, 120.f), -86.f));
+    const f32x2 l2 = pair(-kLog2e, -kLog2e);
+    const f32x2 p = mul2(g, l2);
+    // the product's rounding and log2 e's own tail
+    const f32x2 lost = fma2(g, pair(-1.9259629911e-8f, -1.9259629911e-8f),
+                            fma2(g, l2, pair(-p.x, -p.y)));
+    e = pair(ex2_approx(p.x), ex2_approx(p.y));
+    e = fma2(e, mul2(lost, pair(kLn2, kLn2)), e);
   } else {
-    e = ex2_approx(min_nan(gate * -kLog2e, 125.f));
+    const f32x2 p = mul2(gate, pair(-kLog2e, -kLog2e));
+    e = pair(ex2_approx(min_nan(p.x, 125.f)), ex2_approx(min_nan(p.y, 125.f)));
   }
-  f = rcp_approx(1.f + e);
-  i = e * f;
+  const f32x2 d = add2(e, pair(1.f, 1.f));
+  f = pair(rcp_approx(d.x), rcp_approx(d.y));
+  i = mul2(e, f);
+}
+// Values v and v + 1 of a vector (the second of a single one is a copy, never used).
+template <class T, int VEC>
+__device__ __forceinline__ f32x2 two(const Vec<T, VEC>& x, int v) {
+  const float a = x.get(v);
+  return pair(a, VEC > 1 ? x.get(v + 1) : a);
+}
+template <int VEC>
+__device__ __forceinline__ f32x2 two(const float* x, int v) {
+  return pair(x[v], VEC > 1 ? x[v + 1] : x[v]);
+}
+template <int VEC>
+__device__ __forceinline__ void set_two(float* x, int v, f32x2 q) {
+  x[v] = q.x;
+  if (VEC > 1) x[v + 1] = q.y;
+}
+// A walk's tick: s = f s + i x.
+template <class T, int VEC>
+__device__ __forceinline__ void tick(const Vec<T, VEC>& x, const Vec<T, VEC>& g, float* s) {
+#pragma unroll
+  for (int v = 0; v < VEC; v += 2) {
+    f32x2 f, i;
+    gates<T>(two(g, v), f, i);
+    set_two<VEC>(s, v, fma2(f, two<VEC>(s, v), mul2(i, two(x, v))));
+  }
 }
 
 __device__ __forceinline__ bool drops(float a) { return __float_as_int(a) < 0; }
@@ -105,12 +134,7 @@ __global__ void k_rec_step(RecArgs a) {
     for (int v = 0; v < VEC; ++v) s.v[v] = 0.f;
   }
   Vec<T, VEC> o;
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    float f, i;
-    gates<T>(g.get(v), f, i);
-    s.v[v] = fmaf(f, s.v[v], i * x.get(v));
-  }
+  tick<T, VEC>(x, g, s.v);
   o.put(s.v);
   st_vec((T*)a.h.p + n * a.h.ns + d, o);
   if (a.s_end) st_vec(a.s_end + c, s);
@@ -199,12 +223,7 @@ __global__ void __launch_bounds__(kSeqThreads, kFwdBlocks) k_rec_seq_fwd(RecArgs
         for (int v = 0; v < VEC; ++v) s.v[v] = 0.f;
       }
       Vec<T, VEC> o;
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        float f, i;
-        gates<T>(g[u].get(v), f, i);
-        s.v[v] = fmaf(f, s.v[v], i * x[u].get(v));
-      }
+      tick<T, VEC>(x[u], g[u], s.v);
       o.put(s.v);
       if (more) {
         x[u] = ld_vec<T, VEC>(xn);
@@ -224,13 +243,9 @@ __global__ void __launch_bounds__(kSeqThreads, kFwdBlocks) k_rec_seq_fwd(RecArgs
 #pragma unroll
     for (int u = 0; u < kRecU; ++u) {
       if (u >= rem) break;
+      if ((rst >> u) & 1) s = vec_zero<float, VEC>();
       Vec<T, VEC> o;
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        float f, i;
-        gates<T>(g[u].get(v), f, i);
-        s.v[v] = fmaf(f, (rst >> u) & 1 ? 0.f : s.v[v], i * x[u].get(v));
-      }
+      tick<T, VEC>(x[u], g[u], s.v);
       o.put(s.v);
       if (p.on) st_vec(hp, o);
       hp += a.h.ts;
@@ -253,15 +268,10 @@ __device__ __forceinline__ void backward_ticks(const Vec<T, VEC>* x, const Vec<T
 #pragma unroll
   for (int u = 0; u < kRecU; ++u) {
     if (u < n) {
+      if (!CLEAN && ((rst >> u) & 1)) s = vec_zero<float, VEC>();
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        prev[u][v] = !CLEAN && ((rst >> u) & 1) ? 0.f : s.v[v];
-        if (u + 1 < kRecU) {
-          float f, i;
-          gates<T>(g[u].get(v), f, i);
-          s.v[v] = fmaf(f, prev[u][v], i * x[u].get(v));
-        }
-      }
+      for (int v = 0; v < VEC; ++v) prev[u][v] = s.v[v];
+      if (u + 1 < kRecU) tick<T, VEC>(x[u], g[u], s.v);
     }
   }
 #pragma unroll
@@ -270,15 +280,16 @@ __device__ __forceinline__ void backward_ticks(const Vec<T, VEC>* x, const Vec<T
       Vec<T, VEC> dx, dg;
       float fx[VEC], fg[VEC];
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        float f, i;
-        gates<T>(g[u].get(v), f, i);
-        const float e = dh[u].get(v) + acc.v[v];
-        const float fe = f * e;
-        fx[v] = i * e;
-        fg[v] = i * fe * (prev[u][v] - x[u].get(v));
-        acc.v[v] = !CLEAN && ((rst >> u) & 1) ? 0.f : fe;
+      for (int v = 0; v < VEC; v += 2) {
+        f32x2 f, i;
+        gates<T>(two(g[u], v), f, i);
+        const f32x2 e = add2(two(dh[u], v), two<VEC>(acc.v, v));
+        const f32x2 fe = mul2(f, e), px = two<VEC>(prev[u], v), xx = two(x[u], v);
+        set_two<VEC>(fx, v, mul2(i, e));
+        set_two<VEC>(fg, v, mul2(mul2(i, fe), add2(px, pair(-xx.x, -xx.y))));
+        set_two<VEC>(acc.v, v, fe);
       }
+      if (!CLEAN && ((rst >> u) & 1)) acc = vec_zero<float, VEC>();
       dx.put(fx);
       dg.put(fg);
       emit(u, dx, dg);
@@ -381,17 +392,22 @@ template <class T, int VEC, bool BWD, bool CLEAN>
 __device__ __forceinline__ void pair_tick(const Vec<T, VEC>& x, const Vec<T, VEC>& g, bool r,
                                           float* A, float* B) {
 #pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    float f, i;
-    gates<T>(g.get(v), f, i);
-    const bool gone = !CLEAN && drops(A[v]);
-    if (BWD) {
-      A[v] = !CLEAN && (r || gone) ? -0.f : A[v] * f;
-      B[v] = !CLEAN && drops(A[v]) ? B[v] : fmaf(A[v], x.get(v), B[v]);
-    } else {
-      B[v] = gone ? B[v] : fmaf(A[v], i * x.get(v), B[v]);
-      A[v] = !CLEAN && (r || gone) ? -0.f : A[v] * f;
+  for (int v = 0; v < VEC; v += 2) {
+    f32x2 f, i;
+    gates<T>(two(g, v), f, i);
+    const f32x2 P = two<VEC>(A, v), S = two<VEC>(B, v);
+    f32x2 nA = mul2(P, f);
+    if (!CLEAN) {
+      nA.x = r || drops(P.x) ? -0.f : nA.x;
+      nA.y = r || drops(P.y) ? -0.f : nA.y;
     }
+    f32x2 nB = BWD ? fma2(nA, two(x, v), S) : fma2(P, mul2(i, two(x, v)), S);
+    if (!CLEAN) {
+      nB.x = drops(BWD ? nA.x : P.x) ? S.x : nB.x;
+      nB.y = drops(BWD ? nA.y : P.y) ? S.y : nB.y;
+    }
+    set_two<VEC>(A, v, nA);
+    set_two<VEC>(B, v, nB);
   }
 }
 
