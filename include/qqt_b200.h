@@ -493,7 +493,7 @@ enum { QQT_F32 = 0, QQT_F16 = 1, QQT_BF16 = 2 };
 
 /* Layer norm of rows of d values (the norms of train/model.py:77-101 and
  * 140-153 on their own): y [rows][d] = (x - mean) rstd w + b (b optional);
- * mean, rstd [rows] (optional) are what the backward call reads. */
+ * mean, rstd [rows] (both or neither) are what the backward call reads. */
 int qqt_layernorm_forward(const void *x, int32_t dtype, int64_t rows, int64_t d, int64_t x_stride,
                           const float *w, const float *b, float eps, void *y, float *mean,
                           float *rstd, qqt_stream_t stream);

@@ -10,7 +10,7 @@
 //
 // Memory bound: 2 values moved per element forward, 3 backward (one read of x
 // and dy serves dx and the weight's gradient).  A row stays in the registers
-// of its team -- 8 lanes, a warp, or a block, by the row's number of 16-byte
+// of its team -- 8 to 32 lanes, or a block, by the row's number of 16-byte
 // vectors -- between the passes over it.  The backward teams walk over rows
 // and keep their columns' sums of dy xh and dy in registers; each block writes
 // one partial row and a second kernel adds the partials in a fixed order, so
@@ -684,22 +684,10 @@ struct LnPlan {
   int64_t blocks;
   LnRing ring;
 };
-static int ln_sms() {
-  static std::atomic<int> n{0};
-  int v = n.load();
-  if (v == 0) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0)
-      v = 148;
-    n.store(v);
-  }
-  return v;
-}
 static LnPlan ln_plan(int64_t rows, int64_t d, int vec, bool bwd) {
   LnPlan p{0, 0, kLnWarpThreads, 0, {0, 0, 0}};
   const int64_t nv = (d + vec - 1) / vec;
-  const int sms = ln_sms();
+  const int sms = sm_count();
   if (nv <= (vec == 8 ? 64 : 128)) {       // a team inside a warp
     const bool one = vec == 8 || nv <= 8;
     p.k = one ? 1 : 2;

@@ -265,6 +265,20 @@ static void launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t sme
   (void)cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
+// SMs of the current device (148 where it cannot be asked).
+static int sm_count() {
+  static std::atomic<int> n{0};
+  int v = n.load();
+  if (v == 0) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0)
+      v = 148;
+    n.store(v);
+  }
+  return v;
+}
+
 static inline bool dtype_ok(int32_t dtype) { return dtype >= QQT_F32 && dtype <= QQT_BF16; }
 
 // Runs f(T{}) with the element type of `dtype`.

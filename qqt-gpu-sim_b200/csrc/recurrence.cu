@@ -37,6 +37,7 @@ constexpr int kFwdBlocks = 6, kBwdBlocks = 4;
 // Channel walks wanted per SM before time is cut: 3072 against 1024 measured
 // 140 against 368 us at 65536 ticks x 1024 channels, and within 2 % of 4096.
 constexpr int64_t kRecWalks = 3072;
+constexpr int64_t kRecMostSegs = 32768;      // (a grid's second dimension ends at 65535)
 
 // f = sigmoid(g) and i = 1 - f = sigmoid(-g), each to a few units of its own
 // last place: e = exp(-g), f = 1 / (1 + e), i = e f.  e = 2^(-g log2 e) carries
@@ -544,19 +545,6 @@ __global__ void __launch_bounds__(1024) k_rec_join(RecArgs a, int segs) {
   }
 }
 
-static int rec_sms() {
-  static std::atomic<int> n{0};
-  int v = n.load();
-  if (v == 0) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0)
-      v = 148;
-    n.store(v);
-  }
-  return v;
-}
-
 // How time is cut: segments of at least 4 kRecU ticks, one where fewer than
 // three would come of it (the inputs are read twice then).
 struct RecCut {
@@ -564,7 +552,8 @@ struct RecCut {
   int segs;
 };
 static RecCut rec_cut(int64_t T, int64_t C) {
-  const int64_t want = (int64_t)rec_sms() * kRecWalks / C;
+  int64_t want = (int64_t)sm_count() * kRecWalks / C;
+  if (want > kRecMostSegs) want = kRecMostSegs;
   int64_t seg = want > 1 ? (T + want - 1) / want : T;
   if (seg < 4 * kRecU) seg = 4 * kRecU;
   seg = (seg + kRecU - 1) / kRecU * kRecU;
@@ -574,8 +563,10 @@ static RecCut rec_cut(int64_t T, int64_t C) {
 }
 
 static bool rec_sizes_ok(int64_t T, int64_t N, int64_t D) {
-  return T >= 0 && N >= 0 && D > 0 && T <= 0x7fffffffll && N <= 0x7fffffffll && D <= 0x7fffffffll &&
-         N * D <= 0x7fffff00ll;
+  return T >= 0 && N >= 0 && D > 0;
+}
+static bool rec_fits(int64_t T, int64_t N, int64_t D) {
+  return T <= 0x7fffffffll && N <= 0x7fffffffll && D <= 0x7fffffffll && N * D <= 0x7fffff00ll;
 }
 static bool seq_vec(const RecSeq& s, int64_t bytes, int64_t es) {
   return !s.p || (aligned_to(s.p, bytes) && (s.ts * es) % bytes == 0 && (s.ns * es) % bytes == 0);
@@ -632,7 +623,7 @@ extern "C" int64_t qqt_recurrence_chunks(int64_t T) {
 }
 
 extern "C" uint64_t qqt_recurrence_work_bytes(int64_t T, int64_t N, int64_t D) {
-  if (!rec_sizes_ok(T, N, D) || T == 0 || N == 0) return 0;
+  if (!rec_sizes_ok(T, N, D) || !rec_fits(T, N, D) || T == 0 || N == 0) return 0;
   const RecCut c = rec_cut(T, N * D);
   return c.segs > 1 ? (uint64_t)(c.segs - 1) * N * D * 8 + (uint64_t)c.segs * N * D * 4 : 0;
 }
@@ -642,6 +633,7 @@ extern "C" int qqt_recurrence_forward(const QqtSeq* x, const QqtSeq* gate, const
                                       int64_t D, const QqtSeq* h, float* h_last, float* carry,
                                       void* work, qqt_stream_t stream) {
   if (!x || !gate || !h || !dtype_ok(dtype) || !rec_sizes_ok(T, N, D)) return QQT_E_ARG;
+  if (!rec_fits(T, N, D)) return QQT_E_LIMIT;
   const int64_t C = N * D;
   if (C == 0) return QQT_OK;
   cudaStream_t st = (cudaStream_t)stream;
@@ -672,6 +664,7 @@ extern "C" int qqt_recurrence_step(const void* x, int64_t x_stride, const void* 
                                    const float* state, int32_t dtype, int64_t N, int64_t D, void* h,
                                    float* state_out, qqt_stream_t stream) {
   if (!dtype_ok(dtype) || !rec_sizes_ok(1, N, D)) return QQT_E_ARG;
+  if (!rec_fits(1, N, D)) return QQT_E_LIMIT;
   if (N == 0) return QQT_OK;
   if (!x || !gate || !state || !h || !state_out) return QQT_E_ARG;
   RecArgs a{};
@@ -701,6 +694,7 @@ extern "C" int qqt_recurrence_backward(const QqtSeq* dh, const float* dh_last, c
                                        const QqtSeq* dx, const QqtSeq* dgate, float* dh0, void* work,
                                        qqt_stream_t stream) {
   if (!x || !gate || !dx || !dgate || !dtype_ok(dtype) || !rec_sizes_ok(T, N, D)) return QQT_E_ARG;
+  if (!rec_fits(T, N, D)) return QQT_E_LIMIT;
   const int64_t C = N * D;
   if (C == 0) return QQT_OK;
   cudaStream_t st = (cudaStream_t)stream;

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from . import _capi as capi
 
@@ -109,6 +110,7 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, mean, rstd, weight = ctx.saved_tensors
         nx, nw, nb = ctx.needs_input_grad[:3]

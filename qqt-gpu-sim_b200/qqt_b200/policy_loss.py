@@ -21,6 +21,7 @@ loss and gradient in one pass over the logits, for `logits.backward(dlogits)`.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _capi as capi
 
@@ -171,6 +172,7 @@ class _PolicyLoss(torch.autograd.Function):
         return loss, stats
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dloss, _):
         logits, actions, old_logp, advantage, ref_logp, legal, mask = ctx.saved_tensors
         heads, clip, kl_coef, entropy_coef = ctx.opts

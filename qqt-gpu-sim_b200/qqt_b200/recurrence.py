@@ -20,6 +20,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _capi as capi
 
@@ -144,6 +145,7 @@ class _Recurrence(torch.autograd.Function):
         return h, last
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dh, dh_last):
         x, gate, saved, reset = ctx.saved_tensors
         dx, dg, dh0 = gated_recurrence_backward(dh, dh_last, x, gate, saved, reset)

@@ -172,6 +172,33 @@ def test_extreme_gates():
 
 
 @gpu
+def test_millions_of_ticks():
+    """One channel over 2.2 million ticks: more segments of the least length
+    than a grid's second dimension holds.  The reference walks the ticks on
+    the host in 64 bits."""
+    _need_cuda()
+    t = 2200003
+    x, g, h0, reset, dh, dl = _data(t, 1, 1, torch.float32, 77)
+    h, last, saved = gated_recurrence_forward(x, g, h0, reset)
+    dx, dg, dh0 = gated_recurrence_backward(dh, dl, x, g, saved, reset)
+    xs, fs = x.double().flatten().tolist(), torch.sigmoid(g.double()).flatten().tolist()
+    rs, ds = reset.flatten().tolist(), dh.double().flatten().tolist()
+    s, hs, es, e = h0.item(), [], [0.0] * t, dl.item()
+    for k in range(t):
+        s = fs[k] * (0.0 if rs[k] else s) + (1 - fs[k]) * xs[k]
+        hs.append(s)
+    for k in range(t - 1, -1, -1):
+        e += ds[k]
+        es[k] = (1 - fs[k]) * e
+        e = 0.0 if rs[k] else fs[k] * e
+    m = max(x.abs().max().item(), abs(h0.item()))
+    _close(h.flatten().cpu(), torch.tensor(hs, dtype=torch.float64), m)
+    want = torch.tensor(es, dtype=torch.float64)
+    _close(dx.flatten().cpu(), want, 4 * max(want.abs().max().item(), dh.abs().max().item()))
+    assert abs(dh0.item() - e) <= C * 4 * max(abs(e), dh.abs().max().item())
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 def test_ticks_equal_the_sequence(dtype):
     """Acting tick by tick, in place, gives the sequence's states: the same
@@ -312,6 +339,9 @@ def test_c_entry_refusals():
     assert f(r(s), r(s), None, P, 0, -4, 2, 8, r(s), P, P, P, None) == 1
     assert f(r(null), r(s), None, P, 0, 4, 2, 8, r(s), P, P, P, None) == 1
     assert f(r(s), r(s), None, P, 0, 4, 0, 8, r(s), P, P, P, None) == 0
+    assert f(r(s), r(s), None, P, 0, 4, 1 << 30, 8, r(s), P, P, P, None) == 3
+    assert L.qqt_recurrence_step(P, 8, P, 8, None, 0, None, 0, 2, 8, P, P, None) == 1
+    assert L.qqt_recurrence_step(P, 8, P, 8, None, 0, P, 4, 2, 8, P, P, None) == 1
     b = L.qqt_recurrence_backward
     assert b(r(s), P, r(s), r(s), None, None, 0, 4, 2, 8, r(s), r(s), P, P, None) == 1
     assert b(r(s), P, r(s), r(s), None, P, 0, 4, 2, 8, None, r(s), P, P, None) == 1
