@@ -17,6 +17,15 @@
 // there are no atomics and results repeat.  Rows that are not made of whole
 // vectors go element by element; rows too long for a block's registers are
 // read again for every pass.
+//
+// Measured on a B200 (its copy bandwidth is 6.55 TB/s):
+//   1048576 x 128 f32    forward 171 us, 6.3 TB/s; backward 252 us, 6.4 TB/s
+//   5632 x 10816 f16     forward 55 us, 4.4 TB/s; backward 110 us, 3.3 TB/s
+//   11267 x 2704 bf16    forward 30 us, 4.1 TB/s; backward 59 us, 3.1 TB/s
+// Short rows are bound by memory.  Rows of a block, 16-bit ones above all, are
+// bound by what each row costs its block beside the memory: two exchanges
+// across the warps forward and one of two sums backward, with 24 warps an SM
+// in all (the backward pass holds 32 sums and 16 weights a thread).
 
 #include "ops_common.cuh"
 

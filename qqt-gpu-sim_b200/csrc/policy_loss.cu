@@ -16,14 +16,26 @@
 // By the number of logits V of a row:
 //  * up to kPlSmall: a thread per row, rows staged in shared memory so that
 //    loads and stores stay contiguous (the policy's 5 + 2 logits);
-//  * else a warp or a block per row: one pass keeps a running maximum and the
-//    two sums, rescaled when the maximum grows; a second pass, whose reads
-//    come from L2, writes the gradient.  Bound by the exponentials (two per
-//    logit on the special-function unit, 16 lanes a cycle and SM) and by
+//  * else 8 lanes, a warp or a block per row: one pass keeps a running maximum
+//    and the two sums, rescaled when the maximum grows; a second pass, whose
+//    reads come from L2, writes the gradient.  Bound by the exponentials (two
+//    per logit on the special-function unit, 16 lanes a cycle and SM) and by
 //    memory at much the same time; the other arithmetic runs in pairs
 //    (f32x2).  A row may begin at any address: vectors are put together from
 //    two aligned ones, so the element a thread works on, and with it every
 //    sum, does not depend on alignment.
+//
+// Measured on a B200 (copy bandwidth 6.55 TB/s):
+//   8192 x 32000 bf16     loss and gradient 228 us, 4.6 TB/s (two values a
+//                         logit); scores 113 us, 4.6 TB/s
+//   2047 x 100003 f16     scores 107 us, 3.8 TB/s (rows at any alignment)
+//   4096 x 32000 f32      loss and gradient 212 us, 4.9 TB/s
+//   1048576 rows of 5 + 2 f32 logits, masked: 47 us, about 950 instructions a
+//                         row (logarithms, exponentials and quotients of both
+//                         heads and of the loss), 2.1 TB/s
+// The vocabulary rows execute about 9 instructions a logit and pass, 60 % of
+// the issue slots, 57 % of the special-function unit and 70 % of the memory
+// bandwidth at once; no one of them is full.
 
 #include "ops_common.cuh"
 
