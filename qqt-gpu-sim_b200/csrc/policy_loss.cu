@@ -30,9 +30,10 @@
 //                         logit); scores 113 us, 4.6 TB/s
 //   2047 x 100003 f16     scores 107 us, 3.8 TB/s (rows at any alignment)
 //   4096 x 32000 f32      loss and gradient 212 us, 4.9 TB/s
-//   1048576 rows of 5 + 2 f32 logits, masked: 47 us, about 950 instructions a
-//                         row (logarithms, exponentials and quotients of both
-//                         heads and of the loss), 2.1 TB/s
+//   1048576 rows of 5 + 2 f32 logits, masked: 40 us, 2.5 TB/s, of which the
+//                         row kernel takes 3/4 of the issue slots (800
+//                         instructions a row: logarithms, exponentials and
+//                         quotients of both heads and of the loss)
 // The vocabulary rows execute about 9 instructions a logit and pass, 60 % of
 // the issue slots, 57 % of the special-function unit and 70 % of the memory
 // bandwidth at once; no one of them is full.
@@ -62,7 +63,7 @@ struct HeadStat {
 __device__ __forceinline__ float rows_counted(const QqtPolicyLoss& a, const int* counts) {
   if (!a.mask) return fmaxf((float)a.rows, 1.f);
   const int l = lane_id();
-  const int n = warp_sum(counts[l] + counts[l + 32]);
+  const int n = __reduce_add_sync(QQT_FULL, counts[l] + counts[l + 32]);
   return fmaxf((float)n, 1.f);
 }
 
@@ -137,7 +138,7 @@ __device__ __forceinline__ RowLoss loss_of(const QqtPolicyLoss& a, const RowIn& 
 // log p of the head's action.  any: some category is legal.
 __device__ __forceinline__ float finish_head(HeadStat& k, bool any, float s, float log_s, float e,
                                              float t_act, bool act_ok) {
-  k.inv_s = any ? 1.f / s : 0.f;
+  k.inv_s = any ? rcp_approx(s) : 0.f;      // s >= 1 or NaN
   k.log_s = log_s;
   k.ent = any ? log_s - e * k.inv_s : 0.f;
   k.t_act = t_act;
@@ -159,28 +160,61 @@ __device__ __forceinline__ float action_grad(const HeadStat& k, float g, float c
 
 // ---------------------------------------------------- few logits: thread per row
 
-// Copies n elements from p to floats, or floats to p, by 16-byte vectors; p on
-// 16 bytes.
+// Copies n elements from p to floats, minus infinity where legal (optional) is
+// 0, or floats to p, by 16-byte vectors; p and legal on 16 bytes.  Rows of V
+// elements are V floats apart, V + 1 where 4 divides V; a vector then lies in
+// one row.
 template <class T>
-__device__ __forceinline__ void stage_in(const T* p, int n, float* to) {
-  constexpr int VEC = 16 / sizeof(T);
-  for (int i = threadIdx.x * VEC; i + VEC <= n; i += kPlSmallRows * VEC) {
-    const Vec<T, VEC> x = ld_vec<T, VEC>(p + i);
-#pragma unroll
-    for (int v = 0; v < VEC; v += 4)
-      *reinterpret_cast<float4*>(to + i + v) =
-          make_float4(x.get(v), x.get(v + 1), x.get(v + 2), x.get(v + 3));
-  }
-  const int i = n / VEC * VEC + threadIdx.x;
-  if (i < n) to[i] = to_f(p[i]);
+__device__ __forceinline__ bool run_fits(int V) {
+  return (V & 3) != 0 || V % (16 / (int)sizeof(T)) == 0;
 }
 template <class T>
-__device__ __forceinline__ void stage_out(T* p, int n, const float* from) {
+__device__ __forceinline__ void stage_in(const T* p, const uint8_t* legal, int n, int V, float* to) {
   constexpr int VEC = 16 / sizeof(T);
+  const bool padded = (V & 3) == 0;
   for (int i = threadIdx.x * VEC; i + VEC <= n; i += kPlSmallRows * VEC) {
+    const Vec<T, VEC> x = ld_vec<T, VEC>(p + i);
     float f[VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) f[v] = from[i + v];
+    for (int v = 0; v < VEC; ++v) f[v] = x.get(v);
+    if (legal) {
+#pragma unroll
+      for (int v = 0; v < VEC; v += 4) {
+        const uchar4 l = *reinterpret_cast<const uchar4*>(legal + i + v);
+        f[v] = l.x ? f[v] : -INFINITY;
+        f[v + 1] = l.y ? f[v + 1] : -INFINITY;
+        f[v + 2] = l.z ? f[v + 2] : -INFINITY;
+        f[v + 3] = l.w ? f[v + 3] : -INFINITY;
+      }
+    }
+    if (padded) {
+      float* q = to + i + i / V;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) q[v] = f[v];
+    } else {
+#pragma unroll
+      for (int v = 0; v < VEC; v += 4)
+        *reinterpret_cast<float4*>(to + i + v) = make_float4(f[v], f[v + 1], f[v + 2], f[v + 3]);
+    }
+  }
+  const int i = n / VEC * VEC + threadIdx.x;      // (none where a vector lies in one row)
+  if (i < n) to[i] = legal && !legal[i] ? -INFINITY : to_f(p[i]);
+}
+template <class T>
+__device__ __forceinline__ void stage_out(T* p, int n, int V, const float* from) {
+  constexpr int VEC = 16 / sizeof(T);
+  const bool padded = (V & 3) == 0;
+  for (int i = threadIdx.x * VEC; i + VEC <= n; i += kPlSmallRows * VEC) {
+    float f[VEC];
+    if (padded) {
+      const float* q = from + i + i / V;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) f[v] = q[v];
+    } else {
+#pragma unroll
+      for (int v = 0; v < VEC; v += 4)
+        *reinterpret_cast<float4*>(f + v) = *reinterpret_cast<const float4*>(from + i + v);
+    }
     Vec<T, VEC> x;
     x.put(f);
     st_vec(p + i, x);
@@ -189,19 +223,36 @@ __device__ __forceinline__ void stage_out(T* p, int n, const float* from) {
   if (i < n) p[i] = from_f<T>(from[i]);
 }
 
-// Rows are V | 1 floats apart in shared memory: threads on rows hit different
-// banks.  Where V is odd and the rows lie one after the other, the block's
-// rows are one run of memory that is copied as it is.
+// The warp's sums of v[0] .. v[3], of v[l & 3] in lane l: two exchanges leave
+// a value a lane, three more add the lanes that hold the same one.
+__device__ __forceinline__ float warp_sum4(const float* v) {
+  const int l = lane_id();
+  const bool odd = l & 1, hi = l & 2;
+  const float a = (odd ? v[1] : v[0]) + __shfl_xor_sync(QQT_FULL, odd ? v[0] : v[1], 1);
+  const float b = (odd ? v[3] : v[2]) + __shfl_xor_sync(QQT_FULL, odd ? v[2] : v[3], 1);
+  float x = (hi ? b : a) + __shfl_xor_sync(QQT_FULL, hi ? a : b, 2);
+#pragma unroll
+  for (int o = 4; o < 32; o *= 2) x += __shfl_xor_sync(QQT_FULL, x, o);
+  return x;
+}
+
+// Rows are V floats apart in shared memory, V + 1 where 4 divides V: at most
+// two threads on rows hit the same bank.  Where the rows lie one after the
+// other, the block's rows are one run of memory; it is copied by vectors, as it
+// is or, where 4 divides V, each vector to its row (1048576 rows of 6: 31 us,
+// 46 by elements).  Bound by the issue of instructions, so eight blocks an SM
+// and 32 registers are better than six and 40 (36.4 against 39.5 us for rows
+// of 5 + 2).
 // NH: the number of heads where it is 1 or 2 (what is kept per head then stays
 // in registers), QQT_MAX_HEADS for any.
 template <class T, int NH>
-__global__ void __launch_bounds__(kPlSmallRows)
+__global__ void __launch_bounds__(kPlSmallRows, 8)
     k_pl_small(QqtPolicyLoss a, int V, const int* __restrict__ counts, float* __restrict__ part,
                int one_block) {
   extern __shared__ __align__(16) float zs[];
   __shared__ float buf[4][32];
   __shared__ int n_mask;
-  const int pitch = V | 1;
+  const int pitch = V & 3 ? V : V + 1;
   const int64_t r0 = (int64_t)blockIdx.x * kPlSmallRows;
   const int n = a.rows - r0 < kPlSmallRows ? (int)(a.rows - r0) : kPlSmallRows;
   const bool loss = a.old_logp != nullptr;
@@ -221,15 +272,18 @@ __global__ void __launch_bounds__(kPlSmallRows)
     mine = warp_sum(count_bytes(a.mask, threadIdx.x, kPlSmallRows, a.rows));
   }
   const T* zp = (const T*)a.logits + r0 * a.row_stride;
-  uint8_t* legal = (uint8_t*)(zs + kPlSmallRows * pitch);
-  if ((V & 1) && a.row_stride == V && ((uintptr_t)zp & 15) == 0) {
-    stage_in(zp, n * V, zs);
+  const uint8_t* lp = a.legal ? a.legal + r0 * a.legal_stride : nullptr;
+  if (a.row_stride == V && (!lp || a.legal_stride == V) && run_fits<T>(V) &&
+      (((uintptr_t)zp | (uintptr_t)lp) & 15) == 0) {
+    stage_in(zp, lp, n * V, V, zs);
   } else {
     int q = threadIdx.x / V, col = threadIdx.x % V;
     const int dr = kPlSmallRows / V, dc = kPlSmallRows % V;
 #pragma unroll 4
     for (int i = threadIdx.x; i < n * V; i += kPlSmallRows) {
-      zs[q * pitch + col] = to_f(zp[q * a.row_stride + col]);
+      zs[q * pitch + col] = lp && !lp[q * a.legal_stride + col]
+                                ? -INFINITY
+                                : to_f(zp[q * a.row_stride + col]);
       q += dr;
       col += dc;
       if (col >= V) {
@@ -238,32 +292,9 @@ __global__ void __launch_bounds__(kPlSmallRows)
       }
     }
   }
-  if (a.legal) {
-    const uint8_t* lp = a.legal + r0 * a.legal_stride;
-    if (a.legal_stride == V && ((uintptr_t)lp & 15) == 0) {
-      for (int i = threadIdx.x * 16; i + 16 <= n * V; i += kPlSmallRows * 16)
-        *reinterpret_cast<uint4*>(legal + i) = *reinterpret_cast<const uint4*>(lp + i);
-      const int i = n * V / 16 * 16 + threadIdx.x;
-      if (i < n * V) legal[i] = lp[i];
-    } else {
-      int q = threadIdx.x / V, col = threadIdx.x % V;
-      const int dr = kPlSmallRows / V, dc = kPlSmallRows % V;
-#pragma unroll 4
-      for (int i = threadIdx.x; i < n * V; i += kPlSmallRows) {
-        legal[i] = lp[q * a.legal_stride + col];
-        q += dr;
-        col += dc;
-        if (col >= V) {
-          col -= V;
-          ++q;
-        }
-      }
-    }
-  }
   __syncthreads();
   if (fold && lane_id() == 0 && mine) atomicAdd(&n_mask, mine);   // whole numbers: any order
   float* z = zs + threadIdx.x * pitch;
-  const uint8_t* lg = legal + threadIdx.x * V;
   HeadStat hs[NH];
   float ms[NH];
   float logp = 0.f, ent = 0.f;
@@ -276,10 +307,8 @@ __global__ void __launch_bounds__(kPlSmallRows)
       const bool in = act >= 0 && act < w;
       if (!in) flag_error(QQT_DEV_BAD_ACTION);
       float m = -INFINITY, s = 0.f, e = 0.f;
-      for (int j = at; j < at + w; ++j) {
-        if (a.legal && !lg[j]) z[j] = -INFINITY;
-        m = max_nan(m, z[j]);
-      }
+#pragma unroll 4
+      for (int j = at; j < at + w; ++j) m = max_nan(m, z[j]);
 #pragma unroll 4
       for (int j = at; j < at + w; ++j) {
         const float t = max_nan(z[j] - m, kFloor), x = ex2_approx(t * kLog2e);
@@ -307,11 +336,8 @@ __global__ void __launch_bounds__(kPlSmallRows)
   const RowLoss l = loss_of(a, row, logp, live);
   if (a.stats) {
     const float v[4] = {l.pg, l.kl, live ? ent : 0.f, l.clip};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float x = warp_sum_f(v[k]);
-      if (lane_id() == 0) buf[k][warp_id()] = x;
-    }
+    const float x = warp_sum4(v);
+    if (lane_id() < 4) buf[lane_id()][warp_id()] = x;
     __syncthreads();
     if (warp_id() == 0) {
       float sum[4];
@@ -352,8 +378,8 @@ __global__ void __launch_bounds__(kPlSmallRows)
   }
   __syncthreads();
   T* op = (T*)a.dlogits + r0 * a.dlogits_stride;
-  if ((V & 1) && a.dlogits_stride == V && ((uintptr_t)op & 15) == 0) {
-    stage_out(op, n * V, zs);
+  if (a.dlogits_stride == V && run_fits<T>(V) && ((uintptr_t)op & 15) == 0) {
+    stage_out(op, n * V, V, zs);
   } else {
     int q = threadIdx.x / V, col = threadIdx.x % V;
     const int dr = kPlSmallRows / V, dc = kPlSmallRows % V;
@@ -976,7 +1002,7 @@ extern "C" int qqt_policy_loss(const QqtPolicyLoss* a, qqt_stream_t stream) {
     with_dtype(a->dtype, [&](auto t) {
       using T = decltype(t);
       if (small) {
-        const size_t smem = (size_t)kPlSmallRows * ((v | 1) * 4 + (a->legal ? v : 0));
+        const size_t smem = (size_t)kPlSmallRows * (v & 3 ? v : v + 1) * 4;
         auto run = [&](auto nh) {
           launch_early(k_pl_small<T, decltype(nh)::value>, dim3(blocks), dim3(kPlSmallRows), smem, st,
                     counts != nullptr, args, (int)v, counts, part, (int)one);
