@@ -37,16 +37,17 @@
 namespace qqt {
 
 constexpr int kRecU = 8;                     // ticks a thread holds, and between saved states
-constexpr int kSeqThreads = 128;
+constexpr int kSeqThreads = 128;             // most threads of a block
 // Blocks of an SM that the registers are cut for.  16-bit forward walks take 4
 // channels a thread, backward ones 2: 8 ticks of 4 channels' states and
 // operands do not fit 128 registers (213 against 340 us measured at 128 ticks
 // x 5632 x 128).
 constexpr int kFwdBlocks = 6, kBwdBlocks = 4;
-// Channel walks wanted per SM before time is cut.  At 65536 ticks x 1024
-// channels of bf16, 8, 16, 24 and 32 x 128 measured 164, 117, 109 and 120 us
-// forward, 185, 171, 174 and 182 us backward.
-constexpr int64_t kRecWalks = 24 * 128;
+// Segments are cut so that all walks run at once forward, in two rounds
+// backward, where a second round fills the SMs that are done (16384 x 4 x 512:
+// f32 forward 96 us against 105 in two rounds and 107 in three; bf16 backward
+// 96 in two, 102 in one, 103 in three).
+constexpr int kFwdRounds = 1, kBwdRounds = 2;
 constexpr int64_t kRecMostSegs = 32768;      // (a grid's second dimension ends at 65535)
 
 // f = sigmoid(g) and i = 1 - f = sigmoid(-g), each to a few units of its own
@@ -200,7 +201,7 @@ __device__ __forceinline__ void load_ticks(const T* p, int64_t ts, int n, Vec<T,
 
 template <class T, int VEC>
 __global__ void __launch_bounds__(kSeqThreads, kFwdBlocks) k_rec_seq_fwd(RecArgs a) {
-  const RecPlace p = rec_place<VEC>(a, (blockIdx.x * kSeqThreads + threadIdx.x) * VEC);
+  const RecPlace p = rec_place<VEC>(a, (blockIdx.x * blockDim.x + threadIdx.x) * VEC);
   const int64_t first = blockIdx.y * a.seg;
   const int64_t ticks = a.nT - first < a.seg ? a.nT - first : a.seg;
   const T *xp = at<T>(a.x, p, first), *gp = at<T>(a.g, p, first);
@@ -310,7 +311,7 @@ __device__ __forceinline__ void backward_ticks(const Vec<T, VEC>* x, const Vec<T
 
 template <class T, int VEC>
 __global__ void __launch_bounds__(kSeqThreads, kBwdBlocks) k_rec_seq_bwd(RecArgs a) {
-  const RecPlace p = rec_place<VEC>(a, (blockIdx.x * kSeqThreads + threadIdx.x) * VEC);
+  const RecPlace p = rec_place<VEC>(a, (blockIdx.x * blockDim.x + threadIdx.x) * VEC);
   const int64_t first = blockIdx.y * a.seg;
   const int64_t end = first + a.seg < a.nT ? first + a.seg : a.nT;
   const int64_t full = end / kRecU;    // (batches are counted from tick 0)
@@ -424,7 +425,7 @@ __device__ __forceinline__ void pair_tick(const Vec<T, VEC>& x, const Vec<T, VEC
 
 template <class T, int VEC, bool BWD>
 __global__ void __launch_bounds__(kSeqThreads, kFwdBlocks) k_rec_sum(RecArgs a) {
-  const RecPlace p = rec_place<VEC>(a, (blockIdx.x * kSeqThreads + threadIdx.x) * VEC);
+  const RecPlace p = rec_place<VEC>(a, (blockIdx.x * blockDim.x + threadIdx.x) * VEC);
   // the segments that some other one follows in the scan's direction
   const int64_t first = (blockIdx.y + (BWD ? 1 : 0)) * a.seg;
   const int64_t end = first + a.seg < a.nT ? first + a.seg : a.nT;
@@ -557,20 +558,27 @@ __global__ void __launch_bounds__(1024) k_rec_join(RecArgs a, int segs) {
 
 // How time is cut: segments of at least 4 kRecU ticks (8 measured 17 against
 // 12 us at 512 ticks x 8 x 256), one where fewer than three would come of it
-// (the inputs are read twice then).
+// (the inputs are read twice then).  It goes by the sizes and the type, not by
+// alignment, and so does the order of the sums.
 struct RecCut {
   int64_t seg;
-  int segs;
+  int segs, threads;
 };
-static RecCut rec_cut(int64_t T, int64_t C) {
-  int64_t want = (int64_t)sm_count() * kRecWalks / C;
+static RecCut rec_cut(int64_t T, int64_t C, int64_t D, int es, bool bwd) {
+  const int v = D % 2 ? 1 : D % 4 == 0 && es == 2 && !bwd ? 4 : 2;
+  const int64_t walks = C / v;
+  const int threads = walks < kSeqThreads ? (int)(walks + 31) / 32 * 32 : kSeqThreads;
+  const int64_t row = (walks + threads - 1) / threads;
+  const int at_once = (bwd ? kBwdBlocks * kBwdRounds : kFwdBlocks * kFwdRounds) *
+                      (kSeqThreads / threads);
+  int64_t want = (int64_t)sm_count() * at_once / row;
   if (want > kRecMostSegs) want = kRecMostSegs;
   int64_t seg = want > 1 ? (T + want - 1) / want : T;
   if (seg < 4 * kRecU) seg = 4 * kRecU;
   seg = (seg + kRecU - 1) / kRecU * kRecU;
   const int64_t segs = (T + seg - 1) / seg;
-  if (segs < 3) return {(T + kRecU - 1) / kRecU * kRecU, 1};
-  return {seg, (int)segs};
+  if (segs < 3) return {(T + kRecU - 1) / kRecU * kRecU, 1, threads};
+  return {seg, (int)segs, threads};
 }
 
 static bool rec_sizes_ok(int64_t T, int64_t N, int64_t D) {
@@ -588,21 +596,22 @@ static RecSeq rec_seq(const QqtSeq* s) {
 
 template <class T, int VEC, bool BWD>
 static int rec_walk(RecArgs a, void* work, cudaStream_t st) {
-  const unsigned blocks = (a.nC / VEC + kSeqThreads - 1) / kSeqThreads;
-  const RecCut cut = rec_cut(a.nT, a.nC);
+  const RecCut cut = rec_cut(a.nT, a.nC, a.nD, sizeof(T), BWD);
+  const dim3 threads(cut.threads);
+  const unsigned blocks = (a.nC / VEC + cut.threads - 1) / cut.threads;
   a.seg = cut.seg;
   if (cut.segs > 1) {
     if (!work) return QQT_E_ARG;
     a.pair = (float2*)work;
     a.enters = (float*)(a.pair + (int64_t)(cut.segs - 1) * a.nC);
-    k_rec_sum<T, VEC, BWD><<<dim3(blocks, cut.segs - 1), kSeqThreads, 0, st>>>(a);
+    k_rec_sum<T, VEC, BWD><<<dim3(blocks, cut.segs - 1), threads, 0, st>>>(a);
     launch_early(k_rec_join<BWD>, dim3((a.nC + 31) / 32), dim3(1024), 0, st, true, a, cut.segs);
   }
   const bool early = cut.segs > 1;
   if (BWD)
-    launch_early(k_rec_seq_bwd<T, VEC>, dim3(blocks, cut.segs), dim3(kSeqThreads), 0, st, early, a);
+    launch_early(k_rec_seq_bwd<T, VEC>, dim3(blocks, cut.segs), threads, 0, st, early, a);
   else
-    launch_early(k_rec_seq_fwd<T, VEC>, dim3(blocks, cut.segs), dim3(kSeqThreads), 0, st, early, a);
+    launch_early(k_rec_seq_fwd<T, VEC>, dim3(blocks, cut.segs), threads, 0, st, early, a);
   return launch_status();
 }
 
@@ -635,8 +644,12 @@ extern "C" int64_t qqt_recurrence_chunks(int64_t T) {
 
 extern "C" uint64_t qqt_recurrence_work_bytes(int64_t T, int64_t N, int64_t D) {
   if (!rec_sizes_ok(T, N, D) || !rec_fits(T, N, D) || T == 0 || N == 0) return 0;
-  const RecCut c = rec_cut(T, N * D);
-  return c.segs > 1 ? (uint64_t)(c.segs - 1) * N * D * 8 + (uint64_t)c.segs * N * D * 4 : 0;
+  int segs = 1;
+  for (int k = 0; k < 4; ++k) {          // of either direction and any type
+    const RecCut c = rec_cut(T, N * D, D, k & 1 ? 2 : 4, k >> 1);
+    if (c.segs > segs) segs = c.segs;
+  }
+  return segs > 1 ? (uint64_t)(segs - 1) * N * D * 8 + (uint64_t)segs * N * D * 4 : 0;
 }
 
 extern "C" int qqt_recurrence_forward(const QqtSeq* x, const QqtSeq* gate, const QqtSeq* reset,
