@@ -66,8 +66,18 @@ __device__ __forceinline__ void team_sum(float* v, float (*buf)[N][32], int& tur
 #pragma unroll
       for (int k = 0; k < N; ++k) b[k][warp_id()] = v[k];
     __syncthreads();
+    const int l = nw <= 8 ? lane_id() & 7 : lane_id();
 #pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = warp_sum_f(lane_id() < nw ? b[k][lane_id()] : 0.f);
+    for (int k = 0; k < N; ++k) v[k] = l < nw ? b[k][l] : 0.f;
+    if (nw <= 8) {
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(QQT_FULL, v[k], o);
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[k] = warp_sum_f(v[k]);
+    }
   }
 }
 
@@ -94,36 +104,67 @@ __device__ __forceinline__ LnTeam ln_team() {
   return t;
 }
 
-// Vector j of a row of d values.  Without WHOLE the row may begin anywhere and
-// end inside a vector: it goes element by element, zeros past its end.
-template <class T, int VEC, bool WHOLE>
-__device__ __forceinline__ Vec<T, VEC> ln_get(const T* p, int j, int d) {
-  if constexpr (WHOLE) {
+// How a row of d values lies in its team's registers.  WHOLE: vectors of VEC
+// values, each one access.  SINGLE: the same vectors value by value, where some
+// address is not on 16 bytes; the sums are WHOLE's.  SPREAD: where d is not
+// made of vectors, the values j, j + step, ... of lane j, so that the lanes of
+// an access lie side by side (3000 x 7001 f16, forward: 56 us, 93 by runs of 8
+// values a lane; 20000 x 1351 bf16: 55 and 100).  Values past the row's end are 0.
+enum LnMode { SINGLE, WHOLE, SPREAD };
+template <int VEC, LnMode M>
+__device__ __forceinline__ int ln_col(int j, int v, int step) {      // of value v of vector j
+  return M == SPREAD ? j + v * step : j * VEC + v;
+}
+// The next vector's j, and the end of j.
+template <int VEC, LnMode M>
+__device__ __forceinline__ int ln_next(int step) {
+  return M == SPREAD ? VEC * step : step;
+}
+template <int VEC, LnMode M>
+__device__ __forceinline__ int ln_end(int d) {
+  return M == SPREAD ? d : (d + VEC - 1) / VEC;
+}
+template <class T, int VEC, LnMode M>
+__device__ __forceinline__ Vec<T, VEC> ln_get(const T* p, int j, int step, int d) {
+  if constexpr (M == WHOLE) {
     return ld_vec<T, VEC>(p + (int64_t)j * VEC);
   } else {
-    float f[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) f[v] = j * VEC + v < d ? to_f(p[(int64_t)j * VEC + v]) : 0.f;
     Vec<T, VEC> r;
-    r.put(f);
+    T e[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      const int c = ln_col<VEC, M>(j, v, step);
+      e[v] = M == SINGLE || c < d ? p[c] : from_f<T>(0.f);
+    }
+    if constexpr (sizeof(T) == 4) {
+      r.put(e);
+    } else {
+      uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+      for (int v = 0; v < VEC; v += 2)
+        w[v / 2] = __byte_perm(*reinterpret_cast<const unsigned short*>(&e[v]),
+                               *reinterpret_cast<const unsigned short*>(&e[v + 1]), 0x5410);
+    }
     return r;
   }
 }
-template <class T, int VEC, bool WHOLE>
-__device__ __forceinline__ void ln_put(T* p, int j, int d, const float* f) {
-  if constexpr (WHOLE) {
+template <class T, int VEC, LnMode M>
+__device__ __forceinline__ void ln_put(T* p, int j, int step, int d, const float* f) {
+  if constexpr (M == WHOLE) {
     Vec<T, VEC> r;
     r.put(f);
     st_vec(p + (int64_t)j * VEC, r);
   } else {
 #pragma unroll
-    for (int v = 0; v < VEC; ++v)
-      if (j * VEC + v < d) p[(int64_t)j * VEC + v] = from_f<T>(f[v]);
+    for (int v = 0; v < VEC; ++v) {
+      const int c = ln_col<VEC, M>(j, v, step);
+      if (M == SINGLE || c < d) p[c] = from_f<T>(f[v]);
+    }
   }
 }
-template <int VEC, bool WHOLE>
-__device__ __forceinline__ Vec<float, VEC> ln_param(const float* p, int j, int d) {
-  if constexpr (WHOLE && VEC == 8) {
+template <int VEC, LnMode M>
+__device__ __forceinline__ Vec<float, VEC> ln_param(const float* p, int j, int step, int d) {
+  if constexpr (M == WHOLE && VEC == 8) {
     Vec<float, VEC> r;
     const float4 lo = *reinterpret_cast<const float4*>(p + j * 8);
     const float4 hi = *reinterpret_cast<const float4*>(p + j * 8 + 4);
@@ -131,18 +172,30 @@ __device__ __forceinline__ Vec<float, VEC> ln_param(const float* p, int j, int d
     r.put(f);
     return r;
   } else {
-    return ln_get<float, VEC, WHOLE>(p, j, d);
+    return ln_get<float, VEC, M>(p, j, step, d);
   }
 }
-template <class T, int VEC, int K, bool WHOLE>
-__device__ __forceinline__ void ln_load(const T* p, const LnTeam& t, int nv, int d, bool on,
+template <class T, int VEC, int K, LnMode M>
+__device__ __forceinline__ void ln_load(const T* p, const LnTeam& t, int d, bool on,
                                         Vec<T, VEC>* out) {
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int j = t.j + k * t.step;
-    out[k] = on && j < nv ? ln_get<T, VEC, WHOLE>(p, j, d) : vec_zero<T, VEC>();
+    const int j = t.j + k * ln_next<VEC, M>(t.step);
+    out[k] = on && j < ln_end<VEC, M>(d) ? ln_get<T, VEC, M>(p, j, t.step, d) : vec_zero<T, VEC>();
   }
 }
+// The parameters of a thread's columns where they stay in registers (KEEP).
+template <int VEC, int K, LnMode M, bool KEEP>
+struct LnParams {
+  Vec<float, VEC> r[KEEP ? K : 1];
+  __device__ __forceinline__ void read(const float* p, const LnTeam& t, int d) {
+    if constexpr (KEEP) ln_load<float, VEC, K, M>(p, t, d, p != nullptr, r);
+  }
+  __device__ __forceinline__ Vec<float, VEC> get(const float* p, int k, int j, int step, int d) const {
+    if constexpr (KEEP) return r[k];
+    return ln_param<VEC, M>(p, j, step, d);
+  }
+};
 // The steps of both passes on one vector, two values at a time.
 // Sums f, and its square once it is centred.
 template <int VEC>
@@ -175,8 +228,8 @@ __device__ __forceinline__ void ln_scale(const float* c, float rs, const Vec<flo
   }
 }
 // Backward, first half: the sums of dy xh and dy (columns), of q and q xh (row).
-template <class T, int VEC>
-__device__ __forceinline__ void ln_gather(const Vec<T, VEC>& cx, const Vec<T, VEC>& cy,
+template <int VEC, class C>
+__device__ __forceinline__ void ln_gather(const C& cx, const C& cy,
                                           const float* w, float mu, float rs, float* aw, float* ab,
                                           f32x2& s1, f32x2& s2) {
   const f32x2 m = pair(-mu, -mu), r = pair(rs, rs);
@@ -195,8 +248,8 @@ __device__ __forceinline__ void ln_gather(const Vec<T, VEC>& cx, const Vec<T, VE
   }
 }
 // Second half: dx = rs q - rs m1 - (x - mu) rs^2 m2, m1 and m2 the row's means.
-template <class T, int VEC>
-__device__ __forceinline__ void ln_spread(const Vec<T, VEC>& cx, const Vec<T, VEC>& cy,
+template <int VEC, class C>
+__device__ __forceinline__ void ln_spread(const C& cx, const C& cy,
                                           const float* w, float mu, float rs, float m1, float m2,
                                           float* o) {
   const f32x2 m = pair(-mu, -mu), r = pair(rs, rs);
@@ -212,21 +265,24 @@ __device__ __forceinline__ void ln_spread(const Vec<T, VEC>& cx, const Vec<T, VE
   }
 }
 
-template <class T, int VEC, int K, int G, bool WHOLE>
+template <class T, int VEC, int K, int G, LnMode M>
 __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K))
     k_ln_fwd(const T* __restrict__ x, int64_t xs, int64_t rows, int d, const float* __restrict__ w,
              const float* __restrict__ b, float eps, T* __restrict__ y, float* __restrict__ mean,
              float* __restrict__ rstd) {
   __shared__ float buf[2][1][32];
   int turn = 0;
-  const int nv = (d + VEC - 1) / VEC;
+  const int nv = ln_end<VEC, M>(d);
   const float inv_d = 1.f / (float)d;
   LnTeam t = ln_team<G>();
   // (a team's lanes shuffle together with the rest of their warp, so a warp
   // goes on until its last team is done)
   const int64_t lead = G && G < 32 ? t.row - (threadIdx.x % 32) / (G ? G : 1) : t.row;
+  LnParams<VEC, K, M, M != WHOLE && VEC * K <= 16> pw, pb;
+  pw.read(w, t, d);
+  pb.read(b, t, d);
   Vec<T, VEC> c[K];
-  ln_load<T, VEC, K, WHOLE>(x + t.row * xs, t, nv, d, t.row < rows, c);
+  ln_load<T, VEC, K, M>(x + t.row * xs, t, d, t.row < rows, c);
   for (int64_t lr = lead; lr < rows; lr += t.rows_step) {
     const bool on = t.row < rows;
     float f[K][VEC];
@@ -240,18 +296,18 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K))
     float s[1] = {s2.x + s2.y};
     // the next row's values are on their way meanwhile
     const int64_t next = t.row + t.rows_step;
-    ln_load<T, VEC, K, WHOLE>(x + next * xs, t, nv, d, next < rows, c);
+    ln_load<T, VEC, K, M>(x + next * xs, t, d, next < rows, c);
     team_sum<G, 1>(s, buf, turn);
     const float mu = s[0] * inv_d;
     s2 = pair(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int j = t.j + k * t.step;
+      const int j = t.j + k * ln_next<VEC, M>(t.step);
       if (j < nv) {
-        if (!WHOLE && (j + 1) * VEC > d)   // what pads the row's last vector adds nothing
+        if (M == SPREAD && ln_col<VEC, M>(j, VEC - 1, t.step) >= d)   // no values: they add nothing
 #pragma unroll
           for (int v = 0; v < VEC; ++v)
-            if (j * VEC + v >= d) f[k][v] = mu;
+            if (ln_col<VEC, M>(j, v, t.step) >= d) f[k][v] = mu;
         ln_centre<VEC>(f[k], mu, s2);
       }
     }
@@ -261,13 +317,13 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K))
     if (on) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int j = t.j + k * t.step;
+        const int j = t.j + k * ln_next<VEC, M>(t.step);
         if (j < nv) {
-          const Vec<float, VEC> wv = ln_param<VEC, WHOLE>(w, j, d);
-          const Vec<float, VEC> bv = b ? ln_param<VEC, WHOLE>(b, j, d) : wv;
+          const Vec<float, VEC> wv = pw.get(w, k, j, t.step, d);
+          const Vec<float, VEC> bv = b ? pb.get(b, k, j, t.step, d) : wv;
           float o[VEC];
           ln_scale<VEC>(f[k], rs, wv, b != nullptr, bv, o);
-          ln_put<T, VEC, WHOLE>(y + t.row * d, j, d, o);
+          ln_put<T, VEC, M>(y + t.row * d, j, t.step, d, o);
         }
       }
       if (t.j == 0 && mean) {
@@ -280,7 +336,7 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K))
 }
 
 // dx of the team's rows, and the block's partial sums of dy xh and dy.
-template <class T, int VEC, int K, int G, bool WHOLE>
+template <class T, int VEC, int K, int G, LnMode M>
 __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K), G ? kLnBwdBlocks : 1)
     k_ln_bwd(const T* __restrict__ dy, int64_t dys, const T* __restrict__ x, int64_t xs,
              int64_t rows, int d, const float* __restrict__ mean, const float* __restrict__ rstd,
@@ -288,10 +344,15 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K), 
   __shared__ float buf[2][2][32];
   extern __shared__ float sums[];          // teams inside a warp: [teams][2 d]
   int turn = 0;
-  const int nv = (d + VEC - 1) / VEC;
+  const int nv = ln_end<VEC, M>(d);
   const float inv_d = 1.f / (float)d;
   LnTeam t = ln_team<G>();
   const int64_t lead = G && G < 32 ? t.row - (threadIdx.x % 32) / (G ? G : 1) : t.row;
+  // Columns read value by value keep their weights in registers where the sums
+  // leave room (60000 x 200 bf16 rows of stride 201: 42 us, 63 without; blocks
+  // of 3000 x 7001 f16: 143, 134 without).
+  LnParams<VEC, K, M, M != WHOLE && G != 0> pr;
+  pr.read(w, t, d);
   float aw[K][VEC], ab[K][VEC];
 #pragma unroll
   for (int k = 0; k < K; ++k)
@@ -300,8 +361,8 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K), 
   // Few elements: the next row is loaded while this one is finished.
   constexpr bool AHEAD = VEC * K <= 8;
   Vec<T, VEC> cx[K], cy[K];
-  ln_load<T, VEC, K, WHOLE>(x + t.row * xs, t, nv, d, t.row < rows, cx);
-  ln_load<T, VEC, K, WHOLE>(dy + t.row * dys, t, nv, d, t.row < rows, cy);
+  ln_load<T, VEC, K, M>(x + t.row * xs, t, d, t.row < rows, cx);
+  ln_load<T, VEC, K, M>(dy + t.row * dys, t, d, t.row < rows, cy);
   float mu = t.row < rows ? mean[t.row] : 0.f, rs = t.row < rows ? rstd[t.row] : 0.f;
   for (int64_t lr = lead; lr < rows; lr += t.rows_step) {
     const bool on = t.row < rows;
@@ -309,10 +370,10 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K), 
     f32x2 s1 = pair(0.f, 0.f), s2 = s1;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int j = t.j + k * t.step;
+      const int j = t.j + k * ln_next<VEC, M>(t.step);
       if (j < nv) {
-        const Vec<float, VEC> wv = ln_param<VEC, WHOLE>(w, j, d);
-        ln_gather<T, VEC>(cx[k], cy[k], wv.v, m0, r0, aw[k], ab[k], s1, s2);
+        const Vec<float, VEC> wv = pr.get(w, k, j, t.step, d);
+        ln_gather<VEC>(cx[k], cy[k], wv.v, m0, r0, aw[k], ab[k], s1, s2);
       }
     }
     float s[2] = {s1.x + s1.y, s2.x + s2.y};
@@ -324,8 +385,8 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K), 
     }
     const int64_t next = t.row + t.rows_step;
     auto load_next = [&] {
-      ln_load<T, VEC, K, WHOLE>(x + next * xs, t, nv, d, next < rows, cx);
-      ln_load<T, VEC, K, WHOLE>(dy + next * dys, t, nv, d, next < rows, cy);
+      ln_load<T, VEC, K, M>(x + next * xs, t, d, next < rows, cx);
+      ln_load<T, VEC, K, M>(dy + next * dys, t, d, next < rows, cy);
       if (next < rows) {
         mu = mean[next];
         rs = rstd[next];
@@ -337,12 +398,12 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K), 
       const float m1 = s[0] * inv_d, m2 = s[1] * inv_d;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int j = t.j + k * t.step;
+        const int j = t.j + k * ln_next<VEC, M>(t.step);
         if (on && j < nv) {
           float o[VEC];
-          const Vec<float, VEC> wv = ln_param<VEC, WHOLE>(w, j, d);
-          ln_spread<T, VEC>(px[k], py[k], wv.v, m0, r0, m1, m2, o);
-          ln_put<T, VEC, WHOLE>(dx + t.row * d, j, d, o);
+          const Vec<float, VEC> wv = pr.get(w, k, j, t.step, d);
+          ln_spread<VEC>(px[k], py[k], wv.v, m0, r0, m1, m2, o);
+          ln_put<T, VEC, M>(dx + t.row * d, j, t.step, d, o);
         }
       }
       if (!AHEAD) load_next();
@@ -354,14 +415,16 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K), 
   if (G == 0) {                            // a block's threads own their columns
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int j = t.j + k * t.step;
+      const int j = t.j + k * ln_next<VEC, M>(t.step);
       if (j < nv)
 #pragma unroll
-        for (int v = 0; v < VEC; ++v)
-          if (WHOLE || j * VEC + v < d) {
-            pw[j * VEC + v] = aw[k][v];
-            pw[d + j * VEC + v] = ab[k][v];
+        for (int v = 0; v < VEC; ++v) {
+          const int c = ln_col<VEC, M>(j, v, t.step);
+          if (M != SPREAD || c < d) {
+            pw[c] = aw[k][v];
+            pw[d + c] = ab[k][v];
           }
+        }
     }
     return;
   }
@@ -369,14 +432,16 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K), 
   float* mine = sums + (int64_t)(threadIdx.x / (G ? G : 1)) * 2 * d;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int j = t.j + k * t.step;
+    const int j = t.j + k * ln_next<VEC, M>(t.step);
     if (j < nv)
 #pragma unroll
-      for (int v = 0; v < VEC; ++v)
-        if (WHOLE || j * VEC + v < d) {
-          mine[j * VEC + v] = aw[k][v];
-          mine[d + j * VEC + v] = ab[k][v];
+      for (int v = 0; v < VEC; ++v) {
+        const int c = ln_col<VEC, M>(j, v, t.step);
+        if (M != SPREAD || c < d) {
+          mine[c] = aw[k][v];
+          mine[d + c] = ab[k][v];
         }
+      }
   }
   __syncthreads();
   for (int c = threadIdx.x; c < 2 * d; c += kLnWarpThreads) {
@@ -430,8 +495,8 @@ __global__ void __launch_bounds__(ln_max_threads(VEC* K))
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int j = threadIdx.x + k * blockDim.x;
-    wr[k] = j < nv ? ln_param<VEC, true>(w, j, d) : vec_zero<float, VEC>();
-    br[k] = j < nv && b ? ln_param<VEC, true>(b, j, d) : vec_zero<float, VEC>();
+    wr[k] = j < nv ? ln_param<VEC, WHOLE>(w, j, 0, d) : vec_zero<float, VEC>();
+    br[k] = j < nv && b ? ln_param<VEC, WHOLE>(b, j, 0, d) : vec_zero<float, VEC>();
   }
   int s = 0;
   uint32_t parity = 0;
@@ -468,7 +533,7 @@ __global__ void __launch_bounds__(ln_max_threads(VEC* K))
       if (j < nv) {
         float o[VEC];
         ln_scale<VEC>(f[k], rs, wr[k], b != nullptr, br[k], o);
-        ln_put<T, VEC, true>(y + row * d, j, d, o);
+        ln_put<T, VEC, WHOLE>(y + row * d, j, 0, d, o);
       }
     }
     if (threadIdx.x == 0 && mean) {
@@ -515,7 +580,7 @@ __global__ void __launch_bounds__(ln_max_threads(VEC* K))
   for (int k = 0; k < K; ++k) {
     const int j = threadIdx.x + k * blockDim.x;
     Vec<float, VEC> wv = vec_zero<float, VEC>();
-    if (WREG && j < nv) wv = ln_param<VEC, true>(w, j, d);
+    if (WREG && j < nv) wv = ln_param<VEC, WHOLE>(w, j, 0, d);
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
       aw[k][v] = ab[k][v] = 0.f;
@@ -546,8 +611,8 @@ __global__ void __launch_bounds__(ln_max_threads(VEC* K))
       const int j = threadIdx.x + k * blockDim.x;
       if (j < nv) {
         Vec<float, VEC> wv;
-        if (!WREG) wv = ln_param<VEC, true>(w, j, d);
-        ln_gather<T, VEC>(ld_vec<T, VEC>(ix + j * VEC), ld_vec<T, VEC>(iy + j * VEC),
+        if (!WREG) wv = ln_param<VEC, WHOLE>(w, j, 0, d);
+        ln_gather<VEC>(ld_vec<T, VEC>(ix + j * VEC), ld_vec<T, VEC>(iy + j * VEC),
                           WREG ? wr[WREG ? k : 0] : wv.v, m0, r0, aw[k], ab[k], s1, s2);
       }
     }
@@ -565,11 +630,11 @@ __global__ void __launch_bounds__(ln_max_threads(VEC* K))
         const int j = threadIdx.x + k * blockDim.x;
         if (j < nv) {
           Vec<float, VEC> wv;
-          if (!WREG) wv = ln_param<VEC, true>(w, j, d);
+          if (!WREG) wv = ln_param<VEC, WHOLE>(w, j, 0, d);
           float o[VEC];
-          ln_spread<T, VEC>(ld_vec<T, VEC>(ix + j * VEC), ld_vec<T, VEC>(iy + j * VEC),
+          ln_spread<VEC>(ld_vec<T, VEC>(ix + j * VEC), ld_vec<T, VEC>(iy + j * VEC),
                             WREG ? wr[WREG ? k : 0] : wv.v, m0, r0, m1, m2, o);
-          ln_put<T, VEC, true>(dx + row * d, j, d, o);
+          ln_put<T, VEC, WHOLE>(dx + row * d, j, 0, d, o);
         }
       }
     }
@@ -798,17 +863,21 @@ extern "C" int qqt_layernorm_forward(const void* x, int32_t dtype, int64_t rows,
     }
     ln_shapes<V>(p, [&](auto kk, auto gg) {
       constexpr int K = decltype(kk)::value, G = decltype(gg)::value;
-      if (!whole) {
-        k_ln_fwd<T, V, K, G, false><<<blocks, p.threads, 0, st>>>(xp, x_stride, rows, (int)d, w, b, eps,
-                                                                  yp, mean, rstd);
+      auto run = [&](auto m) {
+        k_ln_fwd<T, V, K, G, decltype(m)::value><<<blocks, p.threads, 0, st>>>(
+            xp, x_stride, rows, (int)d, w, b, eps, yp, mean, rstd);
+      };
+      if (d % V) {
+        run(std::integral_constant<LnMode, SPREAD>{});
+      } else if (!whole) {
+        run(std::integral_constant<LnMode, SINGLE>{});
       } else if constexpr (G == 0) {
         const size_t smem = (size_t)p.ring.stages * p.ring.stage_bytes;
         if (ln_allow_smem((const void*)k_ln_row_fwd<T, V, K>, smem))
           k_ln_row_fwd<T, V, K><<<blocks, p.threads, smem, st>>>(xp, x_stride, rows, (int)d, w, b, eps,
                                                                  yp, mean, rstd, p.ring);
       } else {
-        k_ln_fwd<T, V, K, G, true><<<blocks, p.threads, 0, st>>>(xp, x_stride, rows, (int)d, w, b, eps,
-                                                                 yp, mean, rstd);
+        run(std::integral_constant<LnMode, WHOLE>{});
       }
     });
     return launch_status();
@@ -847,17 +916,21 @@ extern "C" int qqt_layernorm_backward(const void* dy, int64_t dy_stride, const v
       ln_shapes<V>(p, [&](auto kk, auto gg) {
         constexpr int K = decltype(kk)::value, G = decltype(gg)::value;
         size_t smem = G ? (size_t)(kLnWarpThreads / (G ? G : 1)) * 2 * d * 4 : 0;
-        if (!whole) {
-          k_ln_bwd<T, V, K, G, false><<<blocks, p.threads, smem, st>>>(
+        auto run = [&](auto m) {
+          k_ln_bwd<T, V, K, G, decltype(m)::value><<<blocks, p.threads, smem, st>>>(
               yp, dy_stride, xp, x_stride, rows, (int)d, mean, rstd, w, gp, part);
+        };
+        if (d % V) {
+          run(std::integral_constant<LnMode, SPREAD>{});
+        } else if (!whole) {
+          run(std::integral_constant<LnMode, SINGLE>{});
         } else if constexpr (G == 0) {
           smem = (size_t)p.ring.stages * p.ring.stage_bytes;
           if (ln_allow_smem((const void*)k_ln_row_bwd<T, V, K>, smem))
             k_ln_row_bwd<T, V, K><<<blocks, p.threads, smem, st>>>(
                 yp, dy_stride, xp, x_stride, rows, (int)d, mean, rstd, w, gp, part, p.ring);
         } else {
-          k_ln_bwd<T, V, K, G, true><<<blocks, p.threads, smem, st>>>(
-              yp, dy_stride, xp, x_stride, rows, (int)d, mean, rstd, w, gp, part);
+          run(std::integral_constant<LnMode, WHOLE>{});
         }
       });
     }
