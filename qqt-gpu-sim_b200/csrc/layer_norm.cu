@@ -34,15 +34,21 @@ namespace qqt {
 constexpr int kLnWarpThreads = 256;   // block of the teams inside a warp
 // Blocks of an SM that walk over rows.  Forward more than are resident (rows
 // are short, the last blocks even out: 180 against 187 us with 8 at 1048576 x
-// 128 f32); backward as many as are resident with 80 registers, since every
-// block ends in a partial row (250 us with 3, 294 with 4 that do not all fit).
-constexpr int kLnFwdBlocks = 16, kLnBwdBlocks = 3;
+// 128 f32); backward as many as are resident, since every block ends in a
+// partial row: 3 with 80 registers (250 us, 294 with 4 that do not all fit), 2
+// with 128 where a lane holds 16 values (40000 x 512 f32: 48 us, 78 with 3 and
+// sums that spill).
+constexpr int kLnFwdBlocks = 16;
+__host__ __device__ constexpr int ln_bwd_blocks(int e) { return e >= 16 ? 2 : 3; }
 // Threads of an SM in blocks that take a row each, 16 or 32 elements a thread.
 constexpr int kLnRowThreads16 = 768, kLnRowThreads32 = 512;
 
 // Largest block that walks rows with e elements a thread: the backward pass
 // keeps 2 e sums besides its operands.
 __host__ __device__ constexpr int ln_max_threads(int e) { return e == 16 ? 768 : 512; }
+// That of rows read value by value with their weights in registers, backward
+// (3000 x 7001 f16: 105 us, 136 with 768 threads of 80 registers).
+constexpr int kLnSpreadThreads = 512;
 
 // 1 / sqrt(v) of the unit with one Newton step: float32 accuracy.
 __device__ __forceinline__ float ln_rstd(float v) {
@@ -337,7 +343,8 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K))
 
 // dx of the team's rows, and the block's partial sums of dy xh and dy.
 template <class T, int VEC, int K, int G, LnMode M>
-__global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K), G ? kLnBwdBlocks : 1)
+__global__ void __launch_bounds__(G ? kLnWarpThreads : M == SPREAD ? kLnSpreadThreads : ln_max_threads(VEC * K),
+                  G ? ln_bwd_blocks(VEC * K) : 1)
     k_ln_bwd(const T* __restrict__ dy, int64_t dys, const T* __restrict__ x, int64_t xs,
              int64_t rows, int d, const float* __restrict__ mean, const float* __restrict__ rstd,
              const float* __restrict__ w, T* __restrict__ dx, float* __restrict__ part) {
@@ -349,17 +356,19 @@ __global__ void __launch_bounds__(G ? kLnWarpThreads : ln_max_threads(VEC * K), 
   LnTeam t = ln_team<G>();
   const int64_t lead = G && G < 32 ? t.row - (threadIdx.x % 32) / (G ? G : 1) : t.row;
   // Columns read value by value keep their weights in registers where the sums
-  // leave room (60000 x 200 bf16 rows of stride 201: 42 us, 63 without; blocks
-  // of 3000 x 7001 f16: 143, 134 without).
-  LnParams<VEC, K, M, M != WHOLE && G != 0> pr;
+  // leave room (60000 x 200 bf16 rows of stride 201: 42 us, 63 without; 30011 x
+  // 517 bf16: 77 and 87).
+  LnParams<VEC, K, M, (M != WHOLE && G != 0) || (M == SPREAD && VEC * K <= 16)> pr;
   pr.read(w, t, d);
   float aw[K][VEC], ab[K][VEC];
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int v = 0; v < VEC; ++v) aw[k][v] = ab[k][v] = 0.f;
-  // Few elements: the next row is loaded while this one is finished.
-  constexpr bool AHEAD = VEC * K <= 8;
+  // Where registers allow it the next row is loaded while this one is finished
+  // (80000 x 384 f16: 51 us, 55 without).
+  constexpr bool AHEAD =
+      VEC * K <= 8 || (sizeof(T) == 2 && VEC * K <= 16 && (G != 0 || M == SPREAD));
   Vec<T, VEC> cx[K], cy[K];
   ln_load<T, VEC, K, M>(x + t.row * xs, t, d, t.row < rows, cx);
   ln_load<T, VEC, K, M>(dy + t.row * dys, t, d, t.row < rows, cy);
@@ -768,19 +777,20 @@ static LnPlan ln_plan(int64_t rows, int64_t d, int vec, bool bwd) {
     p.g = nv <= 8 * p.k ? 8 : nv <= 16 * p.k ? 16 : 32;
     if (nv > 32 * p.k) p.k *= 2;
     const int64_t per_block = kLnWarpThreads / p.g, need = (rows + per_block - 1) / per_block;
-    const int64_t room = (int64_t)sms * (bwd ? kLnBwdBlocks : kLnFwdBlocks);
+    const int64_t room = (int64_t)sms * (bwd ? ln_bwd_blocks(p.k * vec) : kLnFwdBlocks);
     p.blocks = need < room ? need : room;
     return p;
   }
   // a block: 16 elements a thread, 32 where that takes too many threads
   p.k = 16 / vec;
-  if (nv > (int64_t)p.k * ln_max_threads(16)) p.k *= 2;
+  const bool few = bwd && d % vec;          // SPREAD's backward pass
+  if (nv > (int64_t)p.k * (few ? kLnSpreadThreads : ln_max_threads(16))) p.k *= 2;
   const int64_t th = (nv + p.k - 1) / p.k;
   if (th > ln_max_threads(p.k * vec)) return p;         // too long
   p.threads = (int)((th + 31) / 32 * 32);
   // blocks of an SM by the threads that the registers allow, and stages by the
   // shared memory that leaves each
-  const int room = p.k * vec == 16 ? kLnRowThreads16 : kLnRowThreads32;
+  const int room = p.k * vec == 16 && !few ? kLnRowThreads16 : kLnRowThreads32;
   int per_sm = room / p.threads;
   per_sm = per_sm < 1 ? 1 : per_sm > 16 ? 16 : per_sm;
   const int64_t row = d * (16 / vec), stage = (row + 127) / 128 * 128 * (bwd ? 2 : 1);
