@@ -28,7 +28,8 @@
 // Measured on a B200 (copy bandwidth 6.55 TB/s):
 //   8192 x 32000 bf16     loss and gradient 228 us, 4.6 TB/s (two values a
 //                         logit); scores 113 us, 4.6 TB/s
-//   2047 x 100003 f16     scores 107 us, 3.8 TB/s (rows at any alignment)
+//   2047 x 100003 f16     loss and gradient 287 us, 2.9 TB/s; scores 107 us, 3.8
+//                         TB/s (rows at any alignment)
 //   4096 x 32000 f32      loss and gradient 212 us, 4.9 TB/s
 //   1048576 rows of 5 + 2 f32 logits, masked: 40 us, 2.5 TB/s, of which the
 //                         row kernel takes 3/4 of the issue slots (800
@@ -668,6 +669,41 @@ __device__ __forceinline__ void put_grads(T* p, int sh, int j, int w, bool on,
   }
 }
 
+// The same where all of the warp's vectors lie whole in the row and sh > 0.  The
+// first lane's part of the word it shares goes out in pieces of 2, 4 and 8
+// bytes, and so does the last lane's (2047 x 100003 f16: 287 us, 340 value by
+// value).
+template <class T, int VEC>
+__device__ __forceinline__ void put_inner(T* p, int sh, int j, const Vec<T, VEC>& x) {
+  const int l = lane_id(), first = VEC - sh, b = sh * (int)sizeof(T);
+  const uint4 own = *reinterpret_cast<const uint4*>(&x);
+  uint4 under;
+  under.x = __shfl_up_sync(QQT_FULL, own.x, 1);
+  under.y = __shfl_up_sync(QQT_FULL, own.y, 1);
+  under.z = __shfl_up_sync(QQT_FULL, own.z, 1);
+  under.w = __shfl_up_sync(QQT_FULL, own.w, 1);
+  char* to = reinterpret_cast<char*>(p + (int64_t)j * VEC - sh);
+  const uint4 word = funnel<T, VEC>(under, own, first);
+  if (l > 0) {
+    *reinterpret_cast<uint4*>(to) = word;
+  } else {                               // bytes b to 15 of the word
+    if (b & 2)
+      *reinterpret_cast<uint16_t*>(to + b) =
+          (uint16_t)((b < 4 ? word.x : b < 8 ? word.y : b < 12 ? word.z : word.w) >> 16);
+    const int q = (b + 3) & ~3;
+    if (q & 4) *reinterpret_cast<uint32_t*>(to + q) = q == 4 ? word.y : word.w;
+    if (q <= 8) *reinterpret_cast<uint2*>(to + 8) = make_uint2(word.z, word.w);
+  }
+  if (l == 31) {                         // bytes 0 to b - 1 of the next word
+    const uint4 rest = funnel<T, VEC>(own, own, first);
+    if (b & 8) *reinterpret_cast<uint2*>(to + 16) = make_uint2(rest.x, rest.y);
+    if (b & 4) *reinterpret_cast<uint32_t*>(to + 16 + (b & 8)) = b & 8 ? rest.z : rest.x;
+    if (b & 2)
+      *reinterpret_cast<uint16_t*>(to + 16 + (b & 12)) =
+          (uint16_t)((b & 12) == 0 ? rest.x : (b & 12) == 4 ? rest.y : (b & 12) == 8 ? rest.z : rest.w);
+  }
+}
+
 template <class T>
 __device__ __forceinline__ int misfit(const T* p) {
   return (int)(((uintptr_t)p & 15) / sizeof(T));
@@ -914,6 +950,9 @@ __global__ void __launch_bounds__(kPlThreads, kPlThreads == 512 ? 2 : 1)
           uint4* q = reinterpret_cast<uint4*>(o) + j0;
 #pragma unroll
           for (int u = 0; u < U; ++u, q += step) *q = *reinterpret_cast<const uint4*>(&c[u]);
+        } else if (G != 8 && whole) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) put_inner<T, VEC>(o, osh, j0 + u * step, c[u]);
         } else {
 #pragma unroll
           for (int u = 0; u < U; ++u) {
