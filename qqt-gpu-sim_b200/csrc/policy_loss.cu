@@ -31,10 +31,10 @@
 //   2047 x 100003 f16     loss and gradient 287 us, 2.9 TB/s; scores 107 us, 3.8
 //                         TB/s (rows at any alignment)
 //   4096 x 32000 f32      loss and gradient 212 us, 4.9 TB/s
-//   1048576 rows of 5 + 2 f32 logits, masked: 40 us, 2.5 TB/s, of which the
-//                         row kernel takes 3/4 of the issue slots (800
-//                         instructions a row: logarithms, exponentials and
-//                         quotients of both heads and of the loss)
+//   1048576 rows of 5 + 2 f32 logits, masked: 39 us, 2.6 TB/s; 86 % of the
+//                         issue slots (900 instructions a row: logarithms,
+//                         exponentials and quotients of both heads and of the
+//                         loss)
 // The vocabulary rows execute about 9 instructions a logit and pass, 60 % of
 // the issue slots, 57 % of the special-function unit and 70 % of the memory
 // bandwidth at once; no one of them is full.
