@@ -299,6 +299,7 @@ __global__ void __launch_bounds__(kPlSmallRows, 8)
   HeadStat hs[NH];
   float ms[NH];
   float logp = 0.f, ent = 0.f;
+  bool dead = !on;                       // some head gives the action no value
   if (on) {
     int at = 0;
 #pragma unroll(NH <= 2 ? NH : 1)
@@ -319,13 +320,16 @@ __global__ void __launch_bounds__(kPlSmallRows, 8)
       HeadStat k;
       k.act = in ? at + (int)act : -1;
       const float za = in ? z[at + act] : -INFINITY;
-      logp += finish_head(k, m != -INFINITY, s, logf(s), e, za - m, za != -INFINITY);
+      const float lh = finish_head(k, m != -INFINITY, s, logf(s), e, za - m, za != -INFINITY);
+      dead |= lh == -INFINITY;
+      logp += lh;
       k.t_act = za == -INFINITY ? 0.f : za - m;
       ms[h] = m;
       ent += k.ent;
       hs[h] = k;
       at += w;
     }
+    if (dead) logp = -INFINITY;          // (another head's NaN would hide it in the sum)
     if (a.logp) a.logp[r] = logp;
     if (a.entropy) a.entropy[r] = ent;
   }
@@ -333,7 +337,7 @@ __global__ void __launch_bounds__(kPlSmallRows, 8)
   if (fold) __syncthreads();
   before_me_done();
   const float count = fold ? fmaxf((float)n_mask, 1.f) : rows_counted(a, counts);
-  const bool live = on && logp != -INFINITY && row.counts;
+  const bool live = !dead && row.counts;
   const RowLoss l = loss_of(a, row, logp, live);
   if (a.stats) {
     const float v[4] = {l.pg, l.kl, live ? ent : 0.f, l.clip};
@@ -373,7 +377,7 @@ __global__ void __launch_bounds__(kPlSmallRows, 8)
         const float t = max_nan(z[j] - m, kFloor);
         z[j] = live ? ex2_approx(t * kLog2e) * fmaf(cs, t, ks) * scale : 0.f;
       }
-      if (live) z[k.act] = action_grad(k, l.g, a.entropy_coef, scale);
+      if (live && k.act >= 0) z[k.act] = action_grad(k, l.g, a.entropy_coef, scale);
       at += w;
     }
   }
@@ -809,6 +813,7 @@ __global__ void __launch_bounds__(kPlThreads, kPlThreads == 512 ? 2 : 1)
   HeadStat hs[QQT_MAX_HEADS];
   float refs[QQT_MAX_HEADS];
   unsigned plain = 0;                    // heads whose sums are against the maximum itself
+  bool dead = false;                     // some head gives the action no value
   float logp = 0.f, ent = 0.f;
   int at = 0;
 #pragma unroll 1
@@ -875,17 +880,19 @@ __global__ void __launch_bounds__(kPlThreads, kPlThreads == 512 ? 2 : 1)
       lp = finish_head(k, any, q.s, log2f(q.s) * kLn2, q.e * kLn2, ta, z_act != -INFINITY);
       refs[h] = q.r;
     }
+    dead |= lp == -INFINITY;
     logp += lp;
     ent += k.ent;
     hs[h] = k;
     at += w;
   }
+  if (dead) logp = -INFINITY;            // (another head's NaN would hide it in the sum)
   if (lead) {
     if (a.logp) a.logp[r] = logp;
     if (a.entropy) a.entropy[r] = ent;
   }
   if (!a.old_logp) return;
-  const bool live = logp != -INFINITY && in.counts;
+  const bool live = !dead && in.counts;
   const RowLoss l = loss_of(a, in, logp, live);
   if (a.stats && lead)
     *reinterpret_cast<float4*>(part + r * 4) =
@@ -964,7 +971,7 @@ __global__ void __launch_bounds__(kPlThreads, kPlThreads == 512 ? 2 : 1)
     }
     // the action's own value, over what its vector's lane or the one above wrote
     __syncwarp();
-    if (live && exists && k.act / VEC % step == tl)
+    if (live && exists && k.act >= 0 && k.act / VEC % step == tl)
       o[k.act] = from_f<T>(action_grad(k, l.g, a.entropy_coef, scale));
     at += w;
   }

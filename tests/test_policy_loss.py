@@ -384,3 +384,50 @@ def test_c_entry_refusals():
     assert call(width=0) == 1 and call(logits=None) == 1 and call(actions=None) == 1
     assert call(old_logp=None) == 1 and call(adv=None) == 1 and call(work=None) == 1
     assert call(n_heads=9) == 3 and call(rows=1 << 33) == 3
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads", [[5, 2], [3] * 8, [60, 40], [900, 500], [20001, 19999]])
+def test_head_without_a_value_beside_a_head_of_nan(heads, dtype):
+    """A row is dead by any one head -- an action outside it, an illegal action,
+    no legal place -- whatever the others hold: NaN or an infinity there neither
+    brings it back nor reaches the sums or the rows around it.  The values of
+    the other rows are those of the same batch with the row's places all
+    illegal, bit for bit."""
+    _need_cuda()
+    v = sum(heads)
+    d = _data(12, v, heads, dtype, 41, legal=True)
+    d["mask"][:] = True
+    ends = [sum(heads[:k + 1]) for k in range(len(heads))]
+    rows = {0: ("outside", 0), 3: ("outside", 1), 4: ("illegal", 0), 6: ("empty", 1),
+            9: ("outside", len(heads) - 1), 11: ("empty", 0)}
+    clean = d["legal"].clone()
+    clean[list(rows)] = False
+    args = (d["old_logp"], d["adv"], d["ref_logp"])
+    want = policy_loss_and_grad(d["logits"], d["actions"], *args, clean, d["mask"], heads, **OPT)
+    for bad in (float("nan"), float("inf")):
+        z, legal, acts = d["logits"].clone(), d["legal"].clone(), d["actions"].clone()
+        for r, (how, k) in rows.items():
+            other = (k + 1) % len(heads)
+            z[r, ends[other] - heads[other] + int(acts[r, other])] = bad     # a legal place
+            at = ends[k] - heads[k]
+            if how == "outside":
+                acts[r, k] = -1 if r % 2 else heads[k]
+            elif how == "illegal":
+                legal[r, at + int(acts[r, k])] = False
+            else:
+                legal[r, at:ends[k]] = False
+        stats, logp, dz = policy_loss_and_grad(z, acts, *args, legal, d["mask"], heads, **OPT)
+        lp, _ = policy_logp(z, acts, legal, heads)
+        p = z.clone().requires_grad_(True)
+        loss, s2 = policy_loss(p, acts, *args, legal, d["mask"], heads, **OPT)
+        loss.backward()
+        torch.cuda.synchronize()
+        assert _capi.device_error() == 1 << 2                  # QQT_DEV_BAD_ACTION
+        assert bool((logp[list(rows)] == -math.inf).all()) and torch.equal(lp, logp)
+        assert not dz[list(rows)].any() and not p.grad[list(rows)].any()
+        assert torch.equal(stats, want[0]) and torch.equal(s2, want[0])
+        assert torch.equal(logp, want[1]) and torch.equal(dz, want[2])
+        keep = [r for r in range(12) if r not in rows]
+        assert torch.isfinite(p.grad[keep]).all() and torch.isfinite(stats).all()
