@@ -33,6 +33,14 @@ def _unit(t: torch.Tensor) -> torch.Tensor:
     return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
+def _like(x: torch.Tensor) -> torch.Tensor:
+    """An output of x's shape and type, dense and with a unit innermost stride:
+    in the order of x's strides where that leaves D innermost.  (It need not
+    where x overlaps itself, as sliding windows do: several strides are 1.)"""
+    out = torch.empty_like(x)
+    return out if x.shape[-1] <= 1 or out.stride(-1) == 1 else x.new_empty(x.shape)
+
+
 def _seqs(*tensors):
     """The tensors as one array of QqtSeq and its entries' addresses (None for
     a tensor that is None); the array has to live until the call is done."""
@@ -95,7 +103,7 @@ def gated_recurrence_forward(x: torch.Tensor, gate: torch.Tensor, h0: torch.Tens
     L = capi.lib()
     x, gate = _unit(x), _unit(gate)
     h0 = None if h0 is None else h0.contiguous()
-    h = torch.empty_like(x)                    # (dense, in the order of x's strides)
+    h = _like(x)
     last = x.new_empty((n, d), dtype=_F32)
     saved = last.new_empty((L.qqt_recurrence_chunks(t), n, d)) if save else None
     work, wp = _work(L, t, n, d, last)
@@ -124,7 +132,7 @@ def gated_recurrence_backward(dh: torch.Tensor | None, dh_last: torch.Tensor | N
     x, gate = _unit(x), _unit(gate)
     dh = None if dh is None else _unit(dh)
     dh_last = None if dh_last is None else dh_last.contiguous()
-    dx, dg = torch.empty_like(x), torch.empty_like(x)
+    dx, dg = _like(x), _like(x)
     dh0 = saved.new_empty((n, d))
     work, wp = _work(L, t, n, d, saved)
     keep, (hs, xs, gs, rs, dxs, dgs) = _seqs(dh, x, gate, reset, dx, dg)

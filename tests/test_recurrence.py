@@ -346,3 +346,64 @@ def test_c_entry_refusals():
     assert b(r(s), P, r(s), r(s), None, None, 0, 4, 2, 8, r(s), r(s), P, P, None) == 1
     assert b(r(s), P, r(s), r(s), None, P, 0, 4, 2, 8, None, r(s), P, P, None) == 1
     assert L.qqt_recurrence_chunks(0) == 0 and L.qqt_recurrence_chunks(1) == 1
+
+
+# Views that overlap themselves: a signal's sliding windows, ticks one sample
+# apart; sequences one sample apart; (T, N, D, strides).
+OVERLAPS = [(5, 3, 60, (1, 64, 1)), (4, 3, 8, (8, 1, 1)), (10, 3, 8, (50, 1, 1)),
+            (3, 1, 16, (1, 16, 1)), (70, 2, 128, (1, 1, 1)), (6, 5, 8, (0, 8, 1))]
+
+
+def _overlapping(t, n, d, strides, **kw):
+    g = torch.Generator(device=kw.get("device", "cpu")).manual_seed(t + d)
+    need = 1 + (t - 1) * strides[0] + (n - 1) * strides[1] + d - 1
+    return [torch.randn(need, generator=g, device=kw.get("device", "cpu"))
+            .to(kw.get("dtype", torch.float32)).as_strided((t, n, d), strides) for _ in range(2)]
+
+
+@pytest.mark.parametrize("t,n,d,strides", OVERLAPS)
+def test_outputs_are_dense_with_a_unit_innermost_stride(t, n, d, strides, monkeypatch):
+    """What the kernels are given to write, with the library replaced by one
+    that records it: d is innermost, and no two values share an address,
+    whatever x's strides."""
+    import ctypes
+    from qqt_b200 import _capi, recurrence
+    written = []
+
+    def note(*operands):
+        for p in operands:
+            ts, ns = (ctypes.c_int64 * 3).from_address(p)[1:]
+            at = (torch.arange(t)[:, None, None] * ts + torch.arange(n)[:, None] * ns
+                  + torch.arange(d)).flatten()
+            assert at.unique().numel() == t * n * d and at.max() < t * n * d
+            written.append((ts, ns, 1))
+        return 0
+
+    class Lib:
+        qqt_recurrence_chunks = staticmethod(lambda t: (t + 7) // 8)
+        qqt_recurrence_work_bytes = staticmethod(lambda t, n, d: 0)
+        qqt_recurrence_forward = staticmethod(lambda *a: note(a[8]))
+        qqt_recurrence_backward = staticmethod(lambda *a: note(a[10], a[11]))
+
+    monkeypatch.setattr(_capi, "lib", lambda: Lib)
+    monkeypatch.setattr(_capi, "launch_stream", lambda *a: 0)
+    x, g = _overlapping(t, n, d, strides)
+    h, _, saved = recurrence.gated_recurrence_forward(x, g)
+    dx, dg, _ = recurrence.gated_recurrence_backward(None, None, x, g, saved)
+    assert [v.stride() for v in (h, dx, dg)] == written
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("t,n,d,strides", OVERLAPS)
+def test_views_that_overlap_themselves(t, n, d, strides, dtype):
+    """Sliding windows give what their copies give, bit for bit."""
+    _need_cuda()
+    x, g = _overlapping(t, n, d, strides, device="cuda", dtype=dtype)
+    dh = torch.randn((t, n, d), device="cuda").to(dtype)
+    h, last, saved = gated_recurrence_forward(x, g)
+    got = (h, last, saved) + gated_recurrence_backward(dh, None, x, g, saved)
+    xc, gc = x.contiguous(), g.contiguous()
+    f = gated_recurrence_forward(xc, gc)
+    want = f + gated_recurrence_backward(dh, None, xc, gc, f[2])
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
