@@ -577,16 +577,20 @@ uint64_t qqt_policy_loss_work_bytes(int64_t rows);
  * them (synchronises the device). */
 int qqt_get_error(uint32_t *code_out);
 
-/* Failure-path check of the policy kernel (no counterpart in the
- * reference, whose torch forward has no device-side waits).  With polls >
+/* Failure-path check of the policy kernel and the layer norm's (no
+ * counterpart in the reference, whose torch forward has no device-side
+ * waits).  With polls >
  * 0, every following launch of the fused MLP kernel (qqt_mlp_act, the
  * tail of qqt_cnn_act, qqt_mlp_train_forward) first makes one bounded
  * mbarrier wait of `polls` polls on a
  * barrier that nothing completes at that point, before any copy or MMA is
  * issued; the wait expires like any wait that runs out (QQT_DEV_TIMEOUT in
  * the error word) and the kernel takes its abort path: no outputs, TMEM
- * freed, every CTA of a cluster through the closing barrier.  polls = 0
- * (the default) turns the check off.  Host-global setting. */
+ * freed, every CTA of a cluster through the closing barrier.  A layer norm
+ * whose rows are staged by bulk copies makes that wait with its first copies
+ * in flight, waits for them, copies no more and ends; what it wrote is not
+ * valid.  polls = 0 (the default) turns the check off.  Host-global
+ * setting. */
 int qqt_test_set_wait_polls(uint32_t polls);
 
 /* Phase stamps (no counterpart in the reference).  A library built with

@@ -477,7 +477,16 @@ constexpr int kLnStages = 8;
 struct LnRing {
   int stages;
   uint32_t stage_bytes, row_bytes;
+  uint32_t test_wait;      // polls of the failure-path check, 0 without it
 };
+
+// The last row that a block still fetches and waits for once its wait for `row`
+// has run out: what is in flight is waited for, row by row, and nothing more
+// is copied, so that nothing arrives after the block has given up its shared
+// memory.
+__device__ __forceinline__ int64_t ln_last(int64_t last, int64_t row, const LnRing& ring) {
+  return min(last, row + (int64_t)(ring.stages - 1) * gridDim.x);
+}
 
 template <class T, int VEC, int K>
 __global__ void __launch_bounds__(ln_max_threads(VEC* K))
@@ -485,19 +494,20 @@ __global__ void __launch_bounds__(ln_max_threads(VEC* K))
                  const float* __restrict__ w, const float* __restrict__ b, float eps,
                  T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd, LnRing ring) {
   extern __shared__ __align__(128) unsigned char stage[];
-  __shared__ uint64_t bar[kLnStages];
+  __shared__ uint64_t bar[kLnStages + 1];   // (the last is the failure-path check's)
   __shared__ float buf[2][1][32];
   int turn = 0;
   const int nv = (d + VEC - 1) / VEC;
   const float inv_d = 1.f / (float)d;
+  int64_t last = rows - 1;
   auto fetch = [&](int64_t row, int s) {
-    if (row < rows) {
+    if (row <= last) {
       stage_arm(&bar[s], ring.row_bytes);
       stage_copy(stage + (size_t)s * ring.stage_bytes, x + row * xs, ring.row_bytes, &bar[s]);
     }
   };
   if (threadIdx.x == 0) {
-    for (int s = 0; s < ring.stages; ++s) stage_init(&bar[s]);
+    for (int s = 0; s <= kLnStages; ++s) stage_init(&bar[s]);
     stage_init_done();
   }
   __syncthreads();
@@ -513,9 +523,10 @@ __global__ void __launch_bounds__(ln_max_threads(VEC* K))
   }
   int s = 0;
   uint32_t parity = 0;
-  bool alive = true;
+  if (ring.test_wait && !stage_wait(&bar[kLnStages], 0, ring.test_wait))
+    last = ln_last(last, blockIdx.x, ring);
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    if (alive) alive = stage_wait(&bar[s], parity);
+    if (row <= last && !stage_wait(&bar[s], parity)) last = ln_last(last, row, ring);
     const T* in = (const T*)(stage + (size_t)s * ring.stage_bytes);
     float f[K][VEC];
     f32x2 s2 = pair(0.f, 0.f);
@@ -567,14 +578,15 @@ __global__ void __launch_bounds__(ln_max_threads(VEC* K))
                  const float* __restrict__ rstd, const float* __restrict__ w, T* __restrict__ dx,
                  float* __restrict__ part, LnRing ring) {
   extern __shared__ __align__(128) unsigned char stage[];
-  __shared__ uint64_t bar[kLnStages];
+  __shared__ uint64_t bar[kLnStages + 1];   // (the last is the failure-path check's)
   __shared__ float buf[2][2][32];
   int turn = 0;
   const int nv = (d + VEC - 1) / VEC;
   const float inv_d = 1.f / (float)d;
   constexpr bool WREG = VEC * K <= 16;     // the weights fit beside the sums
+  int64_t last = rows - 1;
   auto fetch = [&](int64_t row, int s) {
-    if (row < rows) {
+    if (row <= last) {
       unsigned char* to = stage + (size_t)s * ring.stage_bytes;
       stage_arm(&bar[s], 2 * ring.row_bytes);
       stage_copy(to, x + row * xs, ring.row_bytes, &bar[s]);
@@ -582,7 +594,7 @@ __global__ void __launch_bounds__(ln_max_threads(VEC* K))
     }
   };
   if (threadIdx.x == 0) {
-    for (int s = 0; s < ring.stages; ++s) stage_init(&bar[s]);
+    for (int s = 0; s <= kLnStages; ++s) stage_init(&bar[s]);
     stage_init_done();
   }
   __syncthreads();
@@ -602,12 +614,13 @@ __global__ void __launch_bounds__(ln_max_threads(VEC* K))
   }
   int s = 0, before = -1;                  // before: the stage of the row before
   uint32_t parity = 0;
-  bool alive = true;
   float mu = 0.f, rs = 0.f;
   if (blockIdx.x < rows) {
     mu = mean[blockIdx.x];
     rs = rstd[blockIdx.x];
   }
+  if (ring.test_wait && !stage_wait(&bar[kLnStages], 0, ring.test_wait))
+    last = ln_last(last, blockIdx.x, ring);
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const float m0 = mu, r0 = rs;
     const int64_t next = row + gridDim.x;
@@ -615,7 +628,7 @@ __global__ void __launch_bounds__(ln_max_threads(VEC* K))
       mu = mean[next];
       rs = rstd[next];
     }
-    if (alive) alive = stage_wait(&bar[s], parity);
+    if (row <= last && !stage_wait(&bar[s], parity)) last = ln_last(last, row, ring);
     const T* ix = (const T*)(stage + (size_t)s * ring.stage_bytes);
     const T* iy = (const T*)((const unsigned char*)ix + ring.stage_bytes / 2);
     f32x2 s1 = pair(0.f, 0.f), s2 = s1;
@@ -772,7 +785,7 @@ struct LnPlan {
   LnRing ring;
 };
 static LnPlan ln_plan(int64_t rows, int64_t d, int vec, bool bwd) {
-  LnPlan p{0, 0, kLnWarpThreads, 0, {0, 0, 0}};
+  LnPlan p{0, 0, kLnWarpThreads, 0, {0, 0, 0, 0}};
   const int64_t nv = (d + vec - 1) / vec;
   const int sms = sm_count();
   if (nv <= (vec == 8 ? 64 : 128)) {       // a team inside a warp
@@ -801,7 +814,8 @@ static LnPlan ln_plan(int64_t rows, int64_t d, int vec, bool bwd) {
   int64_t n = 220 * 1024 / per_sm / stage;
   while (n < 3 && per_sm > 1) n = 220 * 1024 / --per_sm / stage;
   if (n < 2) return p;                                  // too long for two stages
-  p.ring = {(int)(n > kLnStages ? kLnStages : n), (uint32_t)stage, (uint32_t)row};
+  p.ring = {(int)(n > kLnStages ? kLnStages : n), (uint32_t)stage, (uint32_t)row,
+            g_test_wait_polls.load(std::memory_order_relaxed)};
   p.blocks = rows < (int64_t)sms * per_sm ? rows : (int64_t)sms * per_sm;
   return p;
 }

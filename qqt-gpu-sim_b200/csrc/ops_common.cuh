@@ -144,7 +144,8 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) { return __ffma
 
 // Rows staged by bulk copies: one mbarrier per stage, armed with the bytes of
 // its copies.  Waits are bounded; a wait that runs out is reported by the
-// device error word, and the kernel goes on to its end without further waits.
+// device error word.  The kernel then issues no further copy, waits (bounded)
+// for those in flight and goes on to its end; what it writes is not valid.
 constexpr uint32_t kStagePolls = 1u << 24;
 __device__ __forceinline__ uint32_t stage_addr(const void* p) {
   return (uint32_t)__cvta_generic_to_shared(p);
@@ -169,8 +170,11 @@ __device__ __forceinline__ void stage_copy(void* dst, const void* src, uint32_t 
       "l"(src), "r"(bytes), "r"(stage_addr(bar))
       : "memory");
 }
-__device__ __forceinline__ bool stage_wait(uint64_t* bar, uint32_t parity) {
-  for (uint32_t i = 0; i < kStagePolls; ++i) {
+// False once `polls` polls have run out; the copy is then given as many again,
+// so that it is not left in flight.
+__device__ __forceinline__ bool stage_wait(uint64_t* bar, uint32_t parity,
+                                           uint32_t polls = kStagePolls) {
+  for (uint32_t i = 0; i < 2 * polls; ++i) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -179,7 +183,10 @@ __device__ __forceinline__ bool stage_wait(uint64_t* bar, uint32_t parity) {
         : "=r"(ok)
         : "r"(stage_addr(bar)), "r"(parity)
         : "memory");
-    if (ok) return true;
+    if (ok) {
+      if (i < polls) return true;
+      break;
+    }
   }
   flag_error(QQT_DEV_TIMEOUT);
   return false;

@@ -256,3 +256,32 @@ def test_c_entry_refusals():
     assert L.qqt_layernorm_backward(P, 8, P, 8, 0, 4, 8, None, P, P, P, P, P, P, None) == 1
     assert L.qqt_layernorm_backward(P, 8, P, 8, 0, 4, 8, P, P, P, P, P, P, None, None) == 1
     assert L.qqt_layernorm_work_bytes(-1, 8) == 0
+
+
+@gpu
+@pytest.mark.parametrize("n,d,dtype", [(3000, 10816, torch.float16), (5000, 2704, torch.bfloat16),
+                                       (2000, 1352, torch.float32), (5, 8192, torch.float32)])
+def test_wait_expiry_ends_the_call(n, d, dtype):
+    """A wait for a staged row that runs out (qqt_test_set_wait_polls: one on a
+    barrier that nothing completes, with the first copies in flight) is
+    reported, the call ends, and the next one is as before."""
+    _need_cuda()
+    from qqt_b200 import _capi
+    x, w, b, dy = _data(n, d, dtype, 13)
+    x, dy = x.contiguous(), dy.contiguous()
+    y, mean, rstd = layer_norm_forward(x, w, b)
+    want = (y, mean, rstd) + layer_norm_backward(dy, x, mean, rstd, w)
+    assert _capi.device_error() == 0
+    lib = _capi.lib()
+    try:
+        assert lib.qqt_test_set_wait_polls(64) == 0
+        layer_norm_forward(x, w, b)
+        assert _capi.device_error() == 1 << 3                  # QQT_DEV_TIMEOUT
+        layer_norm_backward(dy, x, mean, rstd, w)
+        assert _capi.device_error() == 1 << 3
+    finally:
+        lib.qqt_test_set_wait_polls(0)
+    again = layer_norm_forward(x, w, b)
+    again = again + layer_norm_backward(dy, x, again[1], again[2], w)
+    assert _capi.device_error() == 0
+    assert all(torch.equal(p, q) for p, q in zip(want, again))
