@@ -522,7 +522,9 @@ int qqt_recurrence_forward(const QqtSeq *x, const QqtSeq *gate, const QqtSeq *re
                            const QqtSeq *h, float *h_last, float *carry, void *work,
                            qqt_stream_t stream);
 /* One tick: x, gate rows of N sequences -> h [N][D]; state -> state_out [N][D]
- * float32 (they may be the same); reset (optional) uint8 (N). */
+ * float32; reset (optional) uint8 (N).  state_out may be the state itself (or
+ * x or gate, float32 and contiguous); where it shares memory with an operand
+ * otherwise, or with h, the call is refused (QQT_E_ARG). */
 int qqt_recurrence_step(const void *x, int64_t x_stride, const void *gate, int64_t gate_stride,
                         const uint8_t *reset, int64_t reset_stride, const float *state,
                         int32_t dtype, int64_t N, int64_t D, void *h, float *state_out,

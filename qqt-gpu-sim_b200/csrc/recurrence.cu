@@ -591,6 +591,22 @@ static bool rec_fits(int64_t T, int64_t N, int64_t D) {
 static bool seq_vec(const RecSeq& s, int64_t bytes, int64_t es) {
   return !s.p || (aligned_to(s.p, bytes) && (s.ts * es) % bytes == 0 && (s.ns * es) % bytes == 0);
 }
+// Whether a step that writes `bytes` bytes from `out` on would write over what
+// another thread has yet to read: n rows of `width` bytes from p, `stride` bytes
+// apart, share memory with them, and not value by value (in_place).
+static bool rec_clash(const void* out, int64_t bytes, const void* p, int64_t n, int64_t stride,
+                      int64_t width, bool in_place) {
+  const int64_t lo = (int64_t)(uintptr_t)out, hi = lo + bytes;
+  int64_t at = (int64_t)(uintptr_t)p;
+  if (at == 0 || (in_place && at == lo)) return false;
+  if (stride < 0) {
+    at += (n - 1) * stride;
+    stride = -stride;
+  }
+  // the first row that ends beyond out's beginning
+  const int64_t row = at + width > lo ? 0 : stride ? (lo - at - width) / stride + 1 : n;
+  return row < n && at + row * stride < hi;
+}
 static RecSeq rec_seq(const QqtSeq* s) {
   return s ? RecSeq{s->p, s->t_stride, s->n_stride} : RecSeq{nullptr, 0, 0};
 }
@@ -692,6 +708,13 @@ extern "C" int qqt_recurrence_step(const void* x, int64_t x_stride, const void* 
   if (!rec_fits(1, N, D)) return QQT_E_LIMIT;
   if (N == 0) return QQT_OK;
   if (!x || !gate || !state || !h || !state_out) return QQT_E_ARG;
+  const int64_t es = dtype == QQT_F32 ? 4 : 2, out = N * D * 4;
+  if (rec_clash(state_out, out, state, N, D * 4, D * 4, true) ||
+      rec_clash(state_out, out, x, N, x_stride * es, D * es, es == 4 && x_stride == D) ||
+      rec_clash(state_out, out, gate, N, gate_stride * es, D * es, es == 4 && gate_stride == D) ||
+      rec_clash(state_out, out, reset, N, reset_stride, 1, false) ||
+      rec_clash(state_out, out, h, N, D * es, D * es, false))
+    return QQT_E_ARG;
   RecArgs a{};
   a.x = RecSeq{x, 0, x_stride};
   a.g = RecSeq{gate, 0, gate_stride};

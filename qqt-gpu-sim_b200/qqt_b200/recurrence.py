@@ -174,8 +174,9 @@ def gated_recurrence_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tens
                           reset: torch.Tensor | None = None,
                           state_out: torch.Tensor | None = None):
     """One tick: (h, new state) for x, gate (N, D), state (N, D) float32 and
-    reset (N,).  state_out receives the new state (it may be `state` itself:
-    the rollout's in-place form); by default it is a new tensor."""
+    reset (N,).  state_out receives the new state; it may be `state` itself
+    (the rollout's in-place form) and overlaps no operand otherwise.  By default
+    it is a new tensor."""
     code = _check(x, gate, state, reset, 2, "state")
     if state is None or not state.is_contiguous():
         raise ValueError("state must be contiguous")
@@ -196,5 +197,7 @@ def gated_recurrence_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tens
         None if reset is None else reset.data_ptr(), 0 if reset is None else reset.stride(0),
         state.data_ptr(), code, n, d, h.data_ptr(), out.data_ptr(), stream)
     if rc:
+        if rc == 1 and state_out is not None:      # (the entry's one refusal left)
+            raise ValueError("state_out overlaps an operand")
         capi.check(rc, "qqt_recurrence_step")
     return h, out

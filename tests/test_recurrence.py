@@ -407,3 +407,60 @@ def test_views_that_overlap_themselves(t, n, d, strides, dtype):
     f = gated_recurrence_forward(xc, gc)
     want = f + gated_recurrence_backward(dh, None, xc, gc, f[2])
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+
+def test_c_step_refuses_a_state_out_that_overlaps():
+    """A thread that wrote what another has yet to read would race: refused
+    before anything is launched, on made-up addresses, from one byte of overlap
+    on.  State and outputs are 5 x 8 floats (160 bytes)."""
+    from qqt_b200 import _capi
+    L = _capi.lib()
+    X, G, S, R, H, OUT = (0x100000 * k for k in range(1, 7))
+
+    def step(out=OUT, x=X, xs=8, dtype=0, reset=None, rs=0, h=H):
+        return L.qqt_recurrence_step(x, xs, G, 8, reset, rs, S, dtype, 5, 8, h, out, None)
+
+    for base in (X, G, S, H):
+        for k in (4, 32, 156, -4, -32, -156):
+            assert step(out=base + k) == 1, (base, k)
+    assert step(out=H) == 1                                   # two outputs in one place
+    assert step(out=X, dtype=1) == 1 and step(out=X, xs=16) == 1
+    assert step(reset=OUT, rs=1) == 1 and step(reset=OUT + 159, rs=1) == 1
+    assert step(reset=OUT - 4, rs=1) == 1 and step(reset=OUT, rs=0) == 1
+    # rows of a wider buffer, 100 floats apart: each of them counts
+    for row in range(5):
+        for k in (-156, -4, 0, 28):
+            assert step(x=X, xs=100, out=X + 400 * row + k) == 1, (row, k)
+    assert step(x=OUT + 4, xs=0) == 1 and step(x=OUT + 1600, xs=-100) == 1
+
+
+@gpu
+def test_state_out_in_every_allowed_place():
+    """The state itself, memory right before and after each operand, the gap
+    between the rows of a wider one, x or gate themselves."""
+    _need_cuda()
+    n, d = 5, 8
+    size = n * d
+    g = torch.Generator(device="cuda").manual_seed(4)
+    fresh = torch.randn(9 * size, generator=g, device="cuda")
+    reset = torch.tensor([0, 1, 0, 0, 1], dtype=torch.uint8, device="cuda")
+
+    def run(where, row=None):
+        buf = fresh.clone()
+        at = [buf[k * size:(k + 1) * size].view(n, d) for k in range(9)]
+        x = buf[:(n - 1) * row + d].as_strided((n, d), (row, 1)) if row else at[1]
+        want = gated_recurrence_step(x, at[5], at[3], reset)
+        out = at[where] if row is None else buf[where:where + size].view(n, d)
+        got = gated_recurrence_step(x, at[5], at[3], reset, state_out=out)
+        assert got[1] is out and all(torch.equal(p, q) for p, q in zip(got, want))
+
+    for where in (0, 1, 2, 3, 4, 5, 6):
+        run(where)
+    run(8, row=60)                       # x's rows at 0, 60, 120, ..: 8 to 59 is free
+    run(20, row=60)
+    with pytest.raises(ValueError, match="overlap"):
+        run(21, row=60)
+    state = fresh[:size].view(n, d)
+    with pytest.raises(ValueError, match="overlap"):
+        gated_recurrence_step(state, state, state, state_out=fresh[d:d + size].view(n, d))
