@@ -488,7 +488,8 @@ uint64_t qqt_mlp_train_work_bytes(int32_t n_rows);
  * Element types of their large operands; parameters, states, statistics and
  * per-row values are float32.  Rows and sequences have a unit innermost
  * stride; the other strides are in elements.  Null pointers mark what an
- * entry point says is optional.  Sizes of zero are no error. */
+ * entry point says is optional.  Workspaces are on 16 bytes (QQT_E_ALIGN).
+ * Sizes of zero are no error. */
 enum { QQT_F32 = 0, QQT_F16 = 1, QQT_BF16 = 2 };
 
 /* Layer norm of rows of d values (the norms of train/model.py:77-101 and

@@ -922,6 +922,7 @@ extern "C" int qqt_layernorm_backward(const void* dy, int64_t dy_stride, const v
   if (rows > 0 && (!dy || !x || !mean || !rstd || !w)) return QQT_E_ARG;
   const bool sums = dw || db;
   if (sums && !work) return QQT_E_ARG;
+  if (sums && !aligned_to(work, 16)) return QQT_E_ALIGN;
   return with_dtype(dtype, [&](auto e) {
     using T = decltype(e);
     constexpr int V = 16 / sizeof(T);

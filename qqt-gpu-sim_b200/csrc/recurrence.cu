@@ -675,6 +675,7 @@ extern "C" int qqt_recurrence_forward(const QqtSeq* x, const QqtSeq* gate, const
                                       void* work, qqt_stream_t stream) {
   if (!x || !gate || !h || !dtype_ok(dtype) || !rec_sizes_ok(T, N, D)) return QQT_E_ARG;
   if (!rec_fits(T, N, D)) return QQT_E_LIMIT;
+  if (!aligned_to(work, 16)) return QQT_E_ALIGN;
   const int64_t C = N * D;
   if (C == 0) return QQT_OK;
   cudaStream_t st = (cudaStream_t)stream;
@@ -743,6 +744,7 @@ extern "C" int qqt_recurrence_backward(const QqtSeq* dh, const float* dh_last, c
                                        qqt_stream_t stream) {
   if (!x || !gate || !dx || !dgate || !dtype_ok(dtype) || !rec_sizes_ok(T, N, D)) return QQT_E_ARG;
   if (!rec_fits(T, N, D)) return QQT_E_LIMIT;
+  if (!aligned_to(work, 16)) return QQT_E_ALIGN;
   const int64_t C = N * D;
   if (C == 0) return QQT_OK;
   cudaStream_t st = (cudaStream_t)stream;

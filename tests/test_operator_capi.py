@@ -52,3 +52,22 @@ def test_work_sizes_cover_both_directions_and_every_type():
     assert L.qqt_recurrence_chunks(0) == 0 and L.qqt_recurrence_chunks(9) == 2
     n = L.qqt_layernorm_work_bytes(1, 7)
     assert n >= 2 * 7 * 4
+
+
+@pytest.mark.parametrize("off", [4, 8, 12])
+def test_workspaces_off_their_alignment_are_refused(off):
+    """The kernels move workspaces by accesses of up to 16 bytes: refused before
+    anything is launched (made-up addresses)."""
+    from qqt_b200 import _capi
+    L, P = _capi.lib(), 0x100000
+    s = _capi.QqtSeq(P, 1024, 1024)
+    r = ctypes.byref(s)
+    assert L.qqt_recurrence_work_bytes(4096, 1, 1024) > 0
+    assert L.qqt_recurrence_forward(r, r, None, P, 0, 4096, 1, 1024, r, P, P, P + off, None) == 2
+    assert L.qqt_recurrence_backward(r, P, r, r, None, P, 0, 4096, 1, 1024, r, r, P, P + off,
+                                     None) == 2
+    assert L.qqt_layernorm_backward(P, 8, P, 8, 0, 4, 8, P, P, P, P, P, P, P + off, None) == 2
+    a = _capi.QqtPolicyLoss(logits=P, row_stride=7, rows=4, actions=P, action_stride=1, old_logp=P,
+                            adv=P, stats=P, work=P + off, grad_scale=1.0, dtype=0, n_heads=1)
+    a.width[0] = 7
+    assert L.qqt_policy_loss(ctypes.byref(a), None) == 2
