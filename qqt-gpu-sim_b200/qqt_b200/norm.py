@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _capi as capi
@@ -121,9 +122,11 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
                eps: float = 1e-5) -> torch.Tensor:
     """(x - mean) / sqrt(var + eps) * weight + bias over the weight's trailing
-    dimensions of x; differentiable in x, weight and bias."""
+    dimensions of x; differentiable in x, weight and bias (backward mode: a
+    forward-mode tangent raises NotImplementedError)."""
+    # (the Function sees to tangents, which set no requires_grad)
     if (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)) \
-            and torch.is_grad_enabled():
+            and torch.is_grad_enabled() or forward_ad._current_level >= 0:
         return _LayerNorm.apply(x, weight, bias, eps)
     return layer_norm_forward(x, weight, bias, eps, False)[0]
 

@@ -20,6 +20,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _capi as capi
@@ -163,9 +164,11 @@ class _Recurrence(torch.autograd.Function):
 def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, h0: torch.Tensor | None = None,
                      reset: torch.Tensor | None = None):
     """(h, h_last) of the recurrence over x, gate (T, N, D); differentiable in
-    x, gate and h0."""
-    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad
-                                    or (h0 is not None and h0.requires_grad)):
+    x, gate and h0 (backward mode: a forward-mode tangent raises
+    NotImplementedError)."""
+    # (the Function sees to tangents, which set no requires_grad)
+    if forward_ad._current_level >= 0 or torch.is_grad_enabled() and (
+            x.requires_grad or gate.requires_grad or (h0 is not None and h0.requires_grad)):
         return _Recurrence.apply(x, gate, h0, reset)
     return gated_recurrence_forward(x, gate, h0, reset, save=False)[:2]
 
@@ -176,7 +179,7 @@ def gated_recurrence_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tens
     """One tick: (h, new state) for x, gate (N, D), state (N, D) float32 and
     reset (N,).  state_out receives the new state; it may be `state` itself
     (the rollout's in-place form) and overlaps no operand otherwise.  By default
-    it is a new tensor."""
+    it is a new tensor.  Not differentiable."""
     code = _check(x, gate, state, reset, 2, "state")
     if state is None or not state.is_contiguous():
         raise ValueError("state must be contiguous")
