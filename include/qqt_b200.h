@@ -550,11 +550,12 @@ uint64_t qqt_recurrence_work_bytes(int64_t T, int64_t N, int64_t D);
  * row; mask (optional) uint8 [rows]; ref_logp optional.  A row none of whose
  * categories in some head is legal, or whose action is not, has logp -inf
  * and adds nothing to the sums or the gradient; an action outside its head
- * raises QQT_DEV_BAD_ACTION.  Outputs, each optional: logp, entropy [rows];
- * stats [5] = loss and the means of policy term, KL, entropy and clipped
- * share; dlogits rows of dlogits_stride = grad_scale upstream[0] dloss/dlogits
- * (upstream optional, 1).  Without stats and dlogits, old_logp .. mask and
- * work are not read.  work = qqt_policy_loss_work_bytes(rows) bytes. */
+ * raises QQT_DEV_BAD_ACTION unless the mask leaves its row out.  Outputs,
+ * each optional: logp, entropy [rows]; stats [5] = loss and the means of
+ * policy term, KL, entropy and clipped share; dlogits rows of dlogits_stride
+ * = grad_scale upstream[0] dloss/dlogits (upstream optional, 1).  Without
+ * stats and dlogits, old_logp .. mask and work are not read.  work =
+ * qqt_policy_loss_work_bytes(rows) bytes. */
 #define QQT_MAX_HEADS 8
 typedef struct QqtPolicyLoss {
   const void *logits;

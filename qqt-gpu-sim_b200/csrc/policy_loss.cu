@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(kPlSmallRows, 8)
       const int w = a.width[h];
       const int64_t act = a.actions[r * a.action_stride + h];
       const bool in = act >= 0 && act < w;
-      if (!in) flag_error(QQT_DEV_BAD_ACTION);
+      if (!in && row.counts) flag_error(QQT_DEV_BAD_ACTION);
       float m = -INFINITY, s = 0.f, e = 0.f;
 #pragma unroll 4
       for (int j = at; j < at + w; ++j) m = max_nan(m, z[j]);
@@ -861,7 +861,7 @@ __global__ void __launch_bounds__(kPlThreads, kPlThreads == 512 ? 2 : 1)
     const bool any = q.m != -INFINITY;
     const bool one_step = q.m >= -L::kLow && q.m <= kRefMost;
     HeadStat k;
-    if (!in_head && lead) flag_error(QQT_DEV_BAD_ACTION);
+    if (!in_head && lead && in.counts) flag_error(QQT_DEV_BAD_ACTION);
     k.act = in_head ? (int)act : -1;
     float lp;
     // (teams of one warp go together: whoever does not need it leaves it unused)

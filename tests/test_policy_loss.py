@@ -431,3 +431,32 @@ def test_head_without_a_value_beside_a_head_of_nan(heads, dtype):
         assert torch.equal(logp, want[1]) and torch.equal(dz, want[2])
         keep = [r for r in range(12) if r not in rows]
         assert torch.isfinite(p.grad[keep]).all() and torch.isfinite(stats).all()
+
+
+@gpu
+@pytest.mark.parametrize("v,heads", [(7, [5, 2]), (24, [3] * 8), (100, [60, 40]), (1000, None),
+                                     (20000, None)])
+def test_padding_actions_of_masked_rows_raise_nothing(v, heads):
+    """Rows that the mask leaves out hold any action (-1, -100, the head's width,
+    far out): the device error word stays clear and the counted rows' values are
+    what they are without the padding.  In a counted row the same action raises."""
+    _need_cuda()
+    d = _data(30, v, heads, torch.float32, 23, legal=True)
+    d["mask"][:] = True
+    d["mask"][[0, 4, 11, 29]] = False
+    args = (d["old_logp"], d["adv"], d["ref_logp"], d["legal"], d["mask"], heads)
+    want = policy_loss_and_grad(d["logits"], d["actions"], *args, **OPT)
+    acts = d["actions"].clone()
+    acts[0], acts[4], acts[11], acts[29] = -1, -100, (heads or [v])[-1], 1 << 40
+    stats, logp, dz = policy_loss_and_grad(d["logits"], acts, *args, **OPT)
+    z = d["logits"].clone().requires_grad_(True)
+    loss, s2 = policy_loss(z, acts, *args, **OPT)
+    loss.backward()
+    torch.cuda.synchronize()
+    assert _capi.device_error() == 0
+    assert torch.equal(stats, want[0]) and torch.equal(dz, want[2]) and torch.equal(s2, stats)
+    assert torch.equal(logp[d["mask"]], want[1][d["mask"]])
+    assert not z.grad[~d["mask"]].any()
+    acts[7] = -1
+    policy_loss_and_grad(d["logits"], acts, *args, **OPT)
+    assert _capi.device_error() == 1 << 2                      # QQT_DEV_BAD_ACTION
