@@ -156,7 +156,7 @@ __device__ __forceinline__ float head_k(const HeadStat& k, float g, float c) {
 }
 __device__ __forceinline__ float action_grad(const HeadStat& k, float g, float c, float scale) {
   const float lp = k.t_act - k.log_s, p = expf(lp);
-  return scale * fmaf(g, 1.f - p, p * (c * (lp + k.ent)));
+  return scale * fmaf(g, 1.f - p, c * (p * (lp + k.ent)));   // (p = 0 first: c lp may overflow)
 }
 
 // ---------------------------------------------------- few logits: thread per row
@@ -321,8 +321,8 @@ __global__ void __launch_bounds__(kPlSmallRows, 8)
       k.act = in ? at + (int)act : -1;
       const float za = in ? z[at + act] : -INFINITY;
       const float lh = finish_head(k, m != -INFINITY, s, logf(s), e, za - m, za != -INFINITY);
-      dead |= lh == -INFINITY;
       logp += lh;
+      dead |= lh == -INFINITY || logp == -INFINITY;
       k.t_act = za == -INFINITY ? 0.f : za - m;
       ms[h] = m;
       ent += k.ent;
@@ -872,16 +872,16 @@ __global__ void __launch_bounds__(kPlThreads, kPlThreads == 512 ? 2 : 1)
     }
     if (any && !one_step) {
       plain |= 1u << h;
-      lp = finish_head(k, any, q.s, logf(q.s), q.e, max_nan(z_act - q.m, kFloor),
-                       z_act != -INFINITY);
+      lp = finish_head(k, any, q.s, logf(q.s), q.e, z_act - q.m, z_act != -INFINITY);
       refs[h] = q.m;
     } else {
-      const float ta = fmaf(max_nan(z_act, -1.0e30f), kLog2e, -q.r) * kLn2;
+      // (far below, where the product may overflow, the maximum is no part of it)
+      const float ta = z_act < -1.0e30f ? z_act : fmaf(z_act, kLog2e, -q.r) * kLn2;
       lp = finish_head(k, any, q.s, log2f(q.s) * kLn2, q.e * kLn2, ta, z_act != -INFINITY);
       refs[h] = q.r;
     }
-    dead |= lp == -INFINITY;
     logp += lp;
+    dead |= lp == -INFINITY || logp == -INFINITY;
     ent += k.ent;
     hs[h] = k;
     at += w;

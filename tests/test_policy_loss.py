@@ -460,3 +460,40 @@ def test_padding_actions_of_masked_rows_raise_nothing(v, heads):
     acts[7] = -1
     policy_loss_and_grad(d["logits"], acts, *args, **OPT)
     assert _capi.device_error() == 1 << 2                      # QQT_DEV_BAD_ACTION
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("v,heads", [(7, [5, 2]), (40, None), (100, [60, 40]), (2000, None),
+                                     (30000, None)])
+def test_actions_far_below_the_maximum_keep_their_logp(v, heads, dtype):
+    """An action more than 1e4 below its row's maximum, wherever that lies, down
+    to the type's lowest value: log p = z - m - log S has one rounding of |z - m|
+    and the bound of the other values besides.  Its ratio is 0, its gradient
+    finite, also with an entropy bonus above 1."""
+    _need_cuda()
+    d = _data(12, v, heads, dtype, 37, ref=False, mask=False)
+    low = torch.finfo(dtype).min
+    half = dtype == torch.float16
+    tops = [0.0, 0.0, -3.2e4, -3.2e4, 5e4, 3.0e4] if half else [0.0, 0.0, -3e6, 3e6, -5e29, 2e7]
+    below = [low, -6.0e4, -6.5e4, low, -2e4, -2.5e4] if half \
+        else [low, -2e30, -4e6, -3e6, -2e30, low]
+    at = 0
+    for k, w in enumerate(heads or [v]):
+        for r, (top, act) in enumerate(zip(tops, below)):
+            z = torch.full((w,), top, device="cuda") - torch.rand(w, device="cuda")
+            z[d["actions"][r, k]] = act
+            d["logits"][r, at:at + w] = z.to(dtype)
+        at += w
+    want = _ref(d, OPT)["logp"]
+    assert bool((want[:6] < -1e4).all())
+    logp, ent = policy_logp(d["logits"], d["actions"], heads=heads)
+    # two heads at the lowest value: beyond float32, which holds -inf there
+    past = torch.isinf(want.float())
+    assert bool((logp[past] == -math.inf).all()) and (len(heads or [v]) > 1 or not past.any())
+    assert bool(((logp.double() - want).abs() <= C * (1 + want.abs()))[~past].all()), (logp, want)
+    assert torch.isfinite(ent).all()
+    stats, lp2, dz = policy_loss_and_grad(d["logits"], d["actions"], want.float(), d["adv"],
+                                          heads=heads, clip=0.2, entropy_coef=2.0)
+    assert torch.equal(lp2, logp) and torch.isfinite(dz).all()
+    assert _capi.device_error() == 0
