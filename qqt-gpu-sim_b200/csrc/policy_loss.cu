@@ -110,8 +110,9 @@ __device__ __forceinline__ RowLoss row_loss(float logp, float old, float a, floa
   RowLoss o;
   const float r = expf(logp - old);
   const float rc = fminf(fmaxf(r, 1.f - lo), 1.f + hi);
-  const float u = r * a, v = rc * a;
-  o.pg = -(r != r || a != a ? r * a : fminf(u, v));
+  // (an advantage of 0 weighs any ratio away, one beyond float32 too)
+  const float u = a == 0.f && r == INFINITY ? 0.f : r * a, v = rc * a;
+  o.pg = -(u != u ? u : fminf(u, v));
   o.clip = r < 1.f - lo || r > 1.f + hi ? 1.f : 0.f;
   const bool bound = (a > 0.f && r > 1.f + hi) || (a < 0.f && r < 1.f - lo);
   o.g = bound ? 0.f : -u;

@@ -497,3 +497,25 @@ def test_actions_far_below_the_maximum_keep_their_logp(v, heads, dtype):
                                           heads=heads, clip=0.2, entropy_coef=2.0)
     assert torch.equal(lp2, logp) and torch.isfinite(dz).all()
     assert _capi.device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("v,heads", [(7, [5, 2]), (300, None), (20000, None)])
+def test_advantage_of_zero_beside_a_ratio_beyond_float32(v, heads):
+    """exp(logp - old) of 200 is a number in 64 bits, and 0 of it is 0: the row
+    adds its entropy and nothing else, in the loss and in the gradient alike.  A
+    NaN ratio is not hidden by the advantage."""
+    _need_cuda()
+    d = _data(9, v, heads, torch.float32, 19, ref=False, mask=False)
+    d["adv"][2], d["adv"][5] = 0.0, -0.0
+    d["old_logp"][[2, 5]] -= 200.0
+    opt = dict(clip=(0.2, 0.3), kl_coef=0.0, entropy_coef=0.02)
+    _check(d, opt)
+    p = d["logits"].clone().requires_grad_(True)
+    loss, stats = policy_loss(p, d["actions"], d["old_logp"], d["adv"], heads=heads, **opt)
+    loss.backward()
+    assert torch.isfinite(stats).all() and torch.isfinite(p.grad).all()
+    d["old_logp"][2] = float("nan")
+    stats, _, dz = policy_loss_and_grad(d["logits"], d["actions"], d["old_logp"], d["adv"],
+                                        heads=heads, **opt)
+    assert stats[1].isnan() and dz[2].isnan().all() and torch.isfinite(dz[5]).all()
