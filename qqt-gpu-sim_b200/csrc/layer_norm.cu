@@ -54,10 +54,11 @@ __host__ __device__ constexpr int ln_max_threads(int e) { return e == 16 ? 768 :
 // (3000 x 7001 f16: 105 us, 136 with 768 threads of 80 registers).
 constexpr int kLnSpreadThreads = 512;
 
-// 1 / sqrt(v) of the unit with one Newton step: float32 accuracy.
+// 1 / sqrt(v) of the unit with one Newton step: float32 accuracy.  Where v or r
+// is infinite the step is 0 x inf, and r is the value already.
 __device__ __forceinline__ float ln_rstd(float v) {
   const float r = rsqrtf(v);
-  return r * fmaf(-0.5f * v * r, r, 1.5f);
+  return r == INFINITY || r == 0.f ? r : r * fmaf(-0.5f * v * r, r, 1.5f);
 }
 
 // Sums of N values over a team of G lanes (G <= 32), or over the block (G =

@@ -285,3 +285,27 @@ def test_wait_expiry_ends_the_call(n, d, dtype):
     again = again + layer_norm_backward(dy, x, again[1], again[2], w)
     assert _capi.device_error() == 0
     assert all(torch.equal(p, q) for p, q in zip(want, again))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 130, 512, 1352, 3001, 9000, 16392, 20001])
+def test_variance_beyond_float32_and_of_zero(d, dtype):
+    """Every path gives what 1 / sqrt(var + eps) is in float32: 0 for a variance
+    past its range (y is the bias, dx 0), infinity for none and eps = 0 (0 times
+    infinity: NaN); the rows beside are untouched."""
+    _need_cuda()
+    x, w, b, dy = _data(5, d, dtype, d)
+    want = layer_norm_forward(x, w, b)
+    wide = x.clone()
+    wide[1] = torch.where(torch.arange(d, device="cuda") % 2 == 0, 1e30, -1e30).to(dtype)
+    wide[3] = 0.0
+    y, mean, rstd = layer_norm_forward(wide, w, b)
+    assert rstd[1] == 0 and torch.equal(y[1], b.to(dtype)) and torch.equal(y[3], b.to(dtype))
+    dx, _, _ = layer_norm_backward(dy, wide, mean, rstd, w)
+    assert not dx[1].any() and torch.isfinite(dx).all()
+    _, _, r0 = layer_norm_forward(wide, w, b, eps=0.0)
+    y0 = layer_norm(wide, w, b, eps=0.0)
+    assert r0[1] == 0 and r0[3] == float("inf") and y0[3].isnan().all()
+    for r in (0, 2, 4):
+        assert torch.equal(y[r], want[0][r]) and torch.isfinite(y0[r]).all()
