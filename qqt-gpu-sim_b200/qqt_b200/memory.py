@@ -86,7 +86,8 @@ def collect_memory(sim, model: MemoryActorCritic, opponent, T: int, state=None, 
     seat).  state, fresh: what the rollout before left under "state" and
     "fresh" (an episode has just begun); None starts anew."""
     n, dev = sim.num_envs, sim.device
-    state = model.initial_state(n) if state is None else state
+    # (the ticks advance a state of this rollout's own in place)
+    state = model.initial_state(n) if state is None else state.clone()
     fresh = torch.ones(n, dtype=torch.bool, device=dev) if fresh is None else fresh
     rows, start = [], state.clone()
     for _ in range(T):

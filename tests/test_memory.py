@@ -140,3 +140,28 @@ def test_rollout_and_update_on_the_simulator():
     assert stats["ent"] > 0 and any(not torch.equal(a, b) for a, b in zip(before, model.parameters()))
     data = collect_memory(sim, model, bot, T, data["state"], data["fresh"])
     assert torch.isfinite(data["logp"]).all()
+
+
+def test_a_rollout_keeps_its_state_when_the_next_goes_on_from_it():
+    """What collect_memory was given and has returned stays as it is: the same
+    state can be collected from twice, and a rollout's last state is that of its
+    own unroll after the next rollout too."""
+    from qqt_b200 import scenarios
+    from qqt_b200.bots import make_bot
+    from qqt_b200.config import SimConfig
+    from qqt_b200.sim import B200Sim
+    torch.manual_seed(0)
+    n = 64
+    cfg = SimConfig(**scenarios.CFG2)
+    sim = B200Sim(cfg, n, seed=1, template=scenarios.corridor_template(cfg, n, 1))
+    bot = make_bot(sim, "random")
+    sim.observe_and_mask()
+    model = MemoryActorCritic(local_features(sim, 0).shape[1], 32).cuda()
+    first = collect_memory(sim, model, bot, 5)
+    kept = {k: v.clone() for k, v in first.items()}
+    for _ in range(2):
+        again = collect_memory(sim, model, bot, 5, first["state"], first["fresh"])
+        assert torch.equal(again["start"], kept["state"])
+        assert not torch.equal(again["state"], kept["state"])
+    for k, v in kept.items():
+        assert torch.equal(first[k], v), k
