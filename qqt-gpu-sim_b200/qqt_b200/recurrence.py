@@ -22,6 +22,7 @@ import ctypes
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _capi as capi
 
@@ -203,4 +204,6 @@ def gated_recurrence_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tens
         if rc == 1 and state_out is not None:      # (the entry's one refusal left)
             raise ValueError("state_out overlaps an operand")
         capi.check(rc, "qqt_recurrence_step")
+    if state_out is not None:
+        increment_version(out)             # autograd learns of the write
     return h, out

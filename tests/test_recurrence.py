@@ -464,3 +464,28 @@ def test_state_out_in_every_allowed_place():
     state = fresh[:size].view(n, d)
     with pytest.raises(ValueError, match="overlap"):
         gated_recurrence_step(state, state, state, state_out=fresh[d:d + size].view(n, d))
+
+
+def test_autograd_learns_of_a_state_written_in_place(monkeypatch):
+    """A graph that saved the state before the tick refuses its backward pass
+    instead of using the new one; the library is replaced by one that does
+    nothing."""
+    from qqt_b200 import _capi
+
+    class Lib:
+        qqt_recurrence_step = staticmethod(lambda *a: 0)
+
+    monkeypatch.setattr(_capi, "lib", lambda: Lib)
+    monkeypatch.setattr(_capi, "launch_stream", lambda *a: 0)
+    x, state = torch.zeros(3, 4), torch.ones(3, 4)
+    w = torch.ones(3, 4, requires_grad=True)
+    loss = (w * state).sum()
+    gated_recurrence_step(x, x, state)
+    loss.backward()                                 # nothing was written over
+    loss = (w * state).sum()
+    gated_recurrence_step(x, x, state, state_out=state)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        s = torch.ones(3, 4)
+        assert gated_recurrence_step(x, x, s, state_out=s)[1] is s
