@@ -309,3 +309,50 @@ def test_variance_beyond_float32_and_of_zero(d, dtype):
     assert r0[1] == 0 and r0[3] == float("inf") and y0[3].isnan().all()
     for r in (0, 2, 4):
         assert torch.equal(y[r], want[0][r]) and torch.isfinite(y0[r]).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,d", [(70, 8), (3001, 64), (999, 200), (700, 512), (300, 1352),
+                                 (500, 2704), (60, 8192), (9, 14084), (7, 16384)])
+def test_backward_of_whole_vectors_at_odd_places(n, d, dtype):
+    """Rows made of whole 16-byte vectors whose strides or addresses are not on
+    16 bytes, x's and dy's differing: the values of the aligned tensors, bit for
+    bit, which are held to float64."""
+    _need_cuda()
+    x, w, b, dy = _data(n, d, dtype, n + d)
+    x, dy = x.contiguous(), dy.contiguous()
+    y, mean, rstd = layer_norm_forward(x, w, b, EPS)
+    want = layer_norm_backward(dy, x, mean, rstd, w)
+    ry, my, rx, mx, rw, mw, rb, mb = _ref(x, w, b, dy)
+    _close(y, ry, my, dtype)
+    _close(want[0], rx, mx, dtype)
+    _close(want[1], rw, mw, torch.float32)
+    _close(want[2], rb, mb, torch.float32)
+    for xo, xp, yo, yp in ((1, 1, 0, 0), (0, 0, 3, 5), (5, 11, 2, 3), (0, 1, 0, 1)):
+        wx = torch.full((n, d + xp + xo), float("nan"), dtype=dtype, device="cuda")
+        wy = torch.full((n, d + yp + yo), float("nan"), dtype=dtype, device="cuda")
+        wx[:, xo:xo + d], wy[:, yo:yo + d] = x, dy
+        vx, vy = wx[:, xo:xo + d], wy[:, yo:yo + d]
+        f = layer_norm_forward(vx, w, b, EPS)
+        assert all(torch.equal(p, q) for p, q in zip(f, (y, mean, rstd)))
+        got = layer_norm_backward(vy, vx, mean, rstd, w)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    wo = torch.empty(d + 1, device="cuda")[1:].copy_(w)      # the weight off 16 bytes
+    got = layer_norm_backward(dy, x, mean, rstd, wo)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@gpu
+@pytest.mark.parametrize("n,d", [(300, 14080), (301, 14081), (200, 14084), (9, 16383), (300, 16384)])
+def test_float32_rows_where_the_plan_changes(n, d):
+    """Two stages of x and dy no longer fit beside 14,080 float32 values a row."""
+    _need_cuda()
+    x, w, b, dy = _data(n, d, torch.float32, d)
+    y, mean, rstd = layer_norm_forward(x, w, b, EPS)
+    dx, dw, db = layer_norm_backward(dy, x, mean, rstd, w)
+    ry, my, rx, mx, rw, mw, rb, mb = _ref(x, w, b, dy)
+    _close(y, ry, my, torch.float32)
+    _close(dx, rx, mx, torch.float32)
+    _close(dw, rw, mw, torch.float32)
+    _close(db, rb, mb, torch.float32)

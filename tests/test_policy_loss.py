@@ -519,3 +519,47 @@ def test_advantage_of_zero_beside_a_ratio_beyond_float32(v, heads):
     stats, _, dz = policy_loss_and_grad(d["logits"], d["actions"], d["old_logp"], d["adv"],
                                         heads=heads, **opt)
     assert stats[1].isnan() and dz[2].isnan().all() and torch.isfinite(dz[5]).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,v,heads", [(50, 7, [5, 2]), (300, 120, [100, 20]), (20, 3000, None),
+                                       (6, 40001, None)])
+def test_autograd_in_16_bits(n, v, heads, dtype):
+    """The autograd loss and its scaled gradient against float64 (the scale's
+    product is one more rounding), the scaled loss as mixed precision trains."""
+    _need_cuda()
+    d = _data(n, v, heads, dtype, n + v, legal=True)
+    scale = 64.0 * n
+    want = _ref(d, OPT, scale)
+    z = d["logits"].clone().requires_grad_(True)
+    loss, stats = policy_loss(z, d["actions"], d["old_logp"], d["adv"], d["ref_logp"], d["legal"],
+                              d["mask"], heads, **OPT)
+    (scale * loss).backward()
+    assert z.grad.dtype == dtype and loss.dtype == torch.float32
+    tol = want["tol"].max().item()
+    terms = want["row_terms"].mean().item()
+    assert bool(((stats.double() - want["stats"]).abs() <= 4 * tol * (1 + terms)).all())
+    err = (z.grad.double() - want["dlogits"]).abs()
+    lim = UNIT[dtype] * want["dlogits"].abs() + want["coef"] * tol + 2.0 ** -25
+    assert bool((err <= lim).all()), (err - lim).max().item()
+
+
+@gpu
+@pytest.mark.parametrize("n,v", [(1000003, 40), (300007, 64)])
+def test_many_rows_of_moderate_width(n, v):
+    """Means over a million rows: a thread adds n / 1024 of the rows' terms one
+    after the other and trees the rest, so a sum is off by at most (n / 1024 + 20)
+    2^-24 of its terms' magnitudes, besides the rows' own errors."""
+    _need_cuda()
+    d = _data(n, v, None, torch.float32, 71)
+    want = _ref(d, OPT)
+    stats, logp, dz = policy_loss_and_grad(d["logits"], d["actions"], d["old_logp"], d["adv"],
+                                           d["ref_logp"], None, d["mask"], **OPT)
+    assert bool(((logp.double() - want["logp"]).abs() <= want["tol"]).all())
+    bound = (want["row_terms"] * (4 * want["tol"] + (n / 1024 + 20) * 2.0 ** -24)).mean().item()
+    assert bool(((stats.double() - want["stats"]).abs() <= bound / 0.7).all()), \
+        (stats, want["stats"], bound)
+    err = (dz.double() - want["dlogits"]).abs()
+    lim = UNIT[torch.float32] * want["dlogits"].abs() + want["coef"] * want["tol"][:, None]
+    assert bool((err <= lim).all())
