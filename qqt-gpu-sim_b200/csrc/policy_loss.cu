@@ -147,6 +147,12 @@ __device__ __forceinline__ float finish_head(HeadStat& k, bool any, float s, flo
   return any && act_ok ? t_act - log_s : -INFINITY;
 }
 
+// The heads' sum, in which a head without a value (-inf) stays: added to
+// another's NaN it would be NaN, and the row would count as live.
+__device__ __forceinline__ float add_logp(float sum, float head) {
+  return sum == -INFINITY || head == -INFINITY ? -INFINITY : sum + head;
+}
+
 // The gradient at a logit that is not the action's, with p = e / S:
 // scale (p (c (log p + H) - G)) = scale e (c_s t + k_s); the terms that may
 // cancel are added before the scale.  At the action's:
@@ -300,7 +306,6 @@ __global__ void __launch_bounds__(kPlSmallRows, 8)
   HeadStat hs[NH];
   float ms[NH];
   float logp = 0.f, ent = 0.f;
-  bool dead = !on;                       // some head gives the action no value
   if (on) {
     int at = 0;
 #pragma unroll(NH <= 2 ? NH : 1)
@@ -322,15 +327,13 @@ __global__ void __launch_bounds__(kPlSmallRows, 8)
       k.act = in ? at + (int)act : -1;
       const float za = in ? z[at + act] : -INFINITY;
       const float lh = finish_head(k, m != -INFINITY, s, logf(s), e, za - m, za != -INFINITY);
-      logp += lh;
-      dead |= lh == -INFINITY || logp == -INFINITY;
+      logp = add_logp(logp, lh);
       k.t_act = za == -INFINITY ? 0.f : za - m;
       ms[h] = m;
       ent += k.ent;
       hs[h] = k;
       at += w;
     }
-    if (dead) logp = -INFINITY;          // (another head's NaN would hide it in the sum)
     if (a.logp) a.logp[r] = logp;
     if (a.entropy) a.entropy[r] = ent;
   }
@@ -338,7 +341,7 @@ __global__ void __launch_bounds__(kPlSmallRows, 8)
   if (fold) __syncthreads();
   before_me_done();
   const float count = fold ? fmaxf((float)n_mask, 1.f) : rows_counted(a, counts);
-  const bool live = !dead && row.counts;
+  const bool live = on && logp != -INFINITY && row.counts;
   const RowLoss l = loss_of(a, row, logp, live);
   if (a.stats) {
     const float v[4] = {l.pg, l.kl, live ? ent : 0.f, l.clip};
@@ -814,7 +817,6 @@ __global__ void __launch_bounds__(kPlThreads, kPlThreads == 512 ? 2 : 1)
   HeadStat hs[QQT_MAX_HEADS];
   float refs[QQT_MAX_HEADS];
   unsigned plain = 0;                    // heads whose sums are against the maximum itself
-  bool dead = false;                     // some head gives the action no value
   float logp = 0.f, ent = 0.f;
   int at = 0;
 #pragma unroll 1
@@ -881,19 +883,17 @@ __global__ void __launch_bounds__(kPlThreads, kPlThreads == 512 ? 2 : 1)
       lp = finish_head(k, any, q.s, log2f(q.s) * kLn2, q.e * kLn2, ta, z_act != -INFINITY);
       refs[h] = q.r;
     }
-    logp += lp;
-    dead |= lp == -INFINITY || logp == -INFINITY;
+    logp = add_logp(logp, lp);
     ent += k.ent;
     hs[h] = k;
     at += w;
   }
-  if (dead) logp = -INFINITY;            // (another head's NaN would hide it in the sum)
   if (lead) {
     if (a.logp) a.logp[r] = logp;
     if (a.entropy) a.entropy[r] = ent;
   }
   if (!a.old_logp) return;
-  const bool live = !dead && in.counts;
+  const bool live = logp != -INFINITY && in.counts;
   const RowLoss l = loss_of(a, in, logp, live);
   if (a.stats && lead)
     *reinterpret_cast<float4*>(part + r * 4) =
