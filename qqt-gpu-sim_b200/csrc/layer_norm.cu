@@ -19,11 +19,11 @@
 // again for every pass.
 //
 // Measured on a B200 (its copy bandwidth is 6.55 TB/s):
-//   1048576 x 128 f32    forward 171 us, 6.3 TB/s; backward 252 us, 6.4 TB/s
-//   5632 x 10816 f16     forward 56 us, 4.3 TB/s; backward 112 us, 3.3 TB/s
-//   11267 x 2704 bf16    forward 30 us, 4.1 TB/s; backward 58 us, 3.2 TB/s
+//   1048576 x 128 f32    forward 172 us, 6.2 TB/s; backward 253 us, 6.4 TB/s
+//   5632 x 10816 f16     forward 57 us, 4.3 TB/s; backward 102 us, 3.6 TB/s
+//   11267 x 2704 bf16    forward 30 us, 4.0 TB/s; backward 56 us, 3.3 TB/s
 //   40000 x 512 f32      forward 32 us, 5.1 TB/s; backward 48 us, 5.1 TB/s
-//   20000 x 1351 bf16    forward 56 us, 1.9 TB/s; backward 111 us, 1.5 TB/s
+//   20000 x 1351 bf16    forward 57 us, 1.9 TB/s; backward 111 us, 1.5 TB/s
 // Short rows are bound by memory.  Rows of a block, 16-bit ones above all, are
 // bound by what each row costs its block beside the memory: two exchanges
 // across the warps forward and one of two sums backward, with 24 warps an SM

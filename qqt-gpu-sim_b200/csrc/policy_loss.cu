@@ -26,16 +26,18 @@
 //    sum, does not depend on alignment.
 //
 // Measured on a B200 (copy bandwidth 6.55 TB/s):
-//   8192 x 32000 bf16     loss and gradient 228 us, 4.6 TB/s (two values a
+//   8192 x 32000 bf16     loss and gradient 225 us, 4.7 TB/s (two values a
 //                         logit); scores 113 us, 4.6 TB/s
-//   2047 x 100003 f16     loss and gradient 287 us, 2.9 TB/s; scores 107 us, 3.8
+//   2047 x 100003 f16     loss and gradient 290 us, 2.8 TB/s; scores 107 us, 3.8
 //                         TB/s (rows at any alignment)
-//   4096 x 32000 f32      loss and gradient 212 us, 4.9 TB/s
+//   4096 x 32000 f32      loss and gradient 209 us, 5.0 TB/s; scores 101 us, 5.2
+//   1048576 x 64 f32      loss and gradient 441 us, 163 of them k_pl_stats, one
+//                         block that adds a partial sum per row; scores 134 us
 //   1048576 rows of 5 + 2 f32 logits, masked: 39 us, 2.6 TB/s; 86 % of the
 //                         issue slots (900 instructions a row: logarithms,
 //                         exponentials and quotients of both heads and of the
 //                         loss)
-// The vocabulary rows execute about 9 instructions a logit and pass, 60 % of
+// The vocabulary rows execute about 9 instructions a logit and pass, 64 % of
 // the issue slots, 57 % of the special-function unit and 70 % of the memory
 // bandwidth at once; no one of them is full.
 
@@ -679,7 +681,7 @@ __device__ __forceinline__ void put_grads(T* p, int sh, int j, int w, bool on,
 
 // The same where all of the warp's vectors lie whole in the row and sh > 0.  The
 // first lane's part of the word it shares goes out in pieces of 2, 4 and 8
-// bytes, and so does the last lane's (2047 x 100003 f16: 287 us, 340 value by
+// bytes, and so does the last lane's (2047 x 100003 f16: 290 us, 340 value by
 // value).
 template <class T, int VEC>
 __device__ __forceinline__ void put_inner(T* p, int sh, int j, const Vec<T, VEC>& x) {

@@ -25,10 +25,10 @@
 //
 // Measured on a B200 (copy bandwidth 6.55 TB/s), bytes of the sequences alone:
 //   128 ticks x 5632 x 128   f32: forward 183 us, 6.05 TB/s, backward 288 us,
-//                            6.4 TB/s; bf16: 104 us, 5.3 TB/s, and 207 us, 4.4
-//   65536 x 1024 bf16        forward 109 us (segment sums 40, join 8, walk 62),
-//                            backward 169 us
-//   10007 x 3 x 517 f32      forward 62 us, backward 91 us, 4-byte loads
+//                            6.4 TB/s; bf16: 105 us, 5.3 TB/s, and 210 us, 4.4
+//   65536 x 1024 bf16        forward 110 us (segment sums 40, join 8, walk 62),
+//                            backward 174 us
+//   10007 x 3 x 517 f32      forward 67 us, backward 97 us, 4-byte loads
 // 32-bit sequences are bound by memory.  The 16-bit backward walk is bound by
 // the loads it has in flight: 128 registers leave 16 warps an SM, each with 24
 // 4-byte loads a lane (100 M warp instructions at an IPC of 0.45).

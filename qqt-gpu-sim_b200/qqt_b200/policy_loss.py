@@ -10,8 +10,10 @@ csrc/policy_loss.cu, straight from the logits: no log-softmax is stored.
 (train/ppo.py:397-424, train/model.py:216-256).  logits (N, V) are float32,
 float16 or bfloat16; `heads` splits V into independent categorical heads
 ((5, 2): the moves and the bomb), one head by default.  A row without a
-legal category in some head, or whose action is not legal, has logp -inf and
-adds nothing to the sums or the gradient.
+legal category in some head, or whose action is illegal or outside its head,
+has logp -inf and adds nothing to the sums or the gradient, whatever its
+other heads hold; an action outside its head also sets the device error word,
+unless the mask leaves its row out.
 
 `policy_loss` is differentiable in the logits.  `policy_loss_and_grad` gives
 loss and gradient in one pass over the logits, for `logits.backward(dlogits)`.
