@@ -711,8 +711,10 @@ extern "C" int qqt_recurrence_step(const void* x, int64_t x_stride, const void* 
   if (!x || !gate || !state || !h || !state_out) return QQT_E_ARG;
   const int64_t es = dtype == QQT_F32 ? 4 : 2, out = N * D * 4;
   if (rec_clash(state_out, out, state, N, D * 4, D * 4, true) ||
-      rec_clash(state_out, out, x, N, x_stride * es, D * es, es == 4 && x_stride == D) ||
-      rec_clash(state_out, out, gate, N, gate_stride * es, D * es, es == 4 && gate_stride == D) ||
+      rec_clash(state_out, out, x, N, x_stride * es, D * es,
+                es == 4 && (N == 1 || x_stride == D)) ||
+      rec_clash(state_out, out, gate, N, gate_stride * es, D * es,
+                es == 4 && (N == 1 || gate_stride == D)) ||
       rec_clash(state_out, out, reset, N, reset_stride, 1, false) ||
       rec_clash(state_out, out, h, N, D * es, D * es, false))
     return QQT_E_ARG;

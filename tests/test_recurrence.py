@@ -489,3 +489,15 @@ def test_autograd_learns_of_a_state_written_in_place(monkeypatch):
     with torch.inference_mode():
         s = torch.ones(3, 4)
         assert gated_recurrence_step(x, x, s, state_out=s)[1] is s
+
+
+@gpu
+def test_state_out_over_the_one_row_of_a_wider_tensor():
+    """With one sequence a row's stride is any: x's own place is allowed."""
+    _need_cuda()
+    wide = torch.randn((1, 40), device="cuda")
+    x, g, s = wide[:, :16], torch.randn((1, 16), device="cuda"), torch.randn((1, 16), device="cuda")
+    assert x.stride(0) == 40
+    want = gated_recurrence_step(x, g, s)
+    got = gated_recurrence_step(x, g, s, state_out=x)
+    assert all(torch.equal(p, q) for p, q in zip(got, want)) and torch.equal(wide[:, :16], want[1])
